@@ -538,6 +538,115 @@ GS3D_API int gs3d_opacity_reset(
     const gs3d_gaussians* gaussians, const gs3d_adam_moments* moments,
     float max_opacity, gs3d_stream_t stream);
 
+/* ---- compressed SH coefficients (no counterpart in the reference, which keeps 4 (d+1)^2 3 bytes
+ * per Gaussian): rows shared through a table, with the table's gradient, and rows in microscaled
+ * 4-bit floating point, with the colours a render takes from them. */
+
+/* Element types of gs3d_rows. */
+#define GS3D_F32 0
+#define GS3D_F16 1
+#define GS3D_BF16 2
+
+/* `rows` rows of `dim` elements; row r starts at element r * row_stride of data (row_stride >= dim;
+ * data aligned to its elements). Rows of SH coefficients have dim = 3 (d+1)^2, channel by channel,
+ * as sh_coeffs holds them. */
+typedef struct gs3d_rows {
+    int64_t rows;
+    int64_t row_stride;
+    int32_t dim;
+    int32_t type;
+    void* data;
+} gs3d_rows;
+
+/* out[i] = scale * table[indices[i]] for every row i of out (1-based indices, out->rows of them;
+ * an index outside 1 .. table->rows gives a row of zeros). Products are formed in fp32 and rounded
+ * once to out's type. out and table have the same dim and do not overlap. */
+GS3D_API int gs3d_table_lookup(const gs3d_rows* table, const int32_t* indices, float scale,
+                               const gs3d_rows* out, gs3d_stream_t stream);
+
+/* table gradient flags */
+#define GS3D_TABLE_ACCUMULATE 1u /* add to table_grads instead of overwriting them */
+
+/* Bytes of workspace gs3d_table_gradient needs for at most grad_rows rows of gradients of dim
+ * elements and a table of table_rows rows. */
+GS3D_API int gs3d_table_gradient_workspace_size(int64_t grad_rows, int64_t table_rows, int32_t dim,
+                                                size_t* bytes);
+
+/* The gradient of gs3d_table_lookup: table_grads[k] = scale * sum of grads[f] over the rows f whose
+ * index is k + 1, summed in fp32 in an order that depends on the indices alone (equal inputs give
+ * equal bits). Rows of the table that no index names get zeros.
+ *   fgidx_to_gidx == NULL: row f has index indices[f] (grads->rows indices).
+ *   fgidx_to_gidx != NULL: row f belongs to filtered Gaussian f, as gs3d_backward writes
+ *     sh_coeffs_grads: its index is indices[fgidx_to_gidx[f] - 1] (n_indices indices; entries
+ *     outside 1 .. n_indices are skipped).
+ * device_counts != NULL: only the first device_counts[0] rows take part (read on the device,
+ * clamped to grads->rows); the others are not read. Indices outside 1 .. table_grads->rows are
+ * skipped. table_grads is GS3D_F32. The workspace (256-byte aligned) is scratch for this call. */
+GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices, int64_t n_indices,
+                                 const int32_t* fgidx_to_gidx, const int32_t* device_counts,
+                                 float scale, const gs3d_rows* table_grads, uint32_t flags,
+                                 void* workspace, size_t workspace_bytes, gs3d_stream_t stream);
+
+/* Microscaled 4-bit rows. An element is a sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (e2m1); a block
+ * of consecutive elements of a row shares a scale (the last block of a row may be short).
+ *   GS3D_NVFP4: blocks of 16, e4m3 block scales, one fp32 scale for all rows (*tensor_scale in
+ *     device memory, within 2^-100 .. 2^100): value = element * block scale * tensor scale,
+ *     rounded once to fp32.
+ *   GS3D_MXFP4: blocks of 32, power-of-two block scales (e8m0: 2^(byte - 127)): value = element *
+ *     block scale. tensor_scale is not read.
+ * codes: (dim + 1) / 2 bytes per row, element 2 j in the low and 2 j + 1 in the high 4 bits of byte
+ * j (0 where the row has no element 2 j + 1); scales: one byte per block, ceil(dim / block) per row.
+ * Rows are contiguous. A scale byte of NaN (e4m3 0x7f, e8m0 0xff) makes the block's values NaN. */
+#define GS3D_NVFP4 0
+#define GS3D_MXFP4 1
+
+typedef struct gs3d_mx4_rows {
+    int64_t rows;
+    int32_t dim;
+    int32_t format;
+    uint8_t* codes;
+    uint8_t* scales;
+    const float* tensor_scale;
+} gs3d_mx4_rows;
+
+/* tensor_scale[0] = max(largest finite |x| / (6 * 448), 2^-100): the GS3D_NVFP4 tensor scale with
+ * which no block scale of x saturates. */
+GS3D_API int gs3d_mx4_tensor_scale(const gs3d_rows* x, float* tensor_scale, gs3d_stream_t stream);
+
+/* Quantise x into `out` (same rows and dim). Per block with largest magnitude a: GS3D_NVFP4 block
+ * scale = a / (6 tensor scale) rounded to the nearest e4m3 value, ties to even, at most 448;
+ * GS3D_MXFP4 block scale = 2^(floor(log2 a) - 2), at least 2^-127. Elements are the quotients by
+ * the block's scale rounded to the nearest element, ties to the even code, magnitudes above 6 to 6.
+ * Every rounding decision is that of the exact quotient. A block with a NaN gets a NaN scale;
+ * infinities keep their sign and become the block's largest magnitude (in GS3D_MXFP4 an infinite
+ * value again). */
+GS3D_API int gs3d_mx4_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, gs3d_stream_t stream);
+
+/* out = the values x stands for, rounded to out's type (same rows and dim). */
+GS3D_API int gs3d_mx4_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, gs3d_stream_t stream);
+
+/* The colours of n Gaussians from 4-bit SH rows, seen from n_views cameras (view_positions: HOST
+ * memory, 3 floats per view, 1 .. GS3D_MAX_FACTORED_VIEWS views): gs3d_shard_colours with the
+ * coefficients gs3d_mx4_dequantise (fp32) gives for row i, or with indices != NULL for row
+ * indices[i] (1-based; outside 1 .. sh->rows: coefficients 0), bit for bit, without writing them.
+ * sh->dim = 3 (d+1)^2 with d >= sh_degree; means4: 4 x n, the first three floats the mean (16-byte
+ * aligned, as means_opacity_features / means_opacities). Float4 row v * view_stride + i of colours
+ * (16-byte aligned), w = 0. */
+GS3D_API int gs3d_mx4_colours(const gs3d_mx4_rows* sh, int32_t sh_degree, const int32_t* indices,
+                              const float* means4, int32_t n, const float* view_positions,
+                              int32_t n_views, float* colours, int64_t view_stride,
+                              gs3d_stream_t stream);
+
+/* gs3d_render_forward_render_only with the SH coefficients of 4-bit rows (row i, or row indices[i]
+ * as in gs3d_mx4_colours): gaussians->sh_coeffs is not read and may be NULL, gaussians->sh_degree is
+ * the degree of sh->dim. The outputs equal those of gs3d_render_forward_render_only on the
+ * dequantised coefficients bit for bit. */
+GS3D_API int gs3d_render_forward_mx4(
+    const gs3d_render_outputs* outputs, const gs3d_render_only_gaussians* gaussians,
+    const gs3d_mx4_rows* sh, const int32_t* indices, const gs3d_camera* camera,
+    const gs3d_tiling* tiling, const gs3d_render_options* options, gs3d_render_buffers* buffers,
+    int32_t* host_counts, uint32_t flags, gs3d_stream_t stream);
+
 /* ---- misc ---------------------------------------------------------------------------- */
 GS3D_API const char* gs3d_last_error_string(void);
 GS3D_API int gs3d_version(void);
@@ -545,7 +654,8 @@ GS3D_API int gs3d_version(void);
 /* Stage timers (no counterpart in the reference beyond its GUI render timer, gui.jl:358-373):
  * when enabled, every entry point records CUDA events on its stream around each stage
  * (keep_compact, project, dup_scan, dup_keys, sort, tiles_end, raster, zero_2d, bwd_raster,
- * bwd_project, adam, loss, adc_stats). Enabling (or disabling) clears earlier records.
+ * bwd_project, adam, loss, adc_stats, table_lookup, table_grad, mx4_quantise, mx4_colours).
+ * Enabling (or disabling) clears earlier records.
  * gs3d_profile_report waits for the recorded events and writes "stage launches total_ms"
  * lines. Host-thread unsafe; for measurement runs. */
 GS3D_API int gs3d_profile_enable(int enable);

@@ -1,0 +1,217 @@
+"""Compressed SH coefficients without a GPU: the C entry points' refusals (every call below is turned
+down before it touches the device) and the Python layer's checks."""
+import ctypes as C
+
+import pytest
+import torch
+
+from gs3d import CompressedGaussiansVector, MX4Rows, _abi
+from gs3d import compressed as gc
+
+LIB = _abi.lib()
+DATA = 0x10000  # never read: the calls are refused, or have nothing to do
+BIG = 1 << 40
+
+
+def rows(n=4, dim=48, stride=None, kind=_abi.GS3D_F32, data=DATA):
+    return _abi.RowsC(n, dim if stride is None else stride, dim, kind, data)
+
+
+def mx4(n=4, dim=48, fmt=_abi.GS3D_NVFP4, codes=DATA, scales=DATA, ts=DATA):
+    return _abi.MX4RowsC(n, dim, fmt, codes, scales, ts)
+
+
+def refused(status, *words):
+    assert status == _abi.GS3D_ERR_INVALID_ARGUMENT, status
+    msg = LIB.gs3d_last_error_string().decode()
+    for w in words:
+        assert w in msg, msg
+
+
+BAD_ROWS = [(dict(n=-1), "rows"), (dict(n=BIG), "rows"), (dict(dim=0), "dim"), (dict(dim=1 << 17), "dim"),
+            (dict(stride=47), "stride"), (dict(kind=3), "type"), (dict(data=None), "NULL"),
+            (dict(data=DATA + 2), "aligned"), (dict(kind=_abi.GS3D_BF16, data=DATA + 1), "aligned")]
+
+
+@pytest.mark.parametrize("bad,word", BAD_ROWS)
+def test_bad_rows_are_refused_everywhere(bad, word):
+    r, ok, q = rows(**bad), rows(), mx4()
+    refused(LIB.gs3d_table_lookup(C.byref(r), DATA, 1.0, C.byref(ok), None), word)
+    refused(LIB.gs3d_table_lookup(C.byref(ok), DATA, 1.0, C.byref(r), None), word)
+    refused(LIB.gs3d_table_gradient(C.byref(r), DATA, 4, None, None, 1.0, C.byref(ok), 0, DATA, BIG, None), word)
+    refused(LIB.gs3d_table_gradient(C.byref(ok), DATA, 4, None, None, 1.0, C.byref(r), 0, DATA, BIG, None), word)
+    refused(LIB.gs3d_mx4_tensor_scale(C.byref(r), DATA, None), word)
+    refused(LIB.gs3d_mx4_quantise(C.byref(r), C.byref(q), None), word)
+    refused(LIB.gs3d_mx4_dequantise(C.byref(q), C.byref(r), None), word)
+
+
+def test_lookup_refusals():
+    t = rows()
+    refused(LIB.gs3d_table_lookup(None, DATA, 1.0, C.byref(t), None), "NULL")
+    refused(LIB.gs3d_table_lookup(C.byref(t), DATA, 1.0, None, None), "NULL")
+    refused(LIB.gs3d_table_lookup(C.byref(t), None, 1.0, C.byref(rows()), None), "NULL")
+    refused(LIB.gs3d_table_lookup(C.byref(t), DATA, 1.0, C.byref(rows(dim=47)), None), "dim")
+    # nothing to do: no launch, no error
+    assert LIB.gs3d_table_lookup(C.byref(t), None, 1.0, C.byref(rows(n=0, data=None)), None) == _abi.GS3D_OK
+
+
+def test_gradient_refusals():
+    g, t = rows(), rows(n=7)
+
+    def call(g=g, idx=DATA, n_idx=4, f2g=None, t=t, flags=0, ws=DATA, nbytes=BIG):
+        return LIB.gs3d_table_gradient(C.byref(g), idx, n_idx, f2g, None, 1.0, C.byref(t), flags, ws, nbytes, None)
+
+    refused(call(t=rows(n=7, dim=12)), "dim")
+    refused(call(t=rows(n=7, kind=_abi.GS3D_BF16)), "GS3D_F32")
+    refused(call(flags=2), "flags")
+    refused(call(n_idx=3), "3 indices for 4 rows")
+    refused(call(n_idx=-1, f2g=DATA), "indices")
+    refused(call(idx=None), "NULL indices")
+    refused(call(ws=DATA + 128), "aligned")
+    size = C.c_size_t(0)
+    _abi.check(LIB.gs3d_table_gradient_workspace_size(4, 7, 48, C.byref(size)))
+    assert call(nbytes=size.value - 1) == _abi.GS3D_ERR_WORKSPACE
+    assert call(ws=None) == _abi.GS3D_ERR_WORKSPACE
+    assert call(t=rows(n=0, data=None)) == _abi.GS3D_OK
+    refused(LIB.gs3d_table_gradient_workspace_size(4, 7, 48, None), "NULL")
+    for bad in ((-1, 7, 48), (BIG, 7, 48), (4, -1, 48), (4, BIG, 48), (4, 7, 0)):
+        refused(LIB.gs3d_table_gradient_workspace_size(*bad, C.byref(size)))
+
+
+def test_gradient_workspace_grows_with_the_rows():
+    size, last = C.c_size_t(0), 0
+    for n in (0, 1, 1000, 100_000, 3_000_000, 1 << 30):
+        _abi.check(LIB.gs3d_table_gradient_workspace_size(n, 65_536, 48, C.byref(size)))
+        assert size.value >= max(last, 4 * n)
+        last = size.value
+
+
+@pytest.mark.parametrize("bad,word", [(dict(n=-1), "rows"), (dict(n=BIG), "rows"), (dict(dim=0), "dim"),
+                                      (dict(fmt=2), "format"), (dict(codes=None), "NULL"),
+                                      (dict(scales=None), "NULL"), (dict(ts=None), "NULL tensor scale")])
+def test_bad_mx4_rows_are_refused_everywhere(bad, word):
+    q, x = mx4(**bad), rows()
+    refused(LIB.gs3d_mx4_quantise(C.byref(x), C.byref(q), None), word)
+    refused(LIB.gs3d_mx4_dequantise(C.byref(q), C.byref(x), None), word)
+    pos = (C.c_float * 3)()
+    refused(LIB.gs3d_mx4_colours(C.byref(q), 0, None, DATA, 4, pos, 1, DATA, 4, None), word)
+
+
+def test_quantise_refusals():
+    refused(LIB.gs3d_mx4_quantise(C.byref(rows(n=5)), C.byref(mx4()), None), "5 rows")
+    refused(LIB.gs3d_mx4_dequantise(C.byref(mx4(dim=47)), C.byref(rows()), None), "47")
+    refused(LIB.gs3d_mx4_tensor_scale(C.byref(rows()), None, None), "NULL")
+    empty = mx4(n=0, codes=None, scales=None, fmt=_abi.GS3D_MXFP4, ts=None)
+    assert LIB.gs3d_mx4_quantise(C.byref(rows(n=0, data=None)), C.byref(empty), None) == _abi.GS3D_OK
+    assert LIB.gs3d_mx4_dequantise(C.byref(empty), C.byref(rows(n=0, data=None)), None) == _abi.GS3D_OK
+
+
+def test_colour_refusals():
+    pos = (C.c_float * 3)()
+
+    def call(q=mx4(), deg=3, idx=None, means=DATA, n=4, p=pos, views=1, out=DATA, stride=4):
+        return LIB.gs3d_mx4_colours(C.byref(q), deg, idx, means, n, p, views, out, stride, None)
+
+    refused(call(q=mx4(dim=47)), "47")
+    refused(call(deg=-1), "degree")
+    refused(call(deg=3, q=mx4(dim=27)), "degree")
+    refused(call(n=5, stride=5), "4 4-bit SH rows for 5 Gaussians")
+    refused(call(n=-1), "-1")
+    refused(call(means=None), "NULL")
+    refused(call(out=None), "NULL")
+    refused(call(p=None), "NULL")
+    refused(call(views=0), "views")
+    refused(call(views=_abi.GS3D_MAX_FACTORED_VIEWS + 1), "views")
+    refused(call(stride=3), "stride")
+    refused(call(means=DATA + 4), "aligned")
+    refused(call(out=DATA + 8), "aligned")
+    assert call(n=0, means=None, out=None, stride=0) == _abi.GS3D_OK
+
+
+def test_render_refusals():
+    cam, til, opt = _abi.Camera(), _abi.TilingC(), _abi.RenderOptionsC()
+    out, buf = _abi.RenderOutputsC(), _abi.RenderBuffersC()
+    cam.width = cam.height = 16
+    cam.near_z, cam.far_z = 0.2, 100.0
+    til.tile_width = til.tile_height = 16
+    til.nb_tiles_x = til.nb_tiles_y = 1
+    opt.sh_degree = 3
+    ro = _abi.RenderOnlyGaussiansC(4, 3, DATA, DATA, None)
+
+    def call(ro=ro, q=mx4(), idx=None, flags=0):
+        return LIB.gs3d_render_forward_mx4(C.byref(out), C.byref(ro) if ro else None, C.byref(q) if q else None,
+                                           idx, C.byref(cam), C.byref(til), C.byref(opt), C.byref(buf), None,
+                                           flags, None)
+
+    refused(call(q=None), "NULL 4-bit")
+    refused(call(ro=None), "NULL Gaussians")
+    refused(call(q=mx4(dim=27)), "27")
+    refused(call(q=mx4(n=3)), "3 4-bit SH rows for 4 Gaussians")
+    refused(call(flags=_abi.GS3D_RENDER_DEFER_COLOUR), "DEFER_COLOUR")
+    opt.sh_degree = 2
+    refused(call(ro=_abi.RenderOnlyGaussiansC(4, 1, DATA, DATA, None), q=mx4(dim=12)), "degree")
+
+
+# -- the Python layer ---------------------------------------------------------------------------
+def test_mx4_rows_checks():
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
+    one = torch.ones(1)
+    q = MX4Rows(u8(5, 14), u8(5, 2), one, 27, "nvfp4")
+    assert (q.rows, q.nbytes) == (5, 5 * 16 + 4)
+    assert MX4Rows(u8(5, 14), u8(5, 1), None, 27, "mxfp4").rows == 5
+    for bad in ((u8(5, 13), u8(5, 2), one, 27, "nvfp4"), (u8(5, 14), u8(5, 1), one, 27, "nvfp4"),
+                (u8(5, 14), u8(4, 2), one, 27, "nvfp4"), (u8(5, 14), u8(5, 2), None, 27, "nvfp4"),
+                (u8(5, 14), u8(5, 2), one.double(), 27, "nvfp4"), (u8(5, 14), u8(5, 1), one, 27, "mxfp4"),
+                (u8(5, 14).char(), u8(5, 2), one, 27, "nvfp4"), (u8(5, 28)[:, ::2], u8(5, 2), one, 27, "nvfp4"),
+                (u8(5, 14), u8(5, 2), one, 27, "fp4")):
+        with pytest.raises(ValueError):
+            MX4Rows(*bad)
+    with pytest.raises(ValueError):
+        MX4Rows.empty(3, 48, "int4", "cpu")
+
+
+def test_compressed_gaussians_checks():
+    q = MX4Rows.empty(6, 48, "mxfp4", "cpu")
+    mo, cov, idx = torch.zeros(6, 4), torch.zeros(6, 6), torch.ones(6, dtype=torch.int32)
+    g = CompressedGaussiansVector(mo, cov, q)
+    assert g.n == 6 and g.sh_degree == 3 and g.to_c().sh_coeffs is None
+    assert CompressedGaussiansVector(mo, cov, MX4Rows.empty(2, 27, "mxfp4", "cpu"), idx).sh_degree == 2
+    for bad in ((mo[:5], cov, q), (mo, cov[:, :5], q), (mo.double(), cov, q), (mo[:5], cov[:5], q),
+                (mo, cov, MX4Rows.empty(6, 47, "mxfp4", "cpu")), (mo, cov, q, idx.long()), (mo, cov, q, idx[:5])):
+        with pytest.raises(ValueError):
+            CompressedGaussiansVector(*bad)
+
+
+def test_rows_of_a_tensor():
+    t = torch.zeros(5, 3, 16)
+    assert (lambda c: (c.rows, c.row_stride, c.dim, c.type))(gc._rows_c(t, "t")) == (5, 48, 48, _abi.GS3D_F32)
+    c = gc._rows_c(torch.zeros(5, 64, dtype=torch.bfloat16)[:, 3:30], "t")
+    assert (c.rows, c.row_stride, c.dim, c.type) == (5, 64, 27, _abi.GS3D_BF16)
+    assert gc._rows_c(torch.zeros(9, 4)[::3], "t").row_stride == 12
+    assert gc._rows_c(torch.zeros(0, 4), "t").rows == 0
+    for bad in (torch.zeros(5), torch.zeros(5, 4).double(), torch.zeros(4, 5).t(), torch.zeros(1, 4).expand(5, 4),
+                torch.zeros(5, 16, 3).transpose(1, 2)):
+        with pytest.raises(ValueError):
+            gc._rows_c(bad, "t")
+
+
+def test_calls_need_cuda_tensors_of_the_right_kind():
+    t, i = torch.zeros(4, 48), torch.ones(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        gc.table_lookup(t, i)
+    with pytest.raises(ValueError, match="int32"):
+        gc.table_lookup(t, i.long())
+    with pytest.raises(ValueError, match="int32"):
+        gc.table_gradient(t, i, 4, fgidx_to_gidx=i.long())
+    with pytest.raises(ValueError, match="CUDA"):
+        gc.table_gradient(t, i, 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        gc.mx4_quantise(t)
+    with pytest.raises(ValueError, match="CUDA"):
+        gc.mx4_dequantise(MX4Rows.empty(4, 48, "mxfp4", "cpu"))
+    with pytest.raises(ValueError, match="positions"):
+        gc.mx4_colours(MX4Rows.empty(4, 48, "mxfp4", "cpu"), torch.zeros(4, 4), [0.0, 0.0, 0.0], 3)
+    with pytest.raises(ValueError):
+        gc.SHTable(torch.zeros(4, 3, 5), i)
+    with pytest.raises(ValueError):
+        gc.fit_table(torch.zeros(4, 3, 16), 0)

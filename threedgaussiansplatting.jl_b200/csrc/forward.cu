@@ -10,6 +10,7 @@
 // F and D never leave the device unless the caller asks for them.
 #include "common.cuh"
 #include "internal.h"
+#include "sh_colour.cuh"
 
 namespace gs3d {
 
@@ -116,30 +117,6 @@ __global__ void __launch_bounds__(kChunkThreads) k_keep_downsweep(const uint8_t*
     }
 }
 
-// sh_coeffs_to_color (sh.jl:38-112) for one channel; hc = coefficient 1 of that channel
-template <int DEG>
-__device__ __forceinline__ float sh_channel(const float* hc, float x, float y, float z) {
-    float cc = sh_basis(1, x, y, z) * hc[0];
-    if (DEG >= 1) {
-        cc += (sh_basis(2, x, y, z) * hc[1] + sh_basis(3, x, y, z) * hc[2] +
-               sh_basis(4, x, y, z) * hc[3]);
-        if (DEG >= 2) {
-            cc += (sh_basis(5, x, y, z) * hc[4] + sh_basis(6, x, y, z) * hc[5] +
-                   sh_basis(7, x, y, z) * hc[6] + sh_basis(8, x, y, z) * hc[7] +
-                   sh_basis(9, x, y, z) * hc[8]);
-            if (DEG >= 3) {
-                cc += (sh_basis(10, x, y, z) * hc[9] + sh_basis(11, x, y, z) * hc[10] +
-                       sh_basis(12, x, y, z) * hc[11] + sh_basis(13, x, y, z) * hc[12] +
-                       sh_basis(14, x, y, z) * hc[13] + sh_basis(15, x, y, z) * hc[14] +
-                       sh_basis(16, x, y, z) * hc[15]);
-            }
-        }
-    }
-    cc += 0.5f;
-    if (cc < 0.0f) cc = 0.0f;
-    return cc;
-}
-
 struct ProjectArgs {
     const float4* mo4;
     const float* scal;
@@ -181,17 +158,6 @@ __device__ __forceinline__ void load_sh_rows(const ProjectArgs& a, int gi,
 #pragma unroll
             for (int i = 0; i < NC; ++i) hc[c][i] = h[c * a.sh_stride + i];
     }
-}
-
-// sh_coeffs_to_color (sh.jl:38-112) seen from camera position p: the clamped colour.
-template <int DEG>
-__device__ __forceinline__ float3 colour_from_sh(const float (&hc)[3][(DEG + 1) * (DEG + 1)],
-                                                 const float* p, float mx0, float my0, float mz0) {
-    const float vx = mx0 - p[0], vy = my0 - p[1], vz = mz0 - p[2];
-    const float inv = 1.0f / sqrtf(vx * vx + vy * vy + vz * vz);
-    const float dx = vx * inv, dy = vy * inv, dz = vz * inv;
-    return make_float3(sh_channel<DEG>(hc[0], dx, dy, dz), sh_channel<DEG>(hc[1], dx, dy, dz),
-                       sh_channel<DEG>(hc[2], dx, dy, dz));
 }
 
 template <int DEG>
@@ -501,13 +467,18 @@ GS3D_API int gs3d_render_forward_workspace_size(int64_t capacity_n, int64_t capa
 }
 
 // cov != NULL: render-only input (g's means_opacity_features hold the opacities themselves).
+// mx4 != NULL (render-only input): the colours come from these 4-bit SH rows (row i, or row
+// mx4_indices[i]) in a kernel of their own before the blend; g's sh_coeffs are not read.
 static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_gaussians* g,
-                               const float* cov, const gs3d_camera* cam, const gs3d_tiling* til,
-                               const gs3d_render_options* opt, gs3d_render_buffers* buf,
-                               int32_t* host_counts, uint32_t flags, gs3d_stream_t stream_) {
+                               const float* cov, const gs3d_mx4_rows* mx4,
+                               const int32_t* mx4_indices, const gs3d_camera* cam,
+                               const gs3d_tiling* til, const gs3d_render_options* opt,
+                               gs3d_render_buffers* buf, int32_t* host_counts, uint32_t flags,
+                               gs3d_stream_t stream_) {
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     GS3D_RETURN_IF(check_common(g, cam, til, opt));
-    if (cov && (flags & GS3D_RENDER_DEFER_COLOUR))
+    if (mx4) GS3D_RETURN_IF(check_mx4_sh(mx4, mx4_indices, g->n, opt->sh_degree));
+    if ((cov || mx4) && (flags & GS3D_RENDER_DEFER_COLOUR))
         return invalid("GS3D_RENDER_DEFER_COLOUR is for trainable Gaussians");
     if (!outputs || !buf) return invalid("NULL outputs or buffers");
     if (g->n > buf->capacity_n) return invalid("n = %d exceeds capacity_n = %lld", g->n, (long long)buf->capacity_n);
@@ -564,7 +535,9 @@ static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_ga
     const int pgrid = grid_for(n, 256, 8);
     {
         ProfScope prof("project", stream);
-        if (cov) {
+        if (mx4) {
+            if (n > 0) k_project<0, true, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt);
+        } else if (cov) {
             switch (opt->sh_degree) {
                 case 0: k_project<0, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
                 case 1: k_project<1, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
@@ -616,6 +589,9 @@ static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_ga
                                            buf->tiles_end_sdfgidx, buf->df2dgs_codes,
                                            buf->sdf2dgs_codes, buf->sdfgidx_to_fgidx, stream));
         }
+        if (mx4)
+            GS3D_RETURN_IF(launch_mx4_render_colours(mx4, mx4_indices, g->means_opacity_features, n,
+                                                     cam, opt->sh_degree, buf, stream));
         if (!(flags & GS3D_RENDER_DEFER_COLOUR)) {
             ProfScope prof("raster", stream);
             GS3D_RETURN_IF(launch_raster(*outputs, *cam, *til, *opt, *buf,
@@ -670,6 +646,9 @@ static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_ga
             counts, buf->capacity_dup, buf->sdf2dgs_codes, nb_tiles, buf->tiles_end_sdfgidx);
         GS3D_LAUNCHED("k_tiles_end");
     }
+    if (mx4)
+        GS3D_RETURN_IF(launch_mx4_render_colours(mx4, mx4_indices, g->means_opacity_features, n, cam,
+                                                 opt->sh_degree, buf, stream));
     // F8 / F9
     if (!(flags & GS3D_RENDER_DEFER_COLOUR)) {
         ProfScope prof("raster", stream);
@@ -687,15 +666,15 @@ GS3D_API int gs3d_render_forward(const gs3d_render_outputs* outputs, const gs3d_
                                  const gs3d_camera* cam, const gs3d_tiling* til,
                                  const gs3d_render_options* opt, gs3d_render_buffers* buf,
                                  int32_t* host_counts, uint32_t flags, gs3d_stream_t stream) {
-    return render_forward_impl(outputs, g, nullptr, cam, til, opt, buf, host_counts, flags, stream);
+    return render_forward_impl(outputs, g, nullptr, nullptr, nullptr, cam, til, opt, buf, host_counts,
+                               flags, stream);
 }
 
-GS3D_API int gs3d_render_forward_render_only(const gs3d_render_outputs* outputs,
-                                             const gs3d_render_only_gaussians* ro,
-                                             const gs3d_camera* cam, const gs3d_tiling* til,
-                                             const gs3d_render_options* opt,
-                                             gs3d_render_buffers* buf, int32_t* host_counts,
-                                             uint32_t flags, gs3d_stream_t stream) {
+static int render_only_impl(const gs3d_render_outputs* outputs, const gs3d_render_only_gaussians* ro,
+                            const gs3d_mx4_rows* mx4, const int32_t* mx4_indices,
+                            const gs3d_camera* cam, const gs3d_tiling* til,
+                            const gs3d_render_options* opt, gs3d_render_buffers* buf,
+                            int32_t* host_counts, uint32_t flags, gs3d_stream_t stream) {
     if (!ro) return invalid("NULL Gaussians");
     if (ro->n > 0 && !ro->covariances) return invalid("NULL covariances");
     gs3d_gaussians g{};
@@ -704,9 +683,30 @@ GS3D_API int gs3d_render_forward_render_only(const gs3d_render_outputs* outputs,
     g.means_opacity_features = ro->means_opacities;
     g.scaling_features = ro->covariances;   // not read: satisfies the shared argument checks
     g.rotation_features = ro->covariances;
-    g.sh_coeffs = ro->sh_coeffs;
-    return render_forward_impl(outputs, &g, ro->n > 0 ? ro->covariances : nullptr, cam, til, opt,
-                               buf, host_counts, flags, stream);
+    g.sh_coeffs = mx4 ? ro->covariances : ro->sh_coeffs;
+    return render_forward_impl(outputs, &g, ro->n > 0 ? ro->covariances : nullptr, mx4, mx4_indices,
+                               cam, til, opt, buf, host_counts, flags, stream);
+}
+
+GS3D_API int gs3d_render_forward_render_only(const gs3d_render_outputs* outputs,
+                                             const gs3d_render_only_gaussians* ro,
+                                             const gs3d_camera* cam, const gs3d_tiling* til,
+                                             const gs3d_render_options* opt,
+                                             gs3d_render_buffers* buf, int32_t* host_counts,
+                                             uint32_t flags, gs3d_stream_t stream) {
+    return render_only_impl(outputs, ro, nullptr, nullptr, cam, til, opt, buf, host_counts, flags, stream);
+}
+
+GS3D_API int gs3d_render_forward_mx4(const gs3d_render_outputs* outputs,
+                                     const gs3d_render_only_gaussians* ro, const gs3d_mx4_rows* sh,
+                                     const int32_t* indices, const gs3d_camera* cam,
+                                     const gs3d_tiling* til, const gs3d_render_options* opt,
+                                     gs3d_render_buffers* buf, int32_t* host_counts, uint32_t flags,
+                                     gs3d_stream_t stream) {
+    if (!sh) return invalid("NULL 4-bit SH rows");
+    if (ro && sh->dim != 3 * (ro->sh_degree + 1) * (ro->sh_degree + 1))
+        return invalid("4-bit SH rows of dim %d for storage SH degree %d", sh->dim, ro->sh_degree);
+    return render_only_impl(outputs, ro, sh, indices, cam, til, opt, buf, host_counts, flags, stream);
 }
 
 GS3D_API int gs3d_render_forward_colour(const gs3d_render_outputs* outputs,

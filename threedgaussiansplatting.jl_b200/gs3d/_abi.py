@@ -29,6 +29,12 @@ GS3D_DENSE_ROW = 60
 GS3D_GEOM_ROW = 12
 GS3D_COLOUR_ROW = 4
 GS3D_MAX_FACTORED_VIEWS = 64
+GS3D_F32 = 0
+GS3D_F16 = 1
+GS3D_BF16 = 2
+GS3D_TABLE_ACCUMULATE = 1
+GS3D_NVFP4 = 0
+GS3D_MXFP4 = 1
 
 f32p = C.POINTER(C.c_float)
 i32p = C.POINTER(C.c_int32)
@@ -125,6 +131,16 @@ class AdcParamsC(C.Structure):
                 ("use_max_scale_pruning", C.c_int32)]
 
 
+class RowsC(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("row_stride", C.c_int64), ("dim", C.c_int32),
+                ("type", C.c_int32), ("data", C.c_void_p)]
+
+
+class MX4RowsC(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("dim", C.c_int32), ("format", C.c_int32),
+                ("codes", C.c_void_p), ("scales", C.c_void_p), ("tensor_scale", C.c_void_p)]
+
+
 P = C.POINTER
 # name -> (restype, argtypes); every symbol include/gs3d.h declares
 SIGNATURES = {
@@ -205,6 +221,20 @@ SIGNATURES = {
     "gs3d_opacity_reset": (C.c_int, [P(GaussiansC), P(AdamMomentsC), C.c_float, C.c_void_p]),
     "gs3d_densify_remap_dense": (C.c_int, [P(AdcBuffersC), C.c_int32, C.c_void_p, C.c_void_p,
                                            C.c_void_p]),
+    "gs3d_table_lookup": (C.c_int, [P(RowsC), C.c_void_p, C.c_float, P(RowsC), C.c_void_p]),
+    "gs3d_table_gradient_workspace_size": (C.c_int, [C.c_int64, C.c_int64, C.c_int32,
+                                                     P(C.c_size_t)]),
+    "gs3d_table_gradient": (C.c_int, [P(RowsC), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                      C.c_float, P(RowsC), C.c_uint32, C.c_void_p, C.c_size_t,
+                                      C.c_void_p]),
+    "gs3d_mx4_tensor_scale": (C.c_int, [P(RowsC), C.c_void_p, C.c_void_p]),
+    "gs3d_mx4_quantise": (C.c_int, [P(RowsC), P(MX4RowsC), C.c_void_p]),
+    "gs3d_mx4_dequantise": (C.c_int, [P(MX4RowsC), P(RowsC), C.c_void_p]),
+    "gs3d_mx4_colours": (C.c_int, [P(MX4RowsC), C.c_int32, C.c_void_p, C.c_void_p, C.c_int32,
+                                   C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
+    "gs3d_render_forward_mx4": (C.c_int, [P(RenderOutputsC), P(RenderOnlyGaussiansC), P(MX4RowsC),
+                                          C.c_void_p, P(Camera), P(TilingC), P(RenderOptionsC),
+                                          P(RenderBuffersC), C.c_void_p, C.c_uint32, C.c_void_p]),
     "gs3d_last_error_string": (C.c_char_p, []),
     "gs3d_version": (C.c_int, []),
     "gs3d_profile_enable": (C.c_int, [C.c_int]),

@@ -1,0 +1,295 @@
+"""SH coefficients in fewer bytes (no counterpart in the reference, which keeps 3 (d+1)^2 floats per
+Gaussian): rows shared through a table, with the table's gradient for fine-tuning, and rows in
+microscaled 4-bit floating point, with the colours a render takes from them. All through libgs3d.so.
+
+    table_lookup / table_gradient ....... out[i] = scale * table[indices[i]], and its gradient
+    mx4_tensor_scale / mx4_quantise /
+    mx4_dequantise ...................... rows <-> 4-bit elements with block scales (MX4Rows)
+    mx4_colours ......................... colours of Gaussians with 4-bit rows from given cameras
+    SHTable, fit_table .................. a model's table and its 1-based row per Gaussian
+    compress ............................ a CompressedGaussiansVector for gs3d.render
+
+Every call runs on `stream` (default: the current stream of its tensors' device), allocates what it
+returns and its workspace there, and does not synchronise; it can be captured into a CUDA graph."""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from . import _abi
+from .structs import (MX4_FORMATS, CompressedGaussiansVector, GaussiansVector, MX4Rows,
+                      RenderOnlyGaussiansVector)
+
+_TYPES = {torch.float32: _abi.GS3D_F32, torch.float16: _abi.GS3D_F16, torch.bfloat16: _abi.GS3D_BF16}
+
+
+def _rows_c(t: torch.Tensor, what: str) -> _abi.RowsC:
+    """gs3d_rows of a (rows, ...) tensor whose trailing axes are contiguous."""
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
+    if t.dim() < 2:
+        raise ValueError(f"{what}: need (rows, ...), got shape {tuple(t.shape)}")
+    rows, dim = t.shape[0], 1
+    for size in t.shape[1:]:
+        dim *= size
+    if t.is_contiguous():
+        stride = dim
+    else:
+        expect = 1
+        for size, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if size != 1 and st != expect:
+                raise ValueError(f"{what}: the elements of a row must be contiguous")
+            expect *= size
+        stride = t.stride(0) if rows > 1 else dim
+        if stride < dim:
+            raise ValueError(f"{what}: rows overlap (row stride {stride}, {dim} elements)")
+    return _abi.RowsC(rows, stride, dim, kind, t.data_ptr())
+
+
+def _check_device(first: torch.Tensor, *others) -> None:
+    if first.device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {first.device}")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+def _check_indices(t: torch.Tensor | None, what: str = "indices") -> None:
+    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous (n,) int32 tensor (1-based)")
+
+
+class _On:
+    """The tensors' device and the call's stream made current, so that what the call allocates
+    belongs to that stream; nothing to do when they are already."""
+
+    def __init__(self, device: torch.device, stream: torch.cuda.Stream | None):
+        if stream is not None and stream.device != device:
+            raise ValueError(f"stream on {stream.device} for tensors on {device}")
+        self.ctx = None
+        if stream is not None:
+            self.ctx = torch.cuda.stream(stream)
+        elif device.index != torch.cuda.current_device():
+            self.ctx = torch.cuda.device(device)
+        self.device = device
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+# -- tables -----------------------------------------------------------------------------------
+def table_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 1.0,
+                 dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """out[i] = scale * table[indices[i] - 1]: the rows of `table` ((rows, ...), float32, float16 or
+    bfloat16) for 1-based int32 `indices`; an index outside 1 .. rows gives zeros. Products are
+    fp32, rounded once to `dtype` (default: the table's). `out` ((n, ...)) is filled in place."""
+    _check_indices(indices)
+    _check_device(table, indices, out)
+    t = _rows_c(table, "table")
+    shape = (indices.shape[0], *table.shape[1:])
+    with _On(table.device, stream) as handle:
+        if out is None:
+            out = torch.empty(shape, dtype=dtype or table.dtype, device=table.device)
+        elif out.shape != shape or (dtype is not None and out.dtype != dtype):
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a lookup of {shape} {dtype or out.dtype}")
+        o = _rows_c(out, "out")
+        _abi.check(_abi.lib().gs3d_table_lookup(C.byref(t), indices.data_ptr(), scale, C.byref(o), handle))
+    return out
+
+
+def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, scale: float = 1.0,
+                   out: torch.Tensor | None = None, accumulate: bool = False,
+                   fgidx_to_gidx: torch.Tensor | None = None,
+                   device_counts: torch.Tensor | None = None,
+                   stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The gradient of table_lookup for a table of `nb_rows` rows: float32 rows out[k] = scale * sum
+    of grads[f] over the rows f with index k + 1, summed in an order fixed by the indices.
+    `fgidx_to_gidx`: row f of `grads` belongs to filtered Gaussian f (as in
+    FilteredGaussiansGradients.sh_coeffs_grads) and has index indices[fgidx_to_gidx[f] - 1];
+    `device_counts`: only the first device_counts[0] rows take part. `accumulate`: add to `out`."""
+    _check_indices(indices)
+    _check_indices(fgidx_to_gidx, "fgidx_to_gidx")
+    _check_device(grads, indices, fgidx_to_gidx, device_counts, out)
+    g = _rows_c(grads, "grads")
+    if fgidx_to_gidx is not None and fgidx_to_gidx.shape[0] < g.rows:
+        raise ValueError(f"{fgidx_to_gidx.shape[0]} fgidx_to_gidx entries for {g.rows} rows")
+    if device_counts is not None and (device_counts.dtype != torch.int32 or device_counts.numel() < 1):
+        raise ValueError("device_counts must hold int32 counts")
+    if accumulate and out is None:
+        raise ValueError("accumulate needs out")
+    shape = (int(nb_rows), *grads.shape[1:])
+    with _On(grads.device, stream) as handle:
+        if out is None:
+            out = torch.empty(shape, dtype=torch.float32, device=grads.device)
+        elif out.shape != shape or out.dtype != torch.float32:
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a float32 table gradient of {shape}")
+        o = _rows_c(out, "out")
+        lib = _abi.lib()
+        nbytes = C.c_size_t(0)
+        _abi.check(lib.gs3d_table_gradient_workspace_size(g.rows, o.rows, g.dim, C.byref(nbytes)))
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=grads.device)
+        _abi.check(lib.gs3d_table_gradient(
+            C.byref(g), indices.data_ptr(), indices.shape[0],
+            None if fgidx_to_gidx is None else fgidx_to_gidx.data_ptr(),
+            None if device_counts is None else device_counts.data_ptr(), scale, C.byref(o),
+            _abi.GS3D_TABLE_ACCUMULATE if accumulate else 0, ws.data_ptr(), nbytes.value, handle))
+    return out
+
+
+# -- 4-bit rows -------------------------------------------------------------------------------
+def mx4_tensor_scale(x: torch.Tensor, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """(1,) float32: max(largest finite |x| / 2688, 2^-100), the nvfp4 tensor scale with which no
+    block of `x` ((rows, ...)) saturates."""
+    _check_device(x)
+    c = _rows_c(x, "x")
+    with _On(x.device, stream) as handle:
+        scale = torch.empty(1, dtype=torch.float32, device=x.device)
+        _abi.check(_abi.lib().gs3d_mx4_tensor_scale(C.byref(c), scale.data_ptr(), handle))
+    return scale
+
+
+def mx4_quantise(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None,
+                 stream: torch.cuda.Stream | None = None) -> MX4Rows:
+    """The rows of `x` ((rows, ...), float32, float16 or bfloat16) as 4-bit elements with block
+    scales (gs3d_mx4_quantise). `tensor_scale` (nvfp4): (1,) float32 on the device, within 2^-100 ..
+    2^100; None: mx4_tensor_scale(x)."""
+    _check_device(x, tensor_scale)
+    c = _rows_c(x, "x")
+    with _On(x.device, stream) as handle:
+        if format == "nvfp4" and tensor_scale is None:
+            tensor_scale = mx4_tensor_scale(x)
+        q = MX4Rows.empty(c.rows, c.dim, format, x.device, tensor_scale)
+        _abi.check(_abi.lib().gs3d_mx4_quantise(C.byref(c), C.byref(q.to_c()), handle))
+    return q
+
+
+def mx4_dequantise(rows: MX4Rows, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                   stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The values `rows` stand for as (rows, dim) `dtype`, or into `out` ((rows, ...) of dim elements)."""
+    _check_device(rows.codes, out)
+    with _On(rows.device, stream) as handle:
+        if out is None:
+            out = torch.empty((rows.rows, rows.dim), dtype=dtype, device=rows.device)
+        o = _rows_c(out, "out")
+        _abi.check(_abi.lib().gs3d_mx4_dequantise(C.byref(rows.to_c()), C.byref(o), handle))
+    return out
+
+
+def mx4_colours(rows: MX4Rows, means: torch.Tensor, positions, sh_degree: int,
+                indices: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Colours of n Gaussians seen from the cameras at `positions` ((views, 3) float32, host): a
+    (views, n, 4) float32 tensor, the fourth value 0 (the rows render_given_colour takes with
+    shard_rows = n, n_ranks = 1). `means`: (n, 4) float32, the first three the mean; Gaussian i has
+    SH row i of `rows`, or row indices[i] (1-based)."""
+    pos = np.ascontiguousarray(positions, dtype=np.float32)
+    if pos.ndim != 2 or pos.shape[1] != 3:
+        raise ValueError(f"positions must be (views, 3), got {pos.shape}")
+    _check_indices(indices)
+    _check_device(rows.codes, means, indices, out)
+    n = means.shape[0]
+    if means.shape != (n, 4) or means.dtype != torch.float32 or not means.is_contiguous():
+        raise ValueError("means must be a contiguous (n, 4) float32 tensor")
+    if indices is not None and indices.shape[0] != n:
+        raise ValueError(f"{indices.shape[0]} indices for {n} Gaussians")
+    shape = (pos.shape[0], n, 4)
+    with _On(rows.device, stream) as handle:
+        if out is None:
+            out = torch.empty(shape, dtype=torch.float32, device=rows.device)
+        elif out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
+        _abi.check(_abi.lib().gs3d_mx4_colours(
+            C.byref(rows.to_c()), int(sh_degree), None if indices is None else indices.data_ptr(),
+            means.data_ptr(), n, pos.ctypes.data, pos.shape[0], out.data_ptr(), n, handle))
+    return out
+
+
+# -- models -----------------------------------------------------------------------------------
+@dataclass
+class SHTable:
+    """SH coefficients shared by Gaussians: Gaussian i has scale * coeffs[indices[i] - 1].
+    `coeffs`: (rows, 3, (d+1)^2) float32, float16 or bfloat16; `indices`: (n,) int32, 1-based."""
+
+    coeffs: torch.Tensor
+    indices: torch.Tensor
+    scale: float = 1.0
+
+    def __post_init__(self):
+        if self.coeffs.dim() != 3 or self.coeffs.shape[1] != 3 or self.coeffs.shape[2] not in (1, 4, 9, 16):
+            raise ValueError(f"coeffs must be (rows, 3, (d+1)^2), got {tuple(self.coeffs.shape)}")
+        _check_indices(self.indices)
+
+    @property
+    def rows(self) -> int:
+        return self.coeffs.shape[0]
+
+    def expand(self, out: torch.Tensor | None = None,
+               stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        """(n, 3, (d+1)^2) float32 SH coefficients, e.g. into a GaussiansVector's sh_coeffs."""
+        return table_lookup(self.coeffs, self.indices, self.scale, torch.float32, out, stream)
+
+    def gradient(self, fgradients, buffers, out: torch.Tensor | None = None, accumulate: bool = False,
+                 stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        """Gradient of `coeffs` from the SH gradients of backward() (FilteredGaussiansGradients and
+        the RenderBuffers of its render)."""
+        return table_gradient(fgradients.sh_coeffs_grads, self.indices, self.rows, self.scale, out,
+                              accumulate, buffers.fgidx_to_gidx, buffers.device_counts, stream)
+
+
+def fit_table(sh_coeffs: torch.Tensor, nb_rows: int, iterations: int = 10, seed: int = 0) -> SHTable:
+    """A table of (at most) `nb_rows` rows for `sh_coeffs` ((n, 3, order) float32 on a CUDA device)
+    by Lloyd's algorithm: rows start as a random choice of the Gaussians' coefficients, then every
+    Gaussian takes its nearest row and every row the mean of its Gaussians (rows without any keep
+    their value). A one-off preparation: the distances are torch products, in chunks."""
+    n = sh_coeffs.shape[0]
+    if n < 1 or nb_rows < 1:
+        raise ValueError(f"a table of {nb_rows} rows for {n} Gaussians")
+    x = sh_coeffs.reshape(n, -1)
+    gen = torch.Generator().manual_seed(int(seed))
+    pick = torch.randperm(n, generator=gen)[:nb_rows].to(x.device)
+    centres = x[pick].clone()
+    rows = centres.shape[0]
+    chunk = max(1, (1 << 28) // rows)
+    indices = torch.empty(n, dtype=torch.int32, device=x.device)
+    for it in range(max(1, int(iterations)) + 1):
+        half = 0.5 * (centres * centres).sum(dim=1)
+        for a in range(0, n, chunk):
+            b = min(n, a + chunk)
+            indices[a:b] = (torch.addmm(half, x[a:b], centres.t(), alpha=-1.0).argmin(dim=1) + 1).to(torch.int32)
+        if it == max(1, int(iterations)):
+            break
+        sums = table_gradient(x, indices, rows)
+        members = torch.bincount(indices.long(), minlength=rows + 1)[1:, None]
+        centres = torch.where(members > 0, sums / members.clamp(min=1), centres)
+    return SHTable(centres.reshape(rows, *sh_coeffs.shape[1:]).contiguous(), indices)
+
+
+def compress(gaussians, format: str = "nvfp4", table: SHTable | None = None) -> CompressedGaussiansVector:
+    """A model for rendering with its SH coefficients in 4 bits: every Gaussian's own row, or with
+    `table` the table's rows (times its scale) and its indices. `gaussians`: GaussiansVector or
+    RenderOnlyGaussiansVector on a CUDA device."""
+    ro = (RenderOnlyGaussiansVector.from_trainable(gaussians) if isinstance(gaussians, GaussiansVector)
+          else gaussians)
+    if table is None:
+        return CompressedGaussiansVector(ro.means_opacities, ro.covariances,
+                                         mx4_quantise(ro.sh_coeffs, format))
+    rows = table_lookup(table.coeffs, torch.arange(1, table.rows + 1, dtype=torch.int32,
+                                                   device=table.coeffs.device), table.scale, torch.float32)
+    return CompressedGaussiansVector(ro.means_opacities, ro.covariances, mx4_quantise(rows, format),
+                                     table.indices)
+
+
+__all__ = ["MX4_FORMATS", "MX4Rows", "SHTable", "CompressedGaussiansVector", "compress", "fit_table",
+           "mx4_colours", "mx4_dequantise", "mx4_quantise", "mx4_tensor_scale", "table_gradient",
+           "table_lookup"]

@@ -6,9 +6,8 @@ import ctypes as C
 import torch
 
 from . import _abi
-from .structs import (GaussiansVector, PinholeCamera, RenderBuffers, RenderOnlyGaussiansVector,
-                      RenderOptions,
-                      RenderOutputs, Tiling)
+from .structs import (CompressedGaussiansVector, GaussiansVector, PinholeCamera, RenderBuffers,
+                      RenderOnlyGaussiansVector, RenderOptions, RenderOutputs, Tiling, _ptr)
 
 
 def _stream_handle(stream: torch.cuda.Stream | None) -> int:
@@ -28,7 +27,8 @@ def render(outputs: RenderOutputs, gaussians: GaussiansVector, camera: PinholeCa
     `reference_order` also fills the unsorted duplicate arrays and the duplicate-count scan
     as the reference does (GS3D_RENDER_REFERENCE_ORDER); the sorted arrays, tile ends and
     images are the same either way. `gaussians` may also be a RenderOnlyGaussiansVector
-    (stored opacities and 3D covariances; gs3d_render_forward_render_only).
+    (stored opacities and 3D covariances; gs3d_render_forward_render_only) or a
+    CompressedGaussiansVector (the same with 4-bit SH rows; gs3d_render_forward_mx4).
     `contrib_masks=False` leaves the buffers' contribution masks unwritten (for renders that no
     backward follows; GS3D_RENDER_NO_CONTRIB_MASKS). `defer_colour=True` stops before the colours
     and the blend (the SH coefficients are not read); `render_colour` completes the render."""
@@ -45,13 +45,18 @@ def render(outputs: RenderOutputs, gaussians: GaussiansVector, camera: PinholeCa
     host = buffers.host_counts
     hptr = C.c_void_p(host.data_ptr()) if host is not None else None
     args = (outputs.to_c(), gaussians.to_c(), camera.to_c(), tiling.to_c(), options.to_c())
-    entry = (lib.gs3d_render_forward_render_only if isinstance(gaussians, RenderOnlyGaussiansVector)
-             else lib.gs3d_render_forward)
+    source = [C.byref(args[1])]
+    if isinstance(gaussians, CompressedGaussiansVector):
+        entry, sh = lib.gs3d_render_forward_mx4, gaussians.sh.to_c()
+        source += [C.byref(sh), C.c_void_p(_ptr(gaussians.indices))]
+    elif isinstance(gaussians, RenderOnlyGaussiansVector):
+        entry = lib.gs3d_render_forward_render_only
+    else:
+        entry = lib.gs3d_render_forward
     for _ in range(4):
         b = buffers.to_c()
-        st = entry(C.byref(args[0]), C.byref(args[1]), C.byref(args[2]),
-                                     C.byref(args[3]), C.byref(args[4]), C.byref(b), hptr,
-                                     flags, C.c_void_p(_stream_handle(stream)))
+        st = entry(C.byref(args[0]), *source, C.byref(args[2]), C.byref(args[3]), C.byref(args[4]),
+                   C.byref(b), hptr, flags, C.c_void_p(_stream_handle(stream)))
         if st == _abi.GS3D_ERR_CAPACITY:
             buffers.grow_dup(int(host[1]) if host is not None else 2 * buffers.capacity_dup)
             continue

@@ -8,6 +8,7 @@ values stored in arrays are 1-based, as in the reference.
     RenderOptions ........ forward_structs.jl:579-719 (image_coordinates.jl for clip bounds)
     Tiling ............... forward_structs.jl:340-424
     GaussiansVector ...... gaussians.jl:30-52 (TrainableGaussiansVector)
+    MX4Rows, CompressedGaussiansVector ... SH coefficients in 4 bits (no reference counterpart)
     RenderBuffers ........ forward_structs.jl:1541-1600, :762-786
     RenderOutputs ........ forward_structs.jl:1-65
 """
@@ -371,6 +372,120 @@ class RenderOnlyGaussiansVector:
         g.covariances = _ptr(self.covariances)
         g.sh_coeffs = _ptr(self.sh_coeffs)
         return g
+
+
+MX4_FORMATS = {"nvfp4": (_abi.GS3D_NVFP4, 16), "mxfp4": (_abi.GS3D_MXFP4, 32)}
+
+
+@dataclass
+class MX4Rows:
+    """Rows of `dim` microscaled 4-bit elements (gs3d_mx4_rows): (rows, ceil(dim / 2)) uint8 codes,
+    element 2 j in the low 4 bits of byte j; (rows, blocks) uint8 block scales, e4m3 for blocks of
+    16 ("nvfp4", with the (1,) float32 `tensor_scale`) or e8m0 for blocks of 32 ("mxfp4")."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    tensor_scale: torch.Tensor | None
+    dim: int
+    format: str
+
+    def __post_init__(self):
+        if self.format not in MX4_FORMATS:
+            raise ValueError(f"4-bit format {self.format!r} is not in {sorted(MX4_FORMATS)}")
+        rows, dim, block = self.codes.shape[0], int(self.dim), MX4_FORMATS[self.format][1]
+        if self.codes.shape != (rows, (dim + 1) // 2) or self.scales.shape != (rows, -(-dim // block)):
+            raise ValueError(f"codes {tuple(self.codes.shape)} and scales {tuple(self.scales.shape)} "
+                             f"are not those of {self.format} rows of {dim} elements")
+        for t in (self.codes, self.scales):
+            if t.dtype != torch.uint8 or not t.is_contiguous() or t.device != self.codes.device:
+                raise ValueError("codes and scales must be contiguous uint8 tensors on one device")
+        ts = self.tensor_scale
+        if self.format == "nvfp4":
+            if ts is None or ts.numel() != 1 or ts.dtype != torch.float32 or ts.device != self.codes.device:
+                raise ValueError("nvfp4 rows need a (1,) float32 tensor scale on their device")
+        elif ts is not None:
+            raise ValueError("mxfp4 rows have no tensor scale")
+
+    @classmethod
+    def empty(cls, rows: int, dim: int, format: str, device, tensor_scale=None) -> "MX4Rows":
+        if format not in MX4_FORMATS:
+            raise ValueError(f"4-bit format {format!r} is not in {sorted(MX4_FORMATS)}")
+        blocks = -(-dim // MX4_FORMATS[format][1])
+        return cls(torch.empty((rows, (dim + 1) // 2), dtype=torch.uint8, device=device),
+                   torch.empty((rows, blocks), dtype=torch.uint8, device=device), tensor_scale, dim, format)
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel() + (0 if self.tensor_scale is None else 4)
+
+    def to(self, device) -> "MX4Rows":
+        ts = self.tensor_scale
+        return MX4Rows(self.codes.to(device), self.scales.to(device),
+                       None if ts is None else ts.to(device), self.dim, self.format)
+
+    def to_c(self) -> _abi.MX4RowsC:
+        return _abi.MX4RowsC(self.codes.shape[0], self.dim, MX4_FORMATS[self.format][0],
+                             _ptr(self.codes), _ptr(self.scales), _ptr(self.tensor_scale))
+
+
+@dataclass
+class CompressedGaussiansVector:
+    """A RenderOnlyGaussiansVector whose SH coefficients are 4-bit rows: Gaussian i takes row i of
+    `sh`, or with `indices` ((n,) int32, 1-based) row indices[i] of a shared table (an index outside
+    1 .. sh.rows: coefficients 0). Rendered by gs3d_render_forward_mx4; not trainable."""
+
+    means_opacities: torch.Tensor
+    covariances: torch.Tensor
+    sh: MX4Rows
+    indices: torch.Tensor | None = None
+
+    def __post_init__(self):
+        n = self.means_opacities.shape[0]
+        if self.means_opacities.shape != (n, 4) or self.covariances.shape != (n, 6):
+            raise ValueError("means_opacities must be (n, 4) and covariances (n, 6)")
+        for t in (self.means_opacities, self.covariances):
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                raise ValueError("means_opacities and covariances must be contiguous float32 tensors")
+        if self.sh.dim not in (3, 12, 27, 48):
+            raise ValueError(f"SH rows of {self.sh.dim} elements match no SH degree <= 3")
+        if self.indices is None:
+            if self.sh.rows != n:
+                raise ValueError(f"{self.sh.rows} SH rows for {n} Gaussians without indices")
+        elif (self.indices.shape != (n,) or self.indices.dtype != torch.int32
+              or not self.indices.is_contiguous()):
+            raise ValueError("indices must be a contiguous (n,) int32 tensor")
+        if any(t is not None and t.device != self.means_opacities.device
+               for t in (self.covariances, self.sh.codes, self.indices)):
+            raise ValueError("all arrays must be on one device")
+
+    @property
+    def n(self) -> int:
+        return self.means_opacities.shape[0]
+
+    @property
+    def sh_degree(self) -> int:
+        return int(round(math.sqrt(self.sh.dim // 3))) - 1
+
+    @property
+    def device(self):
+        return self.means_opacities.device
+
+    def to(self, device) -> "CompressedGaussiansVector":
+        return CompressedGaussiansVector(
+            self.means_opacities.to(device), self.covariances.to(device), self.sh.to(device),
+            None if self.indices is None else self.indices.to(device))
+
+    def to_c(self) -> _abi.RenderOnlyGaussiansC:
+        return _abi.RenderOnlyGaussiansC(self.n, self.sh_degree, _ptr(self.means_opacities),
+                                         _ptr(self.covariances), None)
 
 
 @dataclass

@@ -32,85 +32,502 @@ __global__ void __launch_bounds__(256) k_table_lookup(const TI* __restrict__ tab
 }
 
 // ---- gradient --------------------------------------------------------------------------------
-// Row f's key: its table row 1 .. rows, or 0 where it takes no part.
-__global__ void __launch_bounds__(256) k_table_keys(const int32_t* __restrict__ indices, int64_t n_indices,
-                                                    const int32_t* __restrict__ f2g,
-                                                    const int32_t* __restrict__ counts, int64_t n, int64_t rows,
-                                                    int64_t* __restrict__ keys, int32_t* __restrict__ vals) {
-    const int64_t live = counts ? min((int64_t)max(counts[0], 0), n) : n;
-    for (int64_t f = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; f < n;
-         f += (int64_t)gridDim.x * blockDim.x) {
-        int k = 0;
-        if (f < live) {
-            const int64_t i = f2g ? (int64_t)f2g[f] - 1 : f;
-            if (i >= 0 && i < n_indices) k = indices[i];
-            if (k < 1 || k > rows) k = 0;
+// 1. Stable sort of the rows by table row (radix_*: 4096-row tiles, digits of up to 10 bits, three
+//    launches a pass, one pass per 10 bits of the row number; up to 4096 rows: one block sorts them in
+//    shared memory). Rows without a valid index drop out of the first pass, which also zeroes
+//    the table's gradients.
+// 2. k_table_segments: the sorted rows are cut into chunks of equal length, a block each, and a chunk
+//    into one run of rows per slot (a slot: the threads side by side on a row's columns). A slot adds
+//    its rows in order; a run of equal indices that starts and ends inside a slot is finished and
+//    stored, the slots' first and last runs are added in slot order through shared memory, and what
+//    crosses a chunk's border is left as a partial sum.
+// 3. k_table_join: the block in whose chunk such a run starts adds its partial sums in chunk order.
+// The order of every sum follows from the sorted order alone, whatever the number of rows that share
+// an index: no atomics, and a row that half of the Gaussians use is spread over the GPU like any other.
+
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortTile = 4096;
+constexpr int kSortRounds = kSortTile / kSortThreads;
+constexpr int kMaxDigitBits = 10;
+
+// Row f's table row 0 .. rows - 1, or -1 where it takes no part.
+struct KeySource {
+    const int32_t* indices;
+    const int32_t* f2g;
+    const int32_t* counts;
+    int64_t n_indices;
+    int32_t n, rows;
+
+    __device__ __forceinline__ int live() const { return counts ? min(max(counts[0], 0), n) : n; }
+    __device__ __forceinline__ int key(int f, int live_rows) const {
+        if (f >= live_rows) return -1;
+        const int64_t i = f2g ? (int64_t)f2g[f] - 1 : f;
+        if (i < 0 || i >= n_indices) return -1;
+        const int k = indices[i];
+        return k >= 1 && k <= rows ? k - 1 : -1;
+    }
+};
+
+// The zeroed table gradients (data NULL: accumulate, nothing to zero).
+struct ZeroRows {
+    float* data;
+    int64_t stride;
+    int32_t rows, dim;
+
+    __device__ __forceinline__ void fill(int64_t thread, int64_t threads) const {
+        if (!data) return;
+        const int64_t total = (int64_t)rows * dim;
+        if (stride == dim && (reinterpret_cast<uintptr_t>(data) & 15) == 0) {
+            float4* d4 = reinterpret_cast<float4*>(data);
+            for (int64_t i = thread; i < total / 4; i += threads) d4[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int64_t i = (total & ~(int64_t)3) + thread; i < total; i += threads) data[i] = 0.0f;
+        } else {
+            for (int64_t i = thread; i < total; i += threads) {
+                const int64_t r = i / dim;
+                data[r * stride + (i - r * dim)] = 0.0f;
+            }
         }
-        keys[f] = k;
-        vals[f] = (int32_t)f;
+    }
+};
+
+struct SortPass {
+    const int32_t* keys_in;  // NULL: the first pass, keys from the source, values f
+    const int32_t* vals_in;
+    int32_t* keys_out;
+    int32_t* vals_out;
+    int32_t* hist;    // [bin][tile]: counts, then their exclusive scan over the tiles
+    int32_t* totals;  // [bin]
+    int32_t* valid;   // number of rows with a valid index (written by the first pass)
+    int32_t ntiles, shift, bits;
+};
+
+// The 16 keys of a thread, warp by warp in row order; -1: none.
+__device__ __forceinline__ void load_tile_keys(const SortPass& p, const KeySource& src, int tile, int (&key)[kSortRounds]) {
+    const int base = tile * kSortTile + (threadIdx.x >> 5) * (kSortRounds * 32) + (threadIdx.x & 31);
+    if (p.keys_in) {
+        const int m = *p.valid;
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) key[r] = base + 32 * r < m ? p.keys_in[base + 32 * r] : -1;
+    } else {
+        const int live = src.live();
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) key[r] = src.key(base + 32 * r, live);
     }
 }
 
-__device__ __forceinline__ int64_t first_not_below(const int64_t* keys, int64_t n, int64_t k) {
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < k) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
-
-// One block per table row: threads side by side on the columns, `slots` of them one after the other
-// on the rows of the segment; the slots' sums are added in order.
-template <typename T>
-__global__ void __launch_bounds__(128) k_table_reduce(const T* __restrict__ grads, int64_t stride, int dim,
-                                                      const int64_t* __restrict__ keys,
-                                                      const int32_t* __restrict__ vals, int64_t n, float scale,
-                                                      float* __restrict__ out, int64_t out_stride, int accumulate) {
-    __shared__ int64_t seg[2];
-    __shared__ float part[128];
-    const int64_t k = blockIdx.x;
-    if (threadIdx.x < 2) seg[threadIdx.x] = first_not_below(keys, n, k + 1 + threadIdx.x);
+__global__ void __launch_bounds__(kSortThreads) k_radix_count(const SortPass p, const KeySource src,
+                                                              const ZeroRows zero) {
+    __shared__ int bins[1 << kMaxDigitBits];
+    const int nbins = 1 << p.bits, tile = blockIdx.x;
+    for (int b = threadIdx.x; b < nbins; b += kSortThreads) bins[b] = 0;
+    int key[kSortRounds];
+    load_tile_keys(p, src, tile, key);
     __syncthreads();
-    const int wide = min(dim, 128), slots = 128 / wide;
-    const int slot = threadIdx.x / wide, col = threadIdx.x - slot * wide;
-    for (int c0 = 0; c0 < dim; c0 += wide) {
-        const int c = c0 + col;
-        float s = 0.0f;
-        if (slot < slots && c < dim)
-            for (int64_t j = seg[0] + slot; j < seg[1]; j += slots) s += to_f32(grads[(int64_t)vals[j] * stride + c]);
-        part[threadIdx.x] = s;
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+        if (key[r] >= 0) atomicAdd(&bins[(key[r] >> p.shift) & (nbins - 1)], 1);
+    if (!p.keys_in) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
+    __syncthreads();
+    for (int b = threadIdx.x; b < nbins; b += kSortThreads) p.hist[(int64_t)b * p.ntiles + tile] = bins[b];
+}
+
+// Block b: exclusive scan of bin b's counts over the tiles.
+__global__ void __launch_bounds__(kSortThreads) k_radix_spine(const SortPass p) {
+    __shared__ int sm[33];
+    int32_t* row = p.hist + (int64_t)blockIdx.x * p.ntiles;
+    int carry = 0, tot;
+    for (int t0 = 0; t0 < p.ntiles; t0 += kSortThreads) {
+        const int t = t0 + threadIdx.x;
+        const int ex = block_exclusive_scan(t < p.ntiles ? row[t] : 0, sm, &tot);
+        if (t < p.ntiles) row[t] = carry + ex;
+        carry += tot;
+    }
+    if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
+}
+
+size_t radix_scatter_smem(int bits) {
+    return (size_t)kSortTile * 8 + (size_t)(1 << bits) * (8 + 2 * kSortWarps);
+}
+
+__global__ void __launch_bounds__(kSortThreads) k_radix_scatter(const SortPass p, const KeySource src) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int sm[33];
+    const int nbins = 1 << p.bits, tile = blockIdx.x;
+    int32_t* keys = reinterpret_cast<int32_t*>(smem);            // the tile in digit order
+    int32_t* vals = keys + kSortTile;
+    int32_t* start = vals + kSortTile;                           // first place of a bin in the tile
+    int32_t* dest = start + nbins;                               // its place in the output, minus start
+    uint16_t* wcount = reinterpret_cast<uint16_t*>(dest + nbins);  // [warp][bin]
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int key[kSortRounds];
+    load_tile_keys(p, src, tile, key);
+    for (int i = threadIdx.x; i < nbins * kSortWarps; i += kSortThreads) wcount[i] = 0;
+    __syncthreads();
+    // stable rank of every key among its warp's keys of the same digit
+    int rank[kSortRounds];
+    const unsigned below = (1u << lane) - 1u;
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+        const int d = key[r] >= 0 ? (key[r] >> p.shift) & (nbins - 1) : nbins;
+        const unsigned peers = __match_any_sync(0xffffffffu, d);
+        const int before = d < nbins ? wcount[w * nbins + d] : 0;
+        rank[r] = before + __popc(peers & below);
+        __syncwarp();
+        if (d < nbins && (peers & below) == 0) wcount[w * nbins + d] = (uint16_t)(before + __popc(peers));
+        __syncwarp();
+    }
+    __syncthreads();
+    // places of the bins in the tile (over this tile's counts) and in the output (over all totals)
+    int here = 0, everywhere = 0;
+    for (int b0 = 0; b0 < nbins; b0 += kSortThreads) {
+        const int b = b0 + threadIdx.x;
+        int run = 0, total = 0, tot;
+        if (b < nbins) {
+#pragma unroll
+            for (int ww = 0; ww < kSortWarps; ++ww) {
+                const int c = wcount[ww * nbins + b];
+                wcount[ww * nbins + b] = (uint16_t)run;
+                run += c;
+            }
+            total = p.totals[b];
+        }
+        const int st = here + block_exclusive_scan(run, sm, &tot);
+        here += tot;
+        const int base = everywhere + block_exclusive_scan(total, sm, &tot);
+        everywhere += tot;
+        if (b < nbins) {
+            start[b] = st;
+            dest[b] = base + p.hist[(int64_t)b * p.ntiles + tile] - st;
+        }
+    }
+    if (!p.keys_in && tile == 0 && threadIdx.x == 0) *p.valid = everywhere;
+    __syncthreads();
+    const int base = tile * kSortTile + w * (kSortRounds * 32) + lane;
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+        if (key[r] >= 0) {
+            const int d = (key[r] >> p.shift) & (nbins - 1);
+            const int at = start[d] + wcount[w * nbins + d] + rank[r];
+            keys[at] = key[r];
+            vals[at] = p.keys_in ? p.vals_in[base + 32 * r] : base + 32 * r;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < here; i += kSortThreads) {
+        const int k = keys[i];
+        const int o = dest[(k >> p.shift) & (nbins - 1)] + i;
+        p.keys_out[o] = k;
+        p.vals_out[o] = vals[i];
+    }
+}
+
+// Up to kSortTile rows: block 0 sorts them in shared memory, 8 bits a pass; the others zero the table.
+constexpr int kSmallThreads = 512;
+constexpr int kSmallWarps = kSmallThreads / 32;
+constexpr int kSmallRounds = kSortTile / kSmallThreads;
+
+__global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource src, const ZeroRows zero, int bits,
+                                                              int32_t* __restrict__ keys_out,
+                                                              int32_t* __restrict__ vals_out,
+                                                              int32_t* __restrict__ valid) {
+    __shared__ int keys[kSortTile], vals[kSortTile];
+    __shared__ uint16_t wcount[kSmallWarps][256];
+    __shared__ int start[256], sm[33];
+    if (gridDim.x > 1 && blockIdx.x > 0) {
+        zero.fill((int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
+        return;
+    }
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned below = (1u << lane) - 1u;
+    const int live = src.live();
+    int count = src.n;
+    for (int shift = 0; shift < max(bits, 1); shift += 8) {
+        const bool first = shift == 0;
+        int key[kSmallRounds], val[kSmallRounds], rank[kSmallRounds];
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r) {
+            const int i = w * (kSmallRounds * 32) + r * 32 + lane;
+            key[r] = -1;
+            val[r] = i;
+            if (first) key[r] = src.key(i, live);
+            else if (i < count) key[r] = keys[i], val[r] = vals[i];
+        }
+        for (int i = threadIdx.x; i < kSmallWarps * 256; i += kSmallThreads) (&wcount[0][0])[i] = 0;
         __syncthreads();
-        if (slot == 0 && c < dim) {
-            for (int q = 1; q < slots; ++q) s += part[q * wide + col];
-            float* o = out + k * out_stride + c;
-            *o = accumulate ? *o + scale * s : scale * s;
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r) {
+            const int d = key[r] >= 0 ? (key[r] >> shift) & 255 : 256;
+            const unsigned peers = __match_any_sync(0xffffffffu, d);
+            const int before = d < 256 ? wcount[w][d] : 0;
+            rank[r] = before + __popc(peers & below);
+            __syncwarp();
+            if (d < 256 && (peers & below) == 0) wcount[w][d] = (uint16_t)(before + __popc(peers));
+            __syncwarp();
         }
         __syncthreads();
+        int run = 0;
+        if (threadIdx.x < 256)
+#pragma unroll
+            for (int ww = 0; ww < kSmallWarps; ++ww) {
+                const int c = wcount[ww][threadIdx.x];
+                wcount[ww][threadIdx.x] = (uint16_t)run;
+                run += c;
+            }
+        int tot;
+        const int st = block_exclusive_scan(run, sm, &tot);
+        if (threadIdx.x < 256) start[threadIdx.x] = st;
+        count = tot;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSmallRounds; ++r)
+            if (key[r] >= 0) {
+                const int d = (key[r] >> shift) & 255;
+                const int at = start[d] + wcount[w][d] + rank[r];
+                keys[at] = key[r];
+                vals[at] = val[r];
+            }
+        __syncthreads();
     }
+    for (int i = threadIdx.x; i < count; i += kSmallThreads) {
+        keys_out[i] = keys[i];
+        vals_out[i] = vals[i];
+    }
+    if (threadIdx.x == 0) *valid = count;
+    if (gridDim.x == 1) zero.fill(threadIdx.x, kSmallThreads);
+}
+
+// VB bytes of a row as VB / sizeof(T) floats.
+template <typename T, int VB>
+struct RowUnit {
+    static constexpr int N = VB / (int)sizeof(T);
+    T e[N];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VB == 16) *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(p));
+        else e[0] = __ldg(p);
+    }
+};
+
+// How a launch cuts the work: `units` units of VB bytes a row, in column tiles of at most 256; `slots`
+// slots a block, each `run` sorted rows long.
+struct SegmentPlan {
+    int units, tile_units, slots, run, chunk, nchunks;
+};
+
+struct Segments {
+    const int32_t* keys;   // sorted
+    const int32_t* vals;
+    const int32_t* valid;
+    float* out;
+    int64_t out_stride;
+    float scale;
+    int accumulate;
+    int32_t* first_key;    // [chunk] index of its first row, -1: none
+    int32_t* owned;        // [chunk] index whose run starts here and goes on in the next chunk, -1: none
+    float* partial;        // [chunk][2][dim]: sums of a first run that began earlier, of the owned run
+};
+
+template <int N>
+__device__ __forceinline__ void store_row(const Segments& g, int key, int col, const float (&s)[N]) {
+    float* o = g.out + (int64_t)key * g.out_stride + col;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float v = g.scale * s[i];
+        o[i] = g.accumulate ? o[i] + v : v;
+    }
+}
+
+template <typename T, int VB>
+__global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ grads, int64_t stride, int dim,
+                                                        const SegmentPlan pl, const Segments g) {
+    using Unit = RowUnit<T, VB>;
+    constexpr int N = Unit::N, AHEAD = 8;
+    extern __shared__ __align__(16) unsigned char smem[];
+    int32_t* sk = reinterpret_cast<int32_t*>(smem);  // the chunk's indices and rows
+    int32_t* sv = sk + pl.chunk;
+    int32_t* pkey = sv + pl.chunk;                   // [slot][2]: the slots' first and last runs
+    float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);  // [slot][2][tile_units * N]
+    const int m = *g.valid;
+    const int begin = blockIdx.x * pl.chunk, count = min(pl.chunk, m - begin);
+    const bool meta = threadIdx.x == 0 && blockIdx.y == 0;
+    if (count <= 0) {
+        if (meta) g.first_key[blockIdx.x] = g.owned[blockIdx.x] = -1;
+        return;
+    }
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        sk[i] = g.keys[begin + i];
+        sv[i] = g.vals[begin + i];
+    }
+    __syncthreads();
+    const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
+    const int unit = blockIdx.y * pl.tile_units + lane;
+    const int col = unit * N;
+    const bool on = unit < pl.units;
+    const int width = pl.tile_units * N;
+    {
+        const int j1 = min((slot + 1) * pl.run, count);
+        int j = slot * pl.run;
+        int cur = j < j1 ? sk[j] : -1;
+        bool first = true;
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+        const T* gc = grads + col;
+        for (; j < j1; j += AHEAD) {
+            Unit u[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                if (on && j + q < j1) u[q].load(gc + (int64_t)sv[j + q] * stride);
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                if (j + q >= j1) break;
+                const int k = sk[j + q];
+                if (k != cur) {
+                    if (first) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) part[(2 * slot) * width + lane * N + i] = acc[i];
+                        if (lane == 0) pkey[2 * slot] = cur;
+                        first = false;
+                    } else if (on) {
+                        store_row<N>(g, cur, col, acc);
+                    }
+                    cur = k;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+                }
+                if (on)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] += to_f32(u[q].e[i]);
+            }
+        }
+        const int which = 2 * slot + (first ? 0 : 1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[which * width + lane * N + i] = acc[i];
+        if (lane == 0) {
+            pkey[which] = cur;
+            if (first) pkey[2 * slot + 1] = -1;
+        }
+    }
+    __syncthreads();
+    if (slot != 0) return;
+    // the slots' open runs in order
+    const bool open_left = begin > 0 && g.keys[begin - 1] == sk[0];
+    const int last = sk[count - 1];
+    const bool open_right = begin + count < m && g.keys[begin + count] == last;
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+    int cur = sk[0];
+    bool first = true;
+    float* partial = g.partial + (int64_t)blockIdx.x * 2 * dim + col;
+    for (int e = 0; e < 2 * pl.slots; ++e) {
+        const int k = pkey[e];
+        if (k < 0) continue;
+        if (k != cur) {
+            if (on) {
+                if (first && open_left) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) partial[i] = acc[i];
+                } else {
+                    store_row<N>(g, cur, col, acc);
+                }
+            }
+            first = false;
+            cur = k;
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += part[e * width + lane * N + i];
+    }
+    const bool earlier = first && open_left;  // the whole chunk goes on from the one before
+    if (on) {
+        if (earlier || open_right) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) partial[(earlier ? 0 : dim) + i] = acc[i];
+        } else {
+            store_row<N>(g, cur, col, acc);
+        }
+    }
+    if (meta) {
+        g.first_key[blockIdx.x] = sk[0];
+        g.owned[blockIdx.x] = open_right && !earlier ? last : -1;
+    }
+}
+
+__global__ void __launch_bounds__(256) k_table_join(int dim, int nchunks, const Segments g) {
+    __shared__ float part[256];
+    const int b = blockIdx.x;
+    const int k = g.owned[b];
+    if (k < 0) return;
+    const int width = min(dim, 256), slots = 256 / width;
+    const int slot = threadIdx.x / width, lane = threadIdx.x - slot * width;
+    const int col = blockIdx.y * 256 + lane;
+    const bool on = slot < slots && col < dim;
+    float s = 0.0f;
+    if (on) {
+        if (slot == 0) s = g.partial[((int64_t)b * 2 + 1) * dim + col];
+        for (int c = b + 1 + slot; c < nchunks && g.first_key[c] == k; c += slots)
+            s += g.partial[(int64_t)c * 2 * dim + col];
+    }
+    part[threadIdx.x] = s;
+    __syncthreads();
+    if (slot != 0 || !on) return;
+    for (int q = 1; q < slots; ++q) s += part[q * width + lane];
+    const float one[1] = {s};
+    store_row<1>(g, k, col, one);
 }
 
 struct GradLayout {
-    size_t keys, vals, skeys, svals, sort, total;
+    size_t keys[2], vals[2], hist, totals, valid, first_key, owned, partial, total;
+    int ntiles, passes, bits, chunks_max;
 };
 
-GradLayout grad_layout(int64_t n) {
-    GradLayout L;
-    size_t off = 0;
-    L.keys = off; off += align256((size_t)n * 8);
-    L.vals = off; off += align256((size_t)n * 4);
-    L.skeys = off; off += align256((size_t)n * 8);
-    L.svals = off; off += align256((size_t)n * 4);
-    L.sort = off; off += radix_sort_workspace_bytes(n);
-    L.total = off;
-    return L;
+constexpr int kMinRun = 4, kMaxRun = 48;  // rows a slot adds: enough blocks for few rows, few borders for many
+
+int slots_for(int tile_units) { return std::max(1, std::min(32, 256 / tile_units)); }
+
+SegmentPlan segment_plan(int64_t n, int units) {
+    SegmentPlan p;
+    p.units = units;
+    p.tile_units = std::min(units, 256);
+    p.slots = slots_for(p.tile_units);
+    const int64_t want = ceil_div(n, (int64_t)p.slots * kSMs * 4);
+    p.run = (int)std::max<int64_t>(kMinRun, std::min<int64_t>(kMaxRun, want));
+    p.chunk = p.slots * p.run;
+    p.nchunks = (int)std::max<int64_t>(1, ceil_div(n, p.chunk));
+    return p;
 }
 
 int bits_of(int64_t v) {
     int b = 0;
     while (v >> b) ++b;
     return b;
+}
+
+
+GradLayout grad_layout(int64_t n, int64_t rows, int dim) {
+    GradLayout L;
+    L.ntiles = (int)ceil_div(n, kSortTile);
+    L.bits = bits_of(std::max<int64_t>(rows, 1) - 1);
+    L.passes = std::max(1, (L.bits + kMaxDigitBits - 1) / kMaxDigitBits);
+    const int digit = (L.bits + L.passes - 1) / L.passes;
+    // the launch picks its unit from the gradients' alignment: room for either
+    L.chunks_max = 0;
+    for (int units = dim; units >= 1; units = units % 2 == 0 ? units / 2 : 0)
+        L.chunks_max = std::max(L.chunks_max, segment_plan(n, units).nchunks);
+    size_t off = 0;
+    for (int i = 0; i < 2; ++i) {
+        L.keys[i] = off; off += align256((size_t)n * 4);
+        L.vals[i] = off; off += align256((size_t)n * 4);
+    }
+    L.hist = off; off += align256((size_t)L.ntiles * ((size_t)1 << digit) * 4);
+    L.totals = off; off += align256(((size_t)1 << kMaxDigitBits) * 4);
+    L.valid = off; off += 256;
+    L.first_key = off; off += align256((size_t)L.chunks_max * 4);
+    L.owned = off; off += align256((size_t)L.chunks_max * 4);
+    L.partial = off; off += align256((size_t)L.chunks_max * 2 * dim * 4);
+    L.total = off;
+    return L;
 }
 
 }  // namespace
@@ -147,7 +564,7 @@ GS3D_API int gs3d_table_gradient_workspace_size(int64_t grad_rows, int64_t table
     if (grad_rows < 0 || grad_rows > kMaxRows || table_rows < 0 || table_rows > kMaxRows || dim < 1 ||
         dim > kMaxRowDim)
         return invalid("%lld rows, table of %lld rows, dim %d", (long long)grad_rows, (long long)table_rows, dim);
-    *bytes = grad_layout(std::max<int64_t>(grad_rows, 1)).total;
+    *bytes = grad_layout(std::max<int64_t>(grad_rows, 1), table_rows, dim).total;
     return GS3D_OK;
 }
 
@@ -167,29 +584,67 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     if (grads->rows > 0 && !indices && n_indices > 0) return invalid("NULL indices");
     if (table_grads->rows == 0) return GS3D_OK;
     const int64_t n = grads->rows;
-    const GradLayout L = grad_layout(std::max<int64_t>(n, 1));
+    const GradLayout L = grad_layout(std::max<int64_t>(n, 1), table_grads->rows, grads->dim);
     if (!workspace || workspace_bytes < L.total)
         return set_error("table gradient workspace %zu bytes < %zu", workspace_bytes, L.total), GS3D_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return invalid("workspace not 256-byte aligned");
     unsigned char* ws = static_cast<unsigned char*>(workspace);
-    int64_t* keys = reinterpret_cast<int64_t*>(ws + L.keys);
-    int32_t* vals = reinterpret_cast<int32_t*>(ws + L.vals);
-    int64_t* skeys = reinterpret_cast<int64_t*>(ws + L.skeys);
-    int32_t* svals = reinterpret_cast<int32_t*>(ws + L.svals);
+    const auto at = [&](size_t off) { return reinterpret_cast<int32_t*>(ws + off); };
+    const bool accumulate = (flags & GS3D_TABLE_ACCUMULATE) != 0;
+    float* out = static_cast<float*>(table_grads->data);
+    const KeySource src{indices, fgidx_to_gidx, device_counts, n_indices, (int32_t)n, (int32_t)table_grads->rows};
+    const ZeroRows zero{accumulate ? nullptr : out, table_grads->row_stride, (int32_t)table_grads->rows,
+                        table_grads->dim};
     ProfScope prof("table_grad", stream);
-    if (n > 0) {
-        k_table_keys<<<grid_for(n, 256, 8), 256, 0, stream>>>(indices, n_indices, fgidx_to_gidx, device_counts, n,
-                                                              table_grads->rows, keys, vals);
-        GS3D_LAUNCHED("k_table_keys");
-        GS3D_RETURN_IF(radix_sort_pairs(ws + L.sort, L.total - L.sort, keys, skeys, vals, svals, n, nullptr, n,
-                                        bits_of(table_grads->rows), stream));
+    int sorted = 0;
+    if (n <= kSortTile) {
+        const int64_t words = accumulate ? 0 : table_grads->rows * table_grads->dim;
+        const int fillers = (int)std::min<int64_t>(ceil_div(words, kSmallThreads * 8), 4 * kSMs);
+        k_sort_small<<<1 + fillers, kSmallThreads, 0, stream>>>(src, zero, L.bits, at(L.keys[0]), at(L.vals[0]),
+                                                                at(L.valid));
+        GS3D_LAUNCHED("k_sort_small");
+    } else {
+        SortPass p{nullptr, nullptr, nullptr, nullptr, at(L.hist), at(L.totals), at(L.valid), L.ntiles, 0, 0};
+        const int digit = (L.bits + L.passes - 1) / L.passes;
+        const size_t smem = radix_scatter_smem(digit);
+        GS3D_CUDA(cudaFuncSetAttribute(k_radix_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)radix_scatter_smem(kMaxDigitBits)),
+                  "scatter smem attribute");
+        for (int i = 0; i < L.passes; ++i) {
+            p.shift = i * digit;
+            p.bits = digit;
+            p.keys_out = at(L.keys[i & 1]);
+            p.vals_out = at(L.vals[i & 1]);
+            k_radix_count<<<L.ntiles, kSortThreads, 0, stream>>>(p, src, zero);
+            GS3D_LAUNCHED("k_radix_count");
+            k_radix_spine<<<1 << digit, kSortThreads, 0, stream>>>(p);
+            GS3D_LAUNCHED("k_radix_spine");
+            k_radix_scatter<<<L.ntiles, kSortThreads, smem, stream>>>(p, src);
+            GS3D_LAUNCHED("k_radix_scatter");
+            p.keys_in = p.keys_out;
+            p.vals_in = p.vals_out;
+            sorted = i & 1;
+        }
     }
+    if (n == 0) return GS3D_OK;
+    const Segments seg{at(L.keys[sorted]), at(L.vals[sorted]), at(L.valid), out, table_grads->row_stride, scale,
+                       accumulate ? 1 : 0, at(L.first_key), at(L.owned), reinterpret_cast<float*>(ws + L.partial)};
     return dispatch_type(grads->type, [&](auto t) {
         using T = typename decltype(t)::T;
-        k_table_reduce<T><<<(unsigned)table_grads->rows, 128, 0, stream>>>(
-            static_cast<const T*>(grads->data), grads->row_stride, grads->dim, skeys, svals, n, scale,
-            static_cast<float*>(table_grads->data), table_grads->row_stride, (flags & GS3D_TABLE_ACCUMULATE) ? 1 : 0);
-        GS3D_LAUNCHED("k_table_reduce");
+        const T* g = static_cast<const T*>(grads->data);
+        constexpr int N = 16 / (int)sizeof(T);
+        const bool wide = grads->dim % N == 0 && grads->row_stride % N == 0 &&
+                          (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+        const int per = wide ? N : 1;
+        const SegmentPlan pl = segment_plan(n, grads->dim / per);
+        const size_t smem = (size_t)pl.chunk * 8 + (size_t)pl.slots * 8 + (size_t)pl.slots * 2 * pl.tile_units * per * 4;
+        const dim3 grid(pl.nchunks, (unsigned)ceil_div(pl.units, pl.tile_units));
+        const int threads = pl.slots * pl.tile_units;
+        if (wide) k_table_segments<T, 16><<<grid, threads, smem, stream>>>(g, grads->row_stride, grads->dim, pl, seg);
+        else k_table_segments<T, (int)sizeof(T)><<<grid, threads, smem, stream>>>(g, grads->row_stride, grads->dim, pl, seg);
+        GS3D_LAUNCHED("k_table_segments");
+        k_table_join<<<dim3(pl.nchunks, (unsigned)ceil_div(grads->dim, 256)), 256, 0, stream>>>(grads->dim, pl.nchunks, seg);
+        GS3D_LAUNCHED("k_table_join");
         return GS3D_OK;
     });
 }

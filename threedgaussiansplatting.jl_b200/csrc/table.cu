@@ -14,11 +14,92 @@ int grid_for(int64_t items, int threads, int per_sm) {
     return (int)std::max<int64_t>(b, 1);
 }
 
+// ---- lookup ----------------------------------------------------------------------------------
+// Bound by the rows written (the table stays in L2). Three forms, by alignment:
+//   k_table_lookup_units   rows in units of N elements (16 bytes of the wider type): threads side by side on a
+//                          row's units, kLookupRows rows a thread, so that 8 independent loads are in flight
+//   k_table_lookup_flat    rows of any length, output contiguous: a thread fills N consecutive elements of the
+//                          output, across a row's end where it comes, and stores them at once
+//   k_table_lookup_scalar  everything else: an element a thread
+constexpr int kLookupRows = 8;
+
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Pack {
+    T e[N];
+};
+
 template <typename TI, typename TO>
-__global__ void __launch_bounds__(256) k_table_lookup(const TI* __restrict__ table, int64_t rows,
-                                                      int64_t table_stride, const int32_t* __restrict__ indices,
-                                                      float scale, TO* __restrict__ out, int64_t n,
-                                                      int64_t out_stride, int dim) {
+constexpr int lookup_pack() { return sizeof(TI) == 2 && sizeof(TO) == 2 ? 8 : 4; }
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(256) k_table_lookup_units(const TI* __restrict__ table, int rows,
+                                                            int64_t table_stride,
+                                                            const int32_t* __restrict__ indices, float scale,
+                                                            TO* __restrict__ out, int n, int64_t out_stride,
+                                                            int units, int tile_units, int slots) {
+    constexpr int N = lookup_pack<TI, TO>();
+    const int slot = threadIdx.x / tile_units;
+    const int unit = blockIdx.y * tile_units + threadIdx.x - slot * tile_units;
+    if (unit >= units) return;
+    const int64_t first = (int64_t)blockIdx.x * slots * kLookupRows + slot;
+    int k[kLookupRows];
+#pragma unroll
+    for (int q = 0; q < kLookupRows; ++q) {
+        const int64_t i = first + q * slots;
+        k[q] = i < n ? __ldg(indices + i) : 0;
+    }
+    Pack<TI, N> v[kLookupRows];
+#pragma unroll
+    for (int q = 0; q < kLookupRows; ++q)
+        if (k[q] >= 1 && k[q] <= rows)
+            v[q] = *reinterpret_cast<const Pack<TI, N>*>(table + (int64_t)(k[q] - 1) * table_stride + unit * N);
+#pragma unroll
+    for (int q = 0; q < kLookupRows; ++q) {
+        const int64_t i = first + q * slots;
+        if (i >= n) break;
+        const bool valid = k[q] >= 1 && k[q] <= rows;
+        Pack<TO, N> o;
+#pragma unroll
+        for (int c = 0; c < N; ++c) o.e[c] = from_f32<TO>(valid ? to_f32(v[q].e[c]) * scale : 0.0f);
+        *reinterpret_cast<Pack<TO, N>*>(out + i * out_stride + unit * N) = o;
+    }
+}
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(256) k_table_lookup_flat(const TI* __restrict__ table, int rows,
+                                                           int64_t table_stride,
+                                                           const int32_t* __restrict__ indices, float scale,
+                                                           TO* __restrict__ out, int64_t total, int dim) {
+    constexpr int N = lookup_pack<TI, TO>();
+    const int64_t e0 = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * N;
+    if (e0 >= total) return;
+    int64_t r = e0 / dim;
+    int c = (int)(e0 - r * dim);
+    int k = __ldg(indices + r);
+    Pack<TO, N> o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        float v = 0.0f;
+        if (e0 + j < total && k >= 1 && k <= rows) v = to_f32(__ldg(table + (int64_t)(k - 1) * table_stride + c)) * scale;
+        o.e[j] = from_f32<TO>(v);
+        if (++c == dim && e0 + j + 1 < total) {
+            c = 0;
+            k = __ldg(indices + ++r);
+        }
+    }
+    if (e0 + N <= total) {
+        *reinterpret_cast<Pack<TO, N>*>(out + e0) = o;
+    } else {
+        for (int j = 0; e0 + j < total; ++j) out[e0 + j] = o.e[j];
+    }
+}
+
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(256) k_table_lookup_scalar(const TI* __restrict__ table, int rows,
+                                                             int64_t table_stride,
+                                                             const int32_t* __restrict__ indices, float scale,
+                                                             TO* __restrict__ out, int64_t n, int64_t out_stride,
+                                                             int dim) {
     const int64_t total = n * dim;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
          i += (int64_t)gridDim.x * blockDim.x) {
@@ -29,6 +110,36 @@ __global__ void __launch_bounds__(256) k_table_lookup(const TI* __restrict__ tab
         if (k >= 1 && k <= rows) v = to_f32(table[(int64_t)(k - 1) * table_stride + c]) * scale;
         out[r * out_stride + c] = from_f32<TO>(v);
     }
+}
+
+template <typename T>
+bool packs(const gs3d_rows* r, int n) {
+    return r->dim % n == 0 && r->row_stride % n == 0 && reinterpret_cast<uintptr_t>(r->data) % (n * sizeof(T)) == 0;
+}
+
+template <typename TI, typename TO>
+int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, const gs3d_rows* out,
+                  cudaStream_t stream) {
+    constexpr int N = lookup_pack<TI, TO>();
+    const TI* t = static_cast<const TI*>(table->data);
+    TO* o = static_cast<TO*>(out->data);
+    const int rows = (int)table->rows, dim = out->dim;
+    const int64_t n = out->rows, total = n * dim;
+    if (packs<TI>(table, N) && packs<TO>(out, N)) {
+        const int units = dim / N, tile_units = std::min(units, 256), slots = std::max(1, 256 / tile_units);
+        const dim3 grid((unsigned)ceil_div(n, (int64_t)slots * kLookupRows), (unsigned)ceil_div(units, tile_units));
+        k_table_lookup_units<TI, TO><<<grid, slots * tile_units, 0, stream>>>(
+            t, rows, table->row_stride, indices, scale, o, (int)n, out->row_stride, units, tile_units, slots);
+    } else if (out->row_stride == dim && reinterpret_cast<uintptr_t>(o) % (N * sizeof(TO)) == 0 &&
+               total / N / 256 < INT_MAX) {
+        k_table_lookup_flat<TI, TO><<<(unsigned)ceil_div(total, N * 256), 256, 0, stream>>>(
+            t, rows, table->row_stride, indices, scale, o, total, dim);
+    } else {
+        k_table_lookup_scalar<TI, TO><<<grid_for(total, 256, 8), 256, 0, stream>>>(
+            t, rows, table->row_stride, indices, scale, o, n, out->row_stride, dim);
+    }
+    GS3D_LAUNCHED("k_table_lookup");
+    return GS3D_OK;
 }
 
 // ---- gradient --------------------------------------------------------------------------------
@@ -550,11 +661,7 @@ GS3D_API int gs3d_table_lookup(const gs3d_rows* table, const int32_t* indices, f
         using TI = typename decltype(ti)::T;
         return dispatch_type(out->type, [&](auto to) {
             using TO = typename decltype(to)::T;
-            k_table_lookup<TI, TO><<<grid_for(out->rows * out->dim, 256, 8), 256, 0, stream>>>(
-                static_cast<const TI*>(table->data), table->rows, table->row_stride, indices, scale,
-                static_cast<TO*>(out->data), out->rows, out->row_stride, out->dim);
-            GS3D_LAUNCHED("k_table_lookup");
-            return GS3D_OK;
+            return launch_lookup<TI, TO>(table, indices, scale, out, stream);
         });
     });
 }

@@ -2,6 +2,8 @@
 //   gs3d_table_lookup    out[i] = scale * table[indices[i]]
 //   gs3d_table_gradient  table_grads[k] = scale * sum of grads[f] over the rows f with index k + 1,
 //                        by the rows sorted by index (stable), so the order of every sum is fixed
+#include <type_traits>
+
 #include "common.cuh"
 #include "internal.h"
 #include "rows.cuh"
@@ -17,16 +19,25 @@ int grid_for(int64_t items, int threads, int per_sm) {
 // ---- lookup ----------------------------------------------------------------------------------
 // Bound by the rows written (the table stays in L2). Three forms, by alignment:
 //   k_table_lookup_units   rows in units of N elements (16 bytes of the wider type): threads side by side on a
-//                          row's units, kLookupRows rows a thread, so that 8 independent loads are in flight
+//                          row's units, kLookupRows rows a thread, as many independent loads in flight
 //   k_table_lookup_flat    rows of any length, output contiguous: a thread fills N consecutive elements of the
 //                          output, across a row's end where it comes, and stores them at once
 //   k_table_lookup_scalar  everything else: an element a thread
-constexpr int kLookupRows = 8;
+constexpr int kLookupRows = 4;  // 1 / 2 / 4 / 8: 129 / 103 / 94 / 117 us at 3M x 48 fp32 (a write-only fill: 79)
 
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Pack {
     T e[N];
 };
+
+// A pack of 8 or 16 bytes to memory that is not read again soon: streamed, so that it does not push
+// the table out of L2 (104 us without, 94 with).
+template <typename T, int N>
+__device__ __forceinline__ void store_streaming(T* p, const Pack<T, N>& v) {
+    using W = typename std::conditional<sizeof(v) == 16, uint4, uint2>::type;
+    static_assert(sizeof(v) == sizeof(W), "packs of 8 or 16 bytes");
+    __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&v));
+}
 
 template <typename TI, typename TO>
 constexpr int lookup_pack() { return sizeof(TI) == 2 && sizeof(TO) == 2 ? 8 : 4; }
@@ -61,7 +72,7 @@ __global__ void __launch_bounds__(256) k_table_lookup_units(const TI* __restrict
         Pack<TO, N> o;
 #pragma unroll
         for (int c = 0; c < N; ++c) o.e[c] = from_f32<TO>(valid ? to_f32(v[q].e[c]) * scale : 0.0f);
-        *reinterpret_cast<Pack<TO, N>*>(out + i * out_stride + unit * N) = o;
+        store_streaming(out + i * out_stride + unit * N, o);
     }
 }
 
@@ -88,7 +99,7 @@ __global__ void __launch_bounds__(256) k_table_lookup_flat(const TI* __restrict_
         }
     }
     if (e0 + N <= total) {
-        *reinterpret_cast<Pack<TO, N>*>(out + e0) = o;
+        store_streaming(out + e0, o);
     } else {
         for (int j = 0; e0 + j < total; ++j) out[e0 + j] = o.e[j];
     }
@@ -156,7 +167,7 @@ int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, c
 // The order of every sum follows from the sorted order alone, whatever the number of rows that share
 // an index: no atomics, and a row that half of the Gaussians use is spread over the GPU like any other.
 
-constexpr int kSortThreads = 256;
+constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortTile = 4096;
 constexpr int kSortRounds = kSortTile / kSortThreads;
@@ -171,12 +182,20 @@ struct KeySource {
     int32_t n, rows;
 
     __device__ __forceinline__ int live() const { return counts ? min(max(counts[0], 0), n) : n; }
-    __device__ __forceinline__ int key(int f, int live_rows) const {
-        if (f >= live_rows) return -1;
-        const int64_t i = f2g ? (int64_t)f2g[f] - 1 : f;
-        if (i < 0 || i >= n_indices) return -1;
-        const int k = indices[i];
-        return k >= 1 && k <= rows ? k - 1 : -1;
+    // The keys of rows f0, f0 + 32, ...: all of a step's loads before the next step's.
+    template <int R>
+    __device__ __forceinline__ void keys(int f0, int (&key)[R]) const {
+        const int last = live();
+        int64_t i[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int f = f0 + 32 * r;
+            i[r] = f >= last ? -1 : f2g ? (int64_t)__ldg(f2g + f) - 1 : f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) key[r] = i[r] >= 0 && i[r] < n_indices ? __ldg(indices + i[r]) : 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) key[r] = key[r] >= 1 && key[r] <= rows ? key[r] - 1 : -1;
     }
 };
 
@@ -203,52 +222,54 @@ struct ZeroRows {
 };
 
 struct SortPass {
-    const int32_t* keys_in;  // NULL: the first pass, keys from the source, values f
-    const int32_t* vals_in;
+    int32_t* keys_in;  // the first pass: all rows' keys, -1 without one, written by its count kernel
+    const int32_t* vals_in;  // NULL: the first pass, values are the rows themselves
     int32_t* keys_out;
     int32_t* vals_out;
     int32_t* hist;    // [bin][tile]: counts, then their exclusive scan over the tiles
     int32_t* totals;  // [bin]
     int32_t* valid;   // number of rows with a valid index (written by the first pass)
-    int32_t ntiles, shift, bits;
+    int32_t n, ntiles, shift, bits;
 };
 
-// The 16 keys of a thread, warp by warp in row order; -1: none.
-__device__ __forceinline__ void load_tile_keys(const SortPass& p, const KeySource& src, int tile, int (&key)[kSortRounds]) {
-    const int base = tile * kSortTile + (threadIdx.x >> 5) * (kSortRounds * 32) + (threadIdx.x & 31);
-    if (p.keys_in) {
-        const int m = *p.valid;
-#pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) key[r] = base + 32 * r < m ? p.keys_in[base + 32 * r] : -1;
-    } else {
-        const int live = src.live();
-#pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) key[r] = src.key(base + 32 * r, live);
-    }
+// A thread's place in a tile: its rows are place, place + 32, ..., warp after warp in row order.
+__device__ __forceinline__ int tile_place(int tile) {
+    return tile * kSortTile + (threadIdx.x >> 5) * (kSortRounds * 32) + (threadIdx.x & 31);
 }
 
 __global__ void __launch_bounds__(kSortThreads) k_radix_count(const SortPass p, const KeySource src,
                                                               const ZeroRows zero) {
     __shared__ int bins[1 << kMaxDigitBits];
-    const int nbins = 1 << p.bits, tile = blockIdx.x;
+    const int nbins = 1 << p.bits, tile = blockIdx.x, place = tile_place(tile);
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) bins[b] = 0;
     int key[kSortRounds];
-    load_tile_keys(p, src, tile, key);
+    if (!p.vals_in) {
+        src.keys(place, key);
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r)
+            if (place + 32 * r < p.n) p.keys_in[place + 32 * r] = key[r];
+    } else {
+        const int m = *p.valid;
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) key[r] = place + 32 * r < m ? p.keys_in[place + 32 * r] : -1;
+    }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r)
         if (key[r] >= 0) atomicAdd(&bins[(key[r] >> p.shift) & (nbins - 1)], 1);
-    if (!p.keys_in) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
+    if (!p.vals_in) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
     __syncthreads();
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) p.hist[(int64_t)b * p.ntiles + tile] = bins[b];
 }
 
+constexpr int kSpineThreads = 256;
+
 // Block b: exclusive scan of bin b's counts over the tiles.
-__global__ void __launch_bounds__(kSortThreads) k_radix_spine(const SortPass p) {
+__global__ void __launch_bounds__(kSpineThreads) k_radix_spine(const SortPass p) {
     __shared__ int sm[33];
     int32_t* row = p.hist + (int64_t)blockIdx.x * p.ntiles;
     int carry = 0, tot;
-    for (int t0 = 0; t0 < p.ntiles; t0 += kSortThreads) {
+    for (int t0 = 0; t0 < p.ntiles; t0 += kSpineThreads) {
         const int t = t0 + threadIdx.x;
         const int ex = block_exclusive_scan(t < p.ntiles ? row[t] : 0, sm, &tot);
         if (t < p.ntiles) row[t] = carry + ex;
@@ -261,7 +282,7 @@ size_t radix_scatter_smem(int bits) {
     return (size_t)kSortTile * 8 + (size_t)(1 << bits) * (8 + 2 * kSortWarps);
 }
 
-__global__ void __launch_bounds__(kSortThreads) k_radix_scatter(const SortPass p, const KeySource src) {
+__global__ void __launch_bounds__(kSortThreads, 3) k_radix_scatter(const SortPass p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int sm[33];
     const int nbins = 1 << p.bits, tile = blockIdx.x;
@@ -271,9 +292,15 @@ __global__ void __launch_bounds__(kSortThreads) k_radix_scatter(const SortPass p
     int32_t* dest = start + nbins;                               // its place in the output, minus start
     uint16_t* wcount = reinterpret_cast<uint16_t*>(dest + nbins);  // [warp][bin]
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int key[kSortRounds];
-    load_tile_keys(p, src, tile, key);
-    for (int i = threadIdx.x; i < nbins * kSortWarps; i += kSortThreads) wcount[i] = 0;
+    const int place = tile_place(tile), m = p.vals_in ? *p.valid : p.n;
+    int key[kSortRounds], val[kSortRounds];
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+        const int i = place + 32 * r;
+        key[r] = i < m ? p.keys_in[i] : -1;
+        val[r] = p.vals_in && i < m ? p.vals_in[i] : i;
+    }
+    for (int i = threadIdx.x; i < nbins * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(wcount)[i] = 0;
     __syncthreads();
     // stable rank of every key among its warp's keys of the same digit
     int rank[kSortRounds];
@@ -312,16 +339,15 @@ __global__ void __launch_bounds__(kSortThreads) k_radix_scatter(const SortPass p
             dest[b] = base + p.hist[(int64_t)b * p.ntiles + tile] - st;
         }
     }
-    if (!p.keys_in && tile == 0 && threadIdx.x == 0) *p.valid = everywhere;
+    if (!p.vals_in && tile == 0 && threadIdx.x == 0) *p.valid = everywhere;
     __syncthreads();
-    const int base = tile * kSortTile + w * (kSortRounds * 32) + lane;
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r)
         if (key[r] >= 0) {
             const int d = (key[r] >> p.shift) & (nbins - 1);
             const int at = start[d] + wcount[w * nbins + d] + rank[r];
             keys[at] = key[r];
-            vals[at] = p.keys_in ? p.vals_in[base + 32 * r] : base + 32 * r;
+            vals[at] = val[r];
         }
     __syncthreads();
     for (int i = threadIdx.x; i < here; i += kSortThreads) {
@@ -350,18 +376,17 @@ __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource sr
     }
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned below = (1u << lane) - 1u;
-    const int live = src.live();
-    int count = src.n;
+    int count = 0;
     for (int shift = 0; shift < max(bits, 1); shift += 8) {
         const bool first = shift == 0;
         int key[kSmallRounds], val[kSmallRounds], rank[kSmallRounds];
+        const int place = w * (kSmallRounds * 32) + lane;
+        if (first) src.keys(place, key);
 #pragma unroll
         for (int r = 0; r < kSmallRounds; ++r) {
-            const int i = w * (kSmallRounds * 32) + r * 32 + lane;
-            key[r] = -1;
-            val[r] = i;
-            if (first) key[r] = src.key(i, live);
-            else if (i < count) key[r] = keys[i], val[r] = vals[i];
+            const int i = place + 32 * r;
+            if (first) val[r] = i;
+            else key[r] = i < count ? keys[i] : -1, val[r] = vals[i];
         }
         for (int i = threadIdx.x; i < kSmallWarps * 256; i += kSmallThreads) (&wcount[0][0])[i] = 0;
         __syncthreads();
@@ -413,8 +438,17 @@ struct RowUnit {
     static constexpr int N = VB / (int)sizeof(T);
     T e[N];
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (VB == 16) *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(p));
-        else e[0] = __ldg(p);
+        // a row is read once, from a place of its own: nothing for L1, and 64 bytes a DRAM access
+        // (a 3M x 192 B gather alone: 117 us plain, 107 us so)
+        if constexpr (VB == 16) {
+            uint4 v;
+            asm("ld.global.nc.L1::no_allocate.L2::64B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                : "l"(p));
+            *reinterpret_cast<uint4*>(e) = v;
+        } else {
+            e[0] = __ldg(p);
+        }
     }
 };
 
@@ -451,7 +485,7 @@ template <typename T, int VB>
 __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ grads, int64_t stride, int dim,
                                                         const SegmentPlan pl, const Segments g) {
     using Unit = RowUnit<T, VB>;
-    constexpr int N = Unit::N, AHEAD = 8;
+    constexpr int N = Unit::N, AHEAD = 4;
     extern __shared__ __align__(16) unsigned char smem[];
     int32_t* sk = reinterpret_cast<int32_t*>(smem);  // the chunk's indices and rows
     int32_t* sv = sk + pl.chunk;
@@ -565,27 +599,53 @@ __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ gr
     }
 }
 
-__global__ void __launch_bounds__(256) k_table_join(int dim, int nchunks, const Segments g) {
-    __shared__ float part[256];
-    const int b = blockIdx.x;
-    const int k = g.owned[b];
-    if (k < 0) return;
-    const int width = min(dim, 256), slots = 256 / width;
-    const int slot = threadIdx.x / width, lane = threadIdx.x - slot * width;
-    const int col = blockIdx.y * 256 + lane;
-    const bool on = slot < slots && col < dim;
-    float s = 0.0f;
-    if (on) {
-        if (slot == 0) s = g.partial[((int64_t)b * 2 + 1) * dim + col];
-        for (int c = b + 1 + slot; c < nchunks && g.first_key[c] == k; c += slots)
-            s += g.partial[(int64_t)c * 2 * dim + col];
+// A warp per chunk for the runs of up to 32 partial sums behind the first (nearly all: an average run is
+// shorter than a chunk), the whole block for the longer ones it meets.
+constexpr int kJoinWarps = 8;
+
+__global__ void __launch_bounds__(32 * kJoinWarps) k_table_join(int dim, int nchunks, const Segments g) {
+    __shared__ int long_run[kJoinWarps];
+    __shared__ float part[32 * kJoinWarps];
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.x * kJoinWarps + w;
+    const int k = b < nchunks ? g.owned[b] : -1;
+    const int next = b + 1 + lane;
+    const unsigned same = __ballot_sync(0xffffffffu, k >= 0 && next < nchunks && g.first_key[next] == k);
+    if (lane == 0) long_run[w] = same == 0xffffffffu ? k : -1;
+    if (k >= 0 && same != 0xffffffffu) {
+        const int more = __ffs(~same) - 1;
+        for (int col = blockIdx.y * 256 + lane; col < min(dim, (int)blockIdx.y * 256 + 256); col += 32) {
+            float s = g.partial[((int64_t)b * 2 + 1) * dim + col];
+#pragma unroll 4
+            for (int c = 1; c <= more; ++c) s += g.partial[(int64_t)(b + c) * 2 * dim + col];
+            const float one[1] = {s};
+            store_row<1>(g, k, col, one);
+        }
     }
-    part[threadIdx.x] = s;
     __syncthreads();
-    if (slot != 0 || !on) return;
-    for (int q = 1; q < slots; ++q) s += part[q * width + lane];
-    const float one[1] = {s};
-    store_row<1>(g, k, col, one);
+    const int width = min(dim, 256), slots = 256 / width;
+    const int slot = threadIdx.x / width, col = blockIdx.y * 256 + threadIdx.x - slot * width;
+    const bool on = slot < slots && col < dim;
+    for (int q = 0; q < kJoinWarps; ++q) {
+        const int lk = long_run[q];
+        if (lk < 0) continue;
+        const int lb = blockIdx.x * kJoinWarps + q;
+        float s = 0.0f;
+        if (on) {
+            if (slot == 0) s = g.partial[((int64_t)lb * 2 + 1) * dim + col];
+#pragma unroll 4
+            for (int c = lb + 1 + slot; c < nchunks && g.first_key[c] == lk; c += slots)
+                s += g.partial[(int64_t)c * 2 * dim + col];
+        }
+        part[threadIdx.x] = s;
+        __syncthreads();
+        if (slot == 0 && on) {
+            for (int t = 1; t < slots; ++t) s += part[t * width + threadIdx.x];
+            const float one[1] = {s};
+            store_row<1>(g, lk, col, one);
+        }
+        __syncthreads();
+    }
 }
 
 struct GradLayout {
@@ -711,7 +771,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
                                                                 at(L.valid));
         GS3D_LAUNCHED("k_sort_small");
     } else {
-        SortPass p{nullptr, nullptr, nullptr, nullptr, at(L.hist), at(L.totals), at(L.valid), L.ntiles, 0, 0};
+        SortPass p{at(L.keys[1]), nullptr, nullptr, nullptr, at(L.hist), at(L.totals), at(L.valid), (int32_t)n, L.ntiles, 0, 0};
         const int digit = (L.bits + L.passes - 1) / L.passes;
         const size_t smem = radix_scatter_smem(digit);
         GS3D_CUDA(cudaFuncSetAttribute(k_radix_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -724,9 +784,9 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
             p.vals_out = at(L.vals[i & 1]);
             k_radix_count<<<L.ntiles, kSortThreads, 0, stream>>>(p, src, zero);
             GS3D_LAUNCHED("k_radix_count");
-            k_radix_spine<<<1 << digit, kSortThreads, 0, stream>>>(p);
+            k_radix_spine<<<1 << digit, kSpineThreads, 0, stream>>>(p);
             GS3D_LAUNCHED("k_radix_spine");
-            k_radix_scatter<<<L.ntiles, kSortThreads, smem, stream>>>(p, src);
+            k_radix_scatter<<<L.ntiles, kSortThreads, smem, stream>>>(p);
             GS3D_LAUNCHED("k_radix_scatter");
             p.keys_in = p.keys_out;
             p.vals_in = p.vals_out;
@@ -750,7 +810,8 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
         if (wide) k_table_segments<T, 16><<<grid, threads, smem, stream>>>(g, grads->row_stride, grads->dim, pl, seg);
         else k_table_segments<T, (int)sizeof(T)><<<grid, threads, smem, stream>>>(g, grads->row_stride, grads->dim, pl, seg);
         GS3D_LAUNCHED("k_table_segments");
-        k_table_join<<<dim3(pl.nchunks, (unsigned)ceil_div(grads->dim, 256)), 256, 0, stream>>>(grads->dim, pl.nchunks, seg);
+        k_table_join<<<dim3((unsigned)ceil_div(pl.nchunks, kJoinWarps), (unsigned)ceil_div(grads->dim, 256)),
+                       32 * kJoinWarps, 0, stream>>>(grads->dim, pl.nchunks, seg);
         GS3D_LAUNCHED("k_table_join");
         return GS3D_OK;
     });

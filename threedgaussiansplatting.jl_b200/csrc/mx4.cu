@@ -305,78 +305,89 @@ __global__ void __launch_bounds__(256) k_mx4_quantise(const T* __restrict__ x, i
 }
 
 // ---- dequantise ------------------------------------------------------------------------------
-// Rows of whole blocks, back to back: the codes, scales and values of all rows are one run each. Eight
-// elements (a word of codes) a thread.
+// Rows of whole blocks, back to back: the codes, scales and values of all rows are one run each. A
+// thread fills kDequantisePacks times 16 bytes of output, next to its neighbours' each time; the word of
+// codes that it takes its half (or all) of is read by both.
+constexpr int kDequantisePacks = 4;
+
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) k_mx4_dequantise_blocks(const uint32_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales,
                                                                const float* __restrict__ tensor_scale,
-                                                               int64_t words, T* __restrict__ out) {
-    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T);
+                                                               int64_t packs, T* __restrict__ out) {
+    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T), R = kDequantisePacks;
     const float g = FMT == GS3D_NVFP4 ? __ldg(tensor_scale) : 1.0f;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= words) return;
-    __half2 e[4];
-    e2m1_word_half(__ldg(codes + i), e);
-    const Mx4Decode<FMT> d(scales[i / (BS / 8)], g);
-    Pack<T, N> o[8 / N];
+    const int64_t first = (int64_t)blockIdx.x * (256 * R) + threadIdx.x;
+    uint32_t word[R], scale[R];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float2 v = d.value(e[k]);
-        o[2 * k / N].e[2 * k % N] = from_f32<T>(v.x);
-        o[2 * k / N].e[2 * k % N + 1] = from_f32<T>(v.y);
+    for (int q = 0; q < R; ++q) {
+        const int64_t i = min(first + 256 * q, packs - 1);
+        word[q] = __ldg(codes + i * N / 8);
+        scale[q] = __ldg(scales + i * N / BS);
     }
 #pragma unroll
-    for (int k = 0; k < 8 / N; ++k) reinterpret_cast<Pack<T, N>*>(out + i * 8)[k] = o[k];
+    for (int q = 0; q < R; ++q) {
+        const int64_t i = first + 256 * q;
+        const Mx4Decode<FMT> d(scale[q], g);
+        Pack<T, N> o;
+        if constexpr (N == 8) {
+            __half2 e[4];
+            e2m1_word_half(word[q], e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 v = mx4_value(d, e[k]);
+                o.e[k] = from_f32<T>(v.x);
+                o.e[k + 4] = from_f32<T>(v.y);
+            }
+        } else {
+            if (threadIdx.x & 1) word[q] >>= 16;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float2 v = mx4_value(d, e2m1_pair_half(word[q] >> (8 * k)));
+                o.e[2 * k] = from_f32<T>(v.x);
+                o.e[2 * k + 1] = from_f32<T>(v.y);
+            }
+        }
+        if (i < packs) __stcs(reinterpret_cast<uint4*>(out) + i, *reinterpret_cast<const uint4*>(&o));
+    }
 }
 
-// Rows of any length, back to back: a CTA takes `per` rows' codes and scales through shared memory,
-// and its threads fill the output's 16-byte packs across the rows' ends.
+// Rows of any length, back to back: a CTA takes `per` rows' codes and scales through shared memory, a
+// block of a row a thread, and hands the values back as one range of bytes.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) k_mx4_dequantise_rows(const uint8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales,
                                                              const float* __restrict__ tensor_scale, int64_t rows,
                                                              int dim, int per, T* __restrict__ out) {
-    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T);
+    constexpr int BS = Mx4Block<FMT>::size;
     extern __shared__ __align__(16) unsigned char smem[];
     const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2;
     const float g = FMT == GS3D_NVFP4 ? __ldg(tensor_scale) : 1.0f;
     const int64_t r0 = (int64_t)blockIdx.x * per;
     const int mine = (int)min((int64_t)per, rows - r0);
     const uint8_t* gc = codes + r0 * cb;
-    const uint8_t* gs = scales + r0 * nb;
-    unsigned char* ss = smem + ((16 + (size_t)per * cb + 15) & ~(size_t)15);
+    unsigned char* go = reinterpret_cast<unsigned char*>(out + r0 * dim);
+    unsigned char* so = smem + ((16 + (size_t)per * cb + 15) & ~(size_t)15);
     copy_in(smem, gc, (int64_t)mine * cb);
-    copy_in(ss, gs, (int64_t)mine * nb);
     __syncthreads();
     const unsigned char* sc = smem + head_of(gc);
-    ss += head_of(gs);
-    const int head = head_of(out + r0 * dim) / (int)sizeof(T);  // elements behind a 16-byte border
-    T* o0 = out + r0 * dim - head;
-    const int end = head + mine * dim;
-    for (int p = threadIdx.x; p * N < end; p += blockDim.x) {
-        Pack<T, N> o;
-        int e = p * N - head;
-        int r = e > 0 ? e / dim : 0, c = max(e, 0) - r * dim;
+    T* sv = reinterpret_cast<T*>(so + head_of(go));
+    for (int i = threadIdx.x; i < mine * nb; i += blockDim.x) {
+        const int r = i / nb, b = i - r * nb;
+        const int len = min(BS, dim - b * BS);
+        const Mx4Decode<FMT> d(__ldg(scales + r0 * nb + i), g);
+        const unsigned char* c = sc + r * cb + b * (BS / 2);
+        T* o = sv + r * dim + b * BS;
 #pragma unroll
-        for (int k = 0; k < N; ++k, ++e) {
-            float v = 0.0f;
-            if (e >= 0 && r < mine) {
-                const Mx4Decode<FMT> d(ss[r * nb + c / BS], g);
-                const float2 two = d.value(e2m1_pair_half(sc[r * cb + c / 2]));
-                v = c & 1 ? two.y : two.x;
-                if (++c == dim) c = 0, ++r;
+        for (int k = 0; k < BS; k += 2)
+            if (k < len) {
+                const float2 v = mx4_value(d, e2m1_pair_half(c[k / 2]));
+                o[k] = from_f32<T>(v.x);
+                if (k + 1 < len) o[k + 1] = from_f32<T>(v.y);
             }
-            o.e[k] = from_f32<T>(v);
-        }
-        if (p * N >= head && (p + 1) * N <= end) {
-            *reinterpret_cast<Pack<T, N>*>(o0 + p * N) = o;
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (p * N + k >= head && p * N + k < end) o0[p * N + k] = o.e[k];
-        }
     }
+    __syncthreads();
+    copy_out(go, so, (int64_t)mine * dim * sizeof(T));
 }
 
 // Rows apart or long: an element a thread.
@@ -394,17 +405,16 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise(const uint8_t* __restric
         const int64_t r = i / dim;
         const int k = (int)(i - r * dim);
         const Mx4Decode<FMT> d(scales[r * nb + k / BS], g);
-        const float2 two = d.value(e2m1_pair_half(codes[r * cb + k / 2]));
+        const float2 two = mx4_value(d, e2m1_pair_half(codes[r * cb + k / 2]));
         out[r * stride + k] = from_f32<T>(k & 1 ? two.y : two.x);
     }
 }
 
-constexpr int kRowsBytes = 16 << 10;  // of a CTA's rows in shared memory (three CTAs' worth of 256 threads fit)
+constexpr int kRowsBytes = 16 << 10;  // the most that a CTA's rows take in shared memory
 
-// Rows a CTA of the *_rows kernels takes: about kRowsBytes of them, fewer where that leaves SMs without.
-int rows_per_cta(int64_t rows, int row_bytes) {
-    const int64_t fit = std::max(1, kRowsBytes / row_bytes);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(fit, ceil_div(rows, 4 * (int64_t)device_sm_count())));
+// Rows a CTA of the *_rows kernels takes: a block for each of its 256 threads, as far as they fit.
+int rows_per_cta(int row_bytes, int row_blocks) {
+    return std::max(1, std::min(kRowsBytes / row_bytes, 256 / row_blocks));
 }
 
 template <typename T, int FMT>
@@ -419,7 +429,7 @@ int launch_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t s
         k_mx4_quantise_blocks<T, FMT><<<(unsigned)ceil_div(blocks, 256), 256, 0, stream>>>(
             in, blocks, x->row_stride, nb, flat, out->codes, out->scales, out->tensor_scale);
     } else if (flat && dim * (int)sizeof(T) <= kRowsBytes) {
-        const int per = rows_per_cta(x->rows, dim * (int)sizeof(T));
+        const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
         const size_t smem = ((16 + (size_t)per * dim * sizeof(T) + 15) & ~(size_t)15) + 16 +
                             (size_t)per * mx4_code_bytes(dim) + 16;
         k_mx4_quantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), 256, smem, stream>>>(
@@ -434,19 +444,19 @@ int launch_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t s
 
 template <typename T, int FMT>
 int launch_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, cudaStream_t stream) {
-    constexpr int BS = Mx4Block<FMT>::size;
+    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T);
     T* o = static_cast<T*>(out->data);
     const int dim = x->dim;
-    const int64_t words = x->rows * dim / 8;
+    const int64_t packs = x->rows * dim / N;
     const bool flat = out->row_stride == dim;
     if (flat && dim % BS == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
-        reinterpret_cast<uintptr_t>(x->codes) % 4 == 0 && words / 256 < INT_MAX) {
-        k_mx4_dequantise_blocks<T, FMT><<<(unsigned)ceil_div(words, 256), 256, 0, stream>>>(
-            reinterpret_cast<const uint32_t*>(x->codes), x->scales, x->tensor_scale, words, o);
+        reinterpret_cast<uintptr_t>(x->codes) % 4 == 0 && packs / 256 < INT_MAX) {
+        k_mx4_dequantise_blocks<T, FMT><<<(unsigned)ceil_div(packs, 256 * kDequantisePacks), 256, 0, stream>>>(
+            reinterpret_cast<const uint32_t*>(x->codes), x->scales, x->tensor_scale, packs, o);
     } else if (flat && dim * (int)sizeof(T) <= kRowsBytes) {
-        const int per = rows_per_cta(x->rows, dim * (int)sizeof(T));
+        const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
         const size_t smem = ((16 + (size_t)per * mx4_code_bytes(dim) + 15) & ~(size_t)15) + 16 +
-                            (size_t)per * mx4_blocks(dim, FMT) + 16;
+                            (size_t)per * dim * sizeof(T) + 16;
         k_mx4_dequantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), 256, smem, stream>>>(
             x->codes, x->scales, x->tensor_scale, x->rows, dim, per, o);
     } else {
@@ -474,66 +484,143 @@ int launch_tensor_scale(const gs3d_rows* x, float* tensor_scale, cudaStream_t st
 }
 
 // ---- colours ---------------------------------------------------------------------------------
-// The coefficients of Gaussian i. WHOLE: rows of exactly the rendered degree, their codes aligned to
-// 8 bytes at degree 3 (24 bytes a row) and to 2 below (2, 6 and 14 bytes): wide loads, and every
-// element's byte and block known at compile time. Else element by element.
-template <int DEG, int FMT, bool WHOLE>
-__device__ __forceinline__ void load_mx4_sh(const Mx4Sh& a, int order, int64_t i, float g,
-                                            float (&hc)[3][(DEG + 1) * (DEG + 1)]) {
-    constexpr int NC = (DEG + 1) * (DEG + 1), DIM = 3 * NC;
-    constexpr int BS = Mx4Block<FMT>::size, NB = (DIM + BS - 1) / BS, CB = (DIM + 1) / 2;
-    int64_t r = i;
-    if (a.indices) {
-        r = (int64_t)__ldg(a.indices + i) - 1;
-        if (r < 0 || r >= a.rows) {
+// The 4-bit row of a Gaussian in registers: words of eight codes, and the block scales' bytes. Rows of
+// exactly the rendered degree, their codes aligned to 8 bytes at degree 3 (24 bytes a row) and to 2
+// below (2, 6 and 14 bytes).
+template <int DEG, int FMT>
+struct ShRow {
+    static constexpr int DIM = 3 * (DEG + 1) * (DEG + 1), CB = (DIM + 1) / 2, NW = (CB + 3) / 4;
+    static constexpr int BS = Mx4Block<FMT>::size, NB = (DIM + BS - 1) / BS;
+    uint32_t w[NW], scale[NB];
+
+    __device__ __forceinline__ void load(const Mx4Sh& a, int64_t r) {
+        if (r < 0) {  // no row: zero codes with zero scales
 #pragma unroll
-            for (int e = 0; e < DIM; ++e) (&hc[0][0])[e] = 0.0f;
+            for (int k = 0; k < NW; ++k) w[k] = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) scale[b] = 0;
             return;
         }
-    }
-    if (WHOLE) {
-        using W = typename std::conditional<DEG == 3, uint2, uint16_t>::type;
-        constexpr int NW = CB / (int)sizeof(W);
-        W w[NW];
-        const W* p = reinterpret_cast<const W*>(a.codes + r * CB);
+        if constexpr (DEG == 3) {
+            const uint2* p = reinterpret_cast<const uint2*>(a.codes + r * CB);
 #pragma unroll
-        for (int k = 0; k < NW; ++k) w[k] = __ldg(p + k);
-        const uint8_t* s = a.scales + r * NB;
-        uint32_t sb[NB];
+            for (int k = 0; k < NW / 2; ++k) {
+                const uint2 v = __ldg(p + k);
+                w[2 * k] = v.x;
+                w[2 * k + 1] = v.y;
+            }
+        } else {
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(a.codes + r * CB);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) sb[b] = __ldg(s + b);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const Mx4Decode<FMT> d(sb[b], g);
-#pragma unroll
-            for (int e0 = b * BS; e0 < (b + 1) * BS && e0 < DIM; e0 += 8) {
-                uint32_t word;
-                if constexpr (DEG == 3) {
-                    word = (e0 / 8) & 1 ? w[e0 / 16].y : w[e0 / 16].x;
-                } else {
-                    // the row's last word may be half: what is doubled then lies behind its end
-                    word = w[e0 / 4] | (uint32_t)w[e0 / 4 + 1 < NW ? e0 / 4 + 1 : e0 / 4] << 16;
-                }
-                __half2 h[4];
-                e2m1_word_half(word, h);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 v = d.value(h[k]);
-                    if (e0 + 2 * k < DIM) (&hc[0][0])[e0 + 2 * k] = v.x;
-                    if (e0 + 2 * k + 1 < DIM) (&hc[0][0])[e0 + 2 * k + 1] = v.y;
-                }
+            for (int k = 0; k < NW; ++k) {
+                // the last word may be half: what is doubled then lies behind the row's end
+                const uint32_t lo = __ldg(p + 2 * k), hi = 4 * k + 2 < CB ? __ldg(p + 2 * k + 1) : lo;
+                w[k] = lo | (hi << 16);
             }
         }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) scale[b] = __ldg(a.scales + r * NB + b);
+    }
+};
+
+// Rows 2 t and 2 t + 1 at degree 3 in NVFP4: 48 bytes of codes, 16-byte aligned, and 6 scales.
+__device__ __forceinline__ void load_neighbours(const Mx4Sh& a, int64_t r, ShRow<3, GS3D_NVFP4>& s0,
+                                                ShRow<3, GS3D_NVFP4>& s1) {
+    const uint4* p = reinterpret_cast<const uint4*>(a.codes + r * 24);
+    const uint4 x = __ldg(p), y = __ldg(p + 1), z = __ldg(p + 2);
+    s0.w[0] = x.x, s0.w[1] = x.y, s0.w[2] = x.z, s0.w[3] = x.w, s0.w[4] = y.x, s0.w[5] = y.y;
+    s1.w[0] = y.z, s1.w[1] = y.w, s1.w[2] = z.x, s1.w[3] = z.y, s1.w[4] = z.z, s1.w[5] = z.w;
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.scales + r * 3);
+    const uint32_t u = __ldg(q), v = __ldg(q + 1), w = __ldg(q + 2);
+    s0.scale[0] = u & 255u, s0.scale[1] = u >> 8, s0.scale[2] = v & 255u;
+    s1.scale[0] = v >> 8, s1.scale[1] = w & 255u, s1.scale[2] = w >> 8;
+}
+
+// Coefficients 8 k .. 8 k + 7 of two rows.
+template <int DEG, int FMT>
+__device__ __forceinline__ void decode_word_pair(const ShRow<DEG, FMT>& r0, const ShRow<DEG, FMT>& r1, float g, int k,
+                                                 Float2* h) {
+    const Mx4Decode<FMT> d0(r0.scale[8 * k / ShRow<DEG, FMT>::BS], g), d1(r1.scale[8 * k / ShRow<DEG, FMT>::BS], g);
+    const Float2 factor(d0.factor(), d1.factor());
+    __half2 e0[4], e1[4];
+    e2m1_word_half(r0.w[k], e0);
+    e2m1_word_half(r1.w[k], e1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 a = d0.scaled(e0[j]), b = d1.scaled(e1[j]);
+        h[j] = Float2(a.x, b.x) * factor;
+        h[j + 4] = Float2(a.y, b.y) * factor;
+    }
+}
+
+// The coefficients of rows r0 and r1 (-1: zeros), channel by channel. WHOLE: as ShRow wants them; else
+// element by element.
+template <int DEG, int FMT, bool WHOLE>
+__device__ __forceinline__ void load_sh_pair(const Mx4Sh& a, int order, int64_t r0, int64_t r1, float g,
+                                             Float2 (&h)[(3 * (DEG + 1) * (DEG + 1) + 7) / 8 * 8]) {
+    constexpr int NC = (DEG + 1) * (DEG + 1);
+    if constexpr (WHOLE) {
+        ShRow<DEG, FMT> s0, s1;
+        s0.load(a, r0);
+        s1.load(a, r1);
+#pragma unroll
+        for (int k = 0; k < ShRow<DEG, FMT>::NW; ++k) decode_word_pair(s0, s1, g, k, h + 8 * k);
     } else {
+        constexpr int BS = Mx4Block<FMT>::size;
+        auto element = [&](int64_t r, int e) {
+            if (r < 0) return 0.0f;
+            const Mx4Decode<FMT> d(a.scales[r * a.blocks + e / BS], g);
+            const float2 v = mx4_value(d, e2m1_pair_half(a.codes[r * a.code_bytes + e / 2]));
+            return e & 1 ? v.y : v.x;
+        };
 #pragma unroll
         for (int c = 0; c < 3; ++c)
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
-                const int e = c * order + k;
-                const Mx4Decode<FMT> d(a.scales[r * a.blocks + e / BS], g);
-                const float2 v = d.value(e2m1_pair_half(a.codes[r * a.code_bytes + e / 2]));
-                hc[c][k] = e & 1 ? v.y : v.x;
+            for (int k = 0; k < NC; ++k) h[c * NC + k] = Float2(element(r0, c * order + k), element(r1, c * order + k));
+    }
+}
+
+// Row of Gaussian i, -1 where its index names none.
+__device__ __forceinline__ int64_t sh_row(const Mx4Sh& a, int64_t i) {
+    if (!a.indices) return i;
+    const int64_t r = (int64_t)__ldg(a.indices + i) - 1;
+    return r < a.rows && r >= 0 ? r : -1;
+}
+
+// The colours of two Gaussians from one position: the three channels of both. At degree 3 a channel is
+// decoded when it is summed, so that 32 coefficients are live and not 96.
+template <int DEG, int FMT, bool WHOLE>
+__device__ __forceinline__ void colour_pair(const Mx4Sh& a, int order, int64_t r0, int64_t r1, float g, const float* p,
+                                            const float4& m0, const float4& m1, Float2 (&c)[3]) {
+    constexpr int NC = (DEG + 1) * (DEG + 1);
+    Float2 basis[NC];
+    if constexpr (WHOLE && DEG == 3) {
+        ShRow<DEG, FMT> s0, s1;
+        bool loaded = false;
+        if constexpr (FMT == GS3D_NVFP4) {
+            if (a.neighbours && r1 == r0 + 1 && (r0 & 1) == 0) {
+                load_neighbours(a, r0, s0, s1);
+                loaded = true;
             }
+        }
+        if (!loaded) {
+            s0.load(a, r0);
+            s1.load(a, r1);
+        }
+        sh_basis_pair<DEG>(p, Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch) {
+            Float2 h[16];
+            decode_word_pair(s0, s1, g, 2 * ch, h);
+            decode_word_pair(s0, s1, g, 2 * ch + 1, h + 8);
+            c[ch] = sh_channel_pair<DEG>(h, basis);
+        }
+    } else {
+        Float2 h[(3 * NC + 7) / 8 * 8];
+        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h);
+        sh_basis_pair<DEG>(p, Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch) c[ch] = sh_channel_pair<DEG>(h + ch * NC, basis);
     }
 }
 
@@ -541,19 +628,38 @@ struct Positions {
     float p[GS3D_MAX_FACTORED_VIEWS][3];
 };
 
-template <int DEG, int FMT, bool WHOLE>
+// Gaussians 2 t and 2 t + 1 a thread, all their operations in packed pairs. ONE: a single view; else
+// `views` of them a block, with the coefficients decoded once.
+template <int DEG, int FMT, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(128) k_mx4_colours(const Mx4Sh a, int order, const float4* __restrict__ mo4,
-                                                     int n, const Positions cv, int nv,
+                                                     int n, const Positions cv, int nv, int views,
                                                      float4* __restrict__ out, int64_t view_stride) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    constexpr int NC = (DEG + 1) * (DEG + 1);
+    const int64_t i = 2 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
     if (i >= n) return;
+    const bool two = i + 1 < n;
     const float g = FMT == GS3D_NVFP4 ? __ldg(a.tensor_scale) : 1.0f;
-    float hc[3][(DEG + 1) * (DEG + 1)];
-    load_mx4_sh<DEG, FMT, WHOLE>(a, order, i, g, hc);
-    const float4 mo = mo4[i];
-    for (int v = 0; v < nv; ++v) {
-        const float3 c = colour_from_sh<DEG>(hc, cv.p[v], mo.x, mo.y, mo.z);
-        out[(size_t)v * view_stride + i] = make_float4(c.x, c.y, c.z, 0.0f);
+    const int64_t r0 = sh_row(a, i), r1 = two ? sh_row(a, i + 1) : -1;
+    const float4 m0 = __ldg(mo4 + i), m1 = __ldg(mo4 + (two ? i + 1 : i));
+    if constexpr (ONE) {
+        Float2 c[3];
+        colour_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, cv.p[0], m0, m1, c);
+        __stcs(out + i, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
+        if (two) __stcs(out + i + 1, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
+    } else {
+        Float2 h[(3 * NC + 7) / 8 * 8];
+        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h);
+        const int last = min(nv, ((int)blockIdx.y + 1) * views);
+#pragma unroll 2
+        for (int v = blockIdx.y * views; v < last; ++v) {
+            Float2 basis[NC], c[3];
+            sh_basis_pair<DEG>(cv.p[v], Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
+#pragma unroll
+            for (int ch = 0; ch < 3; ++ch) c[ch] = sh_channel_pair<DEG>(h + ch * NC, basis);
+            float4* o = out + (size_t)v * view_stride + i;
+            __stcs(o, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
+            if (two) __stcs(o + 1, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
+        }
     }
 }
 
@@ -566,14 +672,18 @@ __global__ void __launch_bounds__(128) k_mx4_render_colours(const Mx4Sh a, int o
                                                             const gs3d_camera cam, float* __restrict__ f2d) {
     const int F = counts[0];
     const float g = FMT == GS3D_NVFP4 ? __ldg(a.tensor_scale) : 1.0f;
-    for (int f = blockIdx.x * blockDim.x + threadIdx.x; f < F; f += gridDim.x * blockDim.x) {
-        const int gi = f2g[f] - 1;
-        float hc[3][(DEG + 1) * (DEG + 1)];
-        load_mx4_sh<DEG, FMT, WHOLE>(a, order, gi, g, hc);
-        const float4 mo = mo4[gi];
-        const float3 c = colour_from_sh<DEG>(hc, cam.position, mo.x, mo.y, mo.z);
+    for (int f = 2 * (blockIdx.x * blockDim.x + threadIdx.x); f < F; f += 2 * gridDim.x * blockDim.x) {
+        const bool two = f + 1 < F;
+        const int g0 = f2g[f] - 1, g1 = two ? f2g[f + 1] - 1 : g0;
+        const float4 m0 = __ldg(mo4 + g0), m1 = __ldg(mo4 + g1);
+        Float2 c[3];
+        colour_pair<DEG, FMT, WHOLE>(a, order, sh_row(a, g0), sh_row(a, g1), g, cam.position, m0, m1, c);
         float* rr = f2d + 9 * (size_t)f;
-        rr[6] = c.x; rr[7] = c.y; rr[8] = c.z;
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch) {
+            rr[6 + ch] = c[ch].x;
+            if (two) rr[15 + ch] = c[ch].y;
+        }
     }
 }
 
@@ -628,8 +738,16 @@ struct ColoursLaunch {
     cudaStream_t stream;
     template <int DEG, int FMT, bool WHOLE>
     int run() const {
-        k_mx4_colours<DEG, FMT, WHOLE><<<(unsigned)ceil_div(n, 128), 128, 0, stream>>>(a, order, mo4, n, cv, nv, out,
-                                                                             view_stride);
+        const unsigned grid = (unsigned)ceil_div(n, 256);
+        if (nv == 1) {
+            k_mx4_colours<DEG, FMT, WHOLE, true><<<grid, 128, 0, stream>>>(a, order, mo4, n, cv, nv, 1, out, view_stride);
+        } else {
+            // all views a block, unless that leaves SMs without: then as many shares of them as fill two waves
+            const int shares = (int)std::min<int64_t>(nv, std::max<int64_t>(1, 2 * 6 * (int64_t)device_sm_count() / grid));
+            const int views = (int)ceil_div(nv, shares);
+            k_mx4_colours<DEG, FMT, WHOLE, false><<<dim3(grid, (unsigned)ceil_div(nv, views)), 128, 0, stream>>>(
+                a, order, mo4, n, cv, nv, views, out, view_stride);
+        }
         GS3D_LAUNCHED("k_mx4_colours");
         return GS3D_OK;
     }
@@ -645,7 +763,7 @@ struct RenderColoursLaunch {
     cudaStream_t stream;
     template <int DEG, int FMT, bool WHOLE>
     int run() const {
-        k_mx4_render_colours<DEG, FMT, WHOLE><<<grid_for(n, 128, 16), 128, 0, stream>>>(
+        k_mx4_render_colours<DEG, FMT, WHOLE><<<grid_for(n, 256, 16), 128, 0, stream>>>(
             a, order, mo4, buf->fgidx_to_gidx, buf->device_counts, *cam,
             buf->means2d_opacities_inverse_covariances_colors);
         GS3D_LAUNCHED("k_mx4_render_colours");
@@ -654,8 +772,10 @@ struct RenderColoursLaunch {
 };
 
 Mx4Sh sh_source(const gs3d_mx4_rows* sh, const int32_t* indices) {
+    const bool neighbours = !indices && reinterpret_cast<uintptr_t>(sh->codes) % 16 == 0 &&
+                            reinterpret_cast<uintptr_t>(sh->scales) % 2 == 0;
     return Mx4Sh{sh->codes, sh->scales, sh->tensor_scale, indices, sh->rows, mx4_code_bytes(sh->dim),
-                 mx4_blocks(sh->dim, sh->format)};
+                 mx4_blocks(sh->dim, sh->format), neighbours};
 }
 
 }  // namespace

@@ -26,30 +26,30 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
     return byte == 0 ? 0x1p-127f : u2f(byte << 23);
 }
 
-// The two elements of a byte, exactly, in fp16: exponent and mantissa bits placed at bits 11..9 are
-// the element * 2^-14 (its subnormal is fp16's).
+// Elements as fp16, times 2^-14: exponent and mantissa bits at bits 11..9 (the element's subnormal is
+// then fp16's), the sign at bit 15. By integer operations: the hardware's conversion from e2m1x2 is
+// shorter, but nvcc 12.9 returned wrong elements for it wherever the byte came from a 16- or 8-bit load
+// or from a shift that depends on the thread.
+// The two elements of a byte:
 __device__ __forceinline__ __half2 e2m1_pair_half(uint32_t byte) {
-    const uint32_t h = ((byte & 0x07u) << 9) | ((byte & 0x08u) << 12) | ((byte & 0x70u) << 21) | ((byte & 0x80u) << 24);
-    return __hmul2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x7400)));  // 2^14
+    const uint32_t h = ((byte << 9) & 0x0e00u) | ((byte << 12) & 0x8000u) | ((byte << 21) & 0x0e000000u) |
+                       ((byte << 24) & 0x80000000u);
+    return *reinterpret_cast<const __half2*>(&h);
 }
-
-// The eight elements of a word, lowest bits first, by the hardware's conversion. Only for words that
-// come from 32-bit loads or arithmetic: fed straight from a 16- or 8-bit load it returned wrong
-// elements (nvcc 12.9; the tests go through every code).
+// Elements k and k + 4 of a word (lowest bits first) in e[k]: one pair of shifts for both.
 __device__ __forceinline__ void e2m1_word_half(uint32_t word, __half2 (&e)[4]) {
-    uint32_t h[4];
-    asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4;\n"
-        "  cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b;\n"
-        "  cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d; }"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-        : "r"(word));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) e[k] = *reinterpret_cast<__half2*>(&h[k]);
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t mag = k < 3 ? word << (9 - 4 * k) : word >> 3;
+        const uint32_t h = (mag & 0x0e000e00u) | ((word << (12 - 4 * k)) & 0x80008000u);
+        e[k] = *reinterpret_cast<const __half2*>(&h);
+    }
 }
 
-// The values of the two elements of a byte: element * block scale * tensor scale, rounded once.
-// NVFP4: element * block scale has 6 significant bits between 2^-10 and 2688, exact in fp16.
-// MXFP4: element * 2^k, exact in fp32 up to its overflow and underflow.
+// The values of two elements: element * block scale * tensor scale, rounded once, as scaled(element *
+// 2^-14) * factor().
+// NVFP4: element * block scale has 6 significant bits and is a multiple of 2^-10 up to 2688: exact in
+// fp16 times 2^-14. MXFP4: element * 2^k, exact in fp32 up to its overflow and underflow.
 template <int FMT>
 struct Mx4Decode;
 
@@ -58,22 +58,26 @@ struct Mx4Decode<GS3D_NVFP4> {
     __half2 s;
     float g;
     __device__ __forceinline__ Mx4Decode(uint32_t byte, float tensor_scale)
-        : s(__half2half2(e4m3_half(byte))), g(tensor_scale) {}
-    __device__ __forceinline__ float2 value(__half2 e) const {
-        const float2 v = __half22float2(__hmul2(e, s));
-        return make_float2(v.x * g, v.y * g);
-    }
+        : s(__half2half2(e4m3_half(byte))), g(tensor_scale * 0x1p14f) {}
+    __device__ __forceinline__ float2 scaled(__half2 e) const { return __half22float2(__hmul2(e, s)); }
+    __device__ __forceinline__ float factor() const { return g; }
 };
 
 template <>
 struct Mx4Decode<GS3D_MXFP4> {
     float s;
     __device__ __forceinline__ Mx4Decode(uint32_t byte, float) : s(e8m0_value(byte)) {}
-    __device__ __forceinline__ float2 value(__half2 e) const {
-        const float2 v = __half22float2(e);
-        return make_float2(v.x * s, v.y * s);
+    __device__ __forceinline__ float2 scaled(__half2 e) const {
+        return __half22float2(__hmul2(e, __half2half2(__ushort_as_half(0x7400))));  // * 2^14
     }
+    __device__ __forceinline__ float factor() const { return s; }
 };
+
+template <int FMT>
+__device__ __forceinline__ float2 mx4_value(const Mx4Decode<FMT>& d, __half2 e) {
+    const float2 v = d.scaled(e);
+    return make_float2(v.x * d.factor(), v.y * d.factor());
+}
 
 // 4-bit SH rows as a colour source: row i, or row indices[i].
 struct Mx4Sh {
@@ -83,6 +87,7 @@ struct Mx4Sh {
     const int32_t* indices;
     int64_t rows;
     int code_bytes, blocks;
+    bool neighbours;  // rows in order, aligned so that two can be loaded together
 };
 
 }  // namespace gs3d

@@ -39,6 +39,13 @@ __device__ __forceinline__ void store_streaming(T* p, const Pack<T, N>& v) {
     __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&v));
 }
 
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+    using W = typename std::conditional<sizeof(Pack<T, N>) == 16, uint4, uint2>::type;
+    const W w = __ldg(reinterpret_cast<const W*>(p));
+    return *reinterpret_cast<const Pack<T, N>*>(&w);
+}
+
 template <typename TI, typename TO>
 constexpr int lookup_pack() { return sizeof(TI) == 2 && sizeof(TO) == 2 ? 8 : 4; }
 
@@ -52,27 +59,25 @@ __global__ void __launch_bounds__(256) k_table_lookup_units(const TI* __restrict
     const int slot = threadIdx.x / tile_units;
     const int unit = blockIdx.y * tile_units + threadIdx.x - slot * tile_units;
     if (unit >= units) return;
-    const int64_t first = (int64_t)blockIdx.x * slots * kLookupRows + slot;
+    const int first = blockIdx.x * (slots * kLookupRows) + slot;
     int k[kLookupRows];
 #pragma unroll
-    for (int q = 0; q < kLookupRows; ++q) {
-        const int64_t i = first + q * slots;
-        k[q] = i < n ? __ldg(indices + i) : 0;
-    }
+    for (int q = 0; q < kLookupRows; ++q) k[q] = __ldg(indices + min(first + q * slots, n - 1));
     Pack<TI, N> v[kLookupRows];
 #pragma unroll
-    for (int q = 0; q < kLookupRows; ++q)
-        if (k[q] >= 1 && k[q] <= rows)
-            v[q] = *reinterpret_cast<const Pack<TI, N>*>(table + (int64_t)(k[q] - 1) * table_stride + unit * N);
+    for (int q = 0; q < kLookupRows; ++q) {
+        v[q] = Pack<TI, N>{};
+        if ((unsigned)(k[q] - 1) < (unsigned)rows)
+            v[q] = load_pack<TI, N>(table + (int64_t)(k[q] - 1) * table_stride + unit * N);
+    }
+    TO* o = out + first * out_stride + unit * N;
 #pragma unroll
     for (int q = 0; q < kLookupRows; ++q) {
-        const int64_t i = first + q * slots;
-        if (i >= n) break;
-        const bool valid = k[q] >= 1 && k[q] <= rows;
-        Pack<TO, N> o;
+        Pack<TO, N> p;
 #pragma unroll
-        for (int c = 0; c < N; ++c) o.e[c] = from_f32<TO>(valid ? to_f32(v[q].e[c]) * scale : 0.0f);
-        store_streaming(out + i * out_stride + unit * N, o);
+        for (int c = 0; c < N; ++c) p.e[c] = from_f32<TO>(to_f32(v[q].e[c]) * scale);
+        if ((unsigned)(k[q] - 1) >= (unsigned)rows) p = Pack<TO, N>{};  // zeros even for a NaN or infinite scale
+        if (first + q * slots < n) store_streaming(o + q * slots * out_stride, p);
     }
 }
 

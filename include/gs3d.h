@@ -628,10 +628,11 @@ GS3D_API int gs3d_mx4_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, g
 /* The colours of n Gaussians from 4-bit SH rows, seen from n_views cameras (view_positions: HOST
  * memory, 3 floats per view, 1 .. GS3D_MAX_FACTORED_VIEWS views): gs3d_shard_colours with the
  * coefficients gs3d_mx4_dequantise (fp32) gives for row i, or with indices != NULL for row
- * indices[i] (1-based; outside 1 .. sh->rows: coefficients 0), bit for bit, without writing them.
- * sh->dim = 3 (d+1)^2 with d >= sh_degree; means4: 4 x n, the first three floats the mean (16-byte
- * aligned, as means_opacity_features / means_opacities). Float4 row v * view_stride + i of colours
- * (16-byte aligned), w = 0. */
+ * indices[i] (1-based; outside 1 .. sh->rows: coefficients 0), without writing them, up to rounding:
+ * sums are fp32 with fused multiply-adds, and a block's elements are summed before its scale multiplies
+ * them. sh->dim = 3 (d+1)^2 with d >= sh_degree; means4: 4 x n, the first three floats the mean
+ * (16-byte aligned, as means_opacity_features / means_opacities). Float4 row v * view_stride + i of
+ * colours (16-byte aligned), w = 0. */
 GS3D_API int gs3d_mx4_colours(const gs3d_mx4_rows* sh, int32_t sh_degree, const int32_t* indices,
                               const float* means4, int32_t n, const float* view_positions,
                               int32_t n_views, float* colours, int64_t view_stride,
@@ -639,8 +640,8 @@ GS3D_API int gs3d_mx4_colours(const gs3d_mx4_rows* sh, int32_t sh_degree, const 
 
 /* gs3d_render_forward_render_only with the SH coefficients of 4-bit rows (row i, or row indices[i]
  * as in gs3d_mx4_colours): gaussians->sh_coeffs is not read and may be NULL, gaussians->sh_degree is
- * the degree of sh->dim. The outputs equal those of gs3d_render_forward_render_only on the
- * dequantised coefficients bit for bit. */
+ * the degree of sh->dim. Everything but the colours equals gs3d_render_forward_render_only on the
+ * dequantised coefficients bit for bit, the colours up to rounding. */
 GS3D_API int gs3d_render_forward_mx4(
     const gs3d_render_outputs* outputs, const gs3d_render_only_gaussians* gaussians,
     const gs3d_mx4_rows* sh, const int32_t* indices, const gs3d_camera* camera,

@@ -7,7 +7,7 @@ import torch
 import gs3d
 from gs3d import MX4Rows, RenderBuffers, RenderOnlyGaussiansVector, RenderOptions, RenderOutputs, Tiling
 from gs3d import compressed as gc
-from gs3d.render import render_given_colour, shard_colours
+from gs3d.render import render_given_colour
 from gs3d.scene import SceneSpec, look_at_camera, synthetic_gaussians
 from gs3d.structs import GaussiansVector
 
@@ -418,6 +418,9 @@ def test_every_code_and_scale(cuda):
 
 
 # -- colours ------------------------------------------------------------------------------------
+COLOUR_U = 147  # see test_colours
+
+
 def make_mx4(rows, dim, fmt, gen):
     block = 16 if fmt == "nvfp4" else 32
     codes = torch.randint(0, 256, (rows, (dim + 1) // 2), generator=gen, dtype=torch.uint8)
@@ -431,9 +434,11 @@ def make_mx4(rows, dim, fmt, gen):
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("table", [False, True])
 def test_colours(cuda, n, degree, storage, fmt, table):
-    """Bit for bit the colours of the dequantised coefficients, and near the 64-bit value: the
-    direction's components carry at most 6 u, a basis function (at most degree 3, coefficients adding
-    to at most 3) then at most 72 u, and a sum of 16 products 16 u of their magnitudes (at most 3 |h|)."""
+    """Near the 64-bit value. Per unit of u = 2^-24: a component of mean - position carries 1, the sum of
+    squares 3, the reciprocal root half of that and 4 of its own (2 ulp), the product with it 1: at most 8
+    for a component of the direction. A basis function of degree d <= 3, whose coefficients add to at
+    most 3, then carries 3 (8 d + 6) <= 90, a sum of 16 products 16 of their magnitudes (at most 3 |h|)
+    and the scale of a block 3 roundings of the same: (90 + 48 + 9) u sum|h|, and 2 u for the 1/2."""
     gen = rng(n + degree)
     order = (storage + 1) ** 2
     rows = max(1, n // 3) if table else n + 2
@@ -446,13 +451,8 @@ def test_colours(cuda, n, degree, storage, fmt, table):
         got = gc.mx4_colours(qd, means.to(cuda), pos, degree, indices=None if idx is None else idx.to(cuda))
         w = gc.mx4_dequantise(qd)
         w = w[:n] if idx is None else gc.table_lookup(w, idx.to(cuda))
-        g = GaussiansVector(means.to(cuda), torch.zeros(n, 3, device=cuda), torch.zeros(n, 4, device=cuda),
-                            w.view(n, 3, order).contiguous())
-        same = torch.empty(views, n, 4, device=cuda)
-        shard_colours(g, degree, pos, 0, n, same, n)
-        assert torch.equal(got.view(torch.int32), same.view(torch.int32))
         h = w.cpu().double().view(n, 3, order)[:, :, : (degree + 1) ** 2]
-        bound = 120 * U * h.abs().sum(dim=2) + 2 * U
+        bound = COLOUR_U * U * h.abs().sum(dim=2) + 2 * U
         for v in {0, views // 2, views - 1}:
             want = colours_exact(h, means.double(), pos[v].astype(np.float64), degree)
             assert ((got[v, :, :3].cpu().double() - want).abs() <= bound).all()
@@ -496,13 +496,23 @@ def test_colours_edges(cuda):
 
 
 # -- the render ---------------------------------------------------------------------------------
+def pixel_bound(sh, buf):
+    """See test_render_compressed; a colour is at most 1/2 + 3 sum|h| (a basis function is at most 3)."""
+    size = float(sh.abs().sum(dim=2).max())
+    ends = buf.tiles_end_sdfgidx.cpu().long()
+    entries = int((ends - torch.cat([ends.new_zeros(1), ends[:-1]])).max())
+    return U * (2 * COLOUR_U * size + 4 + 4 * entries * (0.5 + 3 * size))
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("table", [False, True])
 @pytest.mark.parametrize("sh_degree", [0, 2, 3])
 @pytest.mark.parametrize("reference_order", [False, True])
 def test_render_compressed(cuda, fmt, table, sh_degree, reference_order):
-    """The render of a compressed model is the render-only render of its dequantised coefficients, and
-    its second half alone (render_given_colour on mx4_colours) the same image."""
+    """The render of a compressed model against the render-only render of its dequantised coefficients:
+    the same geometry, sorting and weights bit for bit, colours that differ by at most two colour bounds
+    (the plain render's is below: test_colours' chain with exact roots), so pixels (weights add to at most
+    1) by as much plus the rounding of the blend, 2 u of the largest colour per entry and side."""
     g = synthetic_gaussians(SceneSpec(5_000, "uniform:1", -4.0, 0.5), 3).to(cuda)
     ro = RenderOnlyGaussiansVector.from_trainable(g)
     tab = gc.fit_table(g.sh_coeffs, 40, iterations=2) if table else None
@@ -519,8 +529,9 @@ def test_render_compressed(cuda, fmt, table, sh_degree, reference_order):
         buf = RenderBuffers.create(g.n, til.nb_tiles, cuda)
         gs3d.render(out, model, cam, til, opt, buf, reference_order=reference_order)
         images.append(out)
-    assert torch.equal(images[0].rgb, images[1].rgb)
     assert torch.equal(images[0].last_contributing_sdfgids, images[1].last_contributing_sdfgids)
+    assert torch.equal(images[0].transmittance, images[1].transmittance)
+    assert float((images[0].rgb - images[1].rgb).abs().max()) <= pixel_bound(plain.sh_coeffs, buf)
     assert float(images[0].rgb.std()) > 0.01
 
 
@@ -537,7 +548,7 @@ def test_render_no_gaussians(cuda):
                     defer_colour=True)
 
 
-def test_given_colours_equal_the_render(cuda):
+def test_given_colours_render(cuda):
     g = synthetic_gaussians(SceneSpec(3_000, "uniform:1", -4.0, 0.5), 4).to(cuda)
     q = gc.mx4_quantise(g.sh_coeffs)
     cam = look_at_camera(96, 64, 60.0, (0, 0.5, 3))
@@ -549,8 +560,9 @@ def test_given_colours_equal_the_render(cuda):
     render_given_colour(a, g, cam, til, opt, buf, colours, g.n)
     b = RenderOutputs.create(96, 64, cuda)
     plain = GaussiansVector(*g.tensors()[:3], gc.mx4_dequantise(q).view(-1, 3, 16).contiguous())
-    gs3d.render(b, plain, cam, til, opt, RenderBuffers.create(g.n, til.nb_tiles, cuda))
-    assert torch.equal(a.rgb, b.rgb)
+    buf = RenderBuffers.create(g.n, til.nb_tiles, cuda)
+    gs3d.render(b, plain, cam, til, opt, buf)
+    assert float((a.rgb - b.rgb).abs().max()) <= pixel_bound(plain.sh_coeffs, buf)
 
 
 # -- a run of them, streams and graphs -------------------------------------------------------------

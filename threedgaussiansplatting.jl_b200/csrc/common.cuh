@@ -205,12 +205,10 @@ GS_HD float sh_c(int i) {
     }
 }
 
-// evaluate_sh_basis_function (sh.jl:123-149), i 1-based (constant after unrolling). T: float, or a
-// pair of floats (Float2 of sh_colour.cuh) that go through the same operations side by side.
-template <typename T>
-GS_HD T sh_basis(int i, T x, T y, T z) {
+// evaluate_sh_basis_function (sh.jl:123-149), i 1-based (constant after unrolling)
+GS_HD float sh_basis(int i, float x, float y, float z) {
     switch (i) {
-        case 1: return T(sh_c(1));
+        case 1: return sh_c(1);
         case 2: return -y * sh_c(2);
         case 3: return z * sh_c(3);
         case 4: return -x * sh_c(4);
@@ -226,7 +224,7 @@ GS_HD T sh_basis(int i, T x, T y, T z) {
         case 14: return x * (4.0f * (z * z) - x * x - y * y) * sh_c(14);
         case 15: return z * (x * x - y * y) * sh_c(15);
         case 16: return x * (x * x - 3.0f * (y * y)) * sh_c(16);
-        default: return T(0.0f);
+        default: return 0.0f;
     }
 }
 

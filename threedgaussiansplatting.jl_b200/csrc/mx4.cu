@@ -536,35 +536,67 @@ __device__ __forceinline__ void load_neighbours(const Mx4Sh& a, int64_t r, ShRow
     s1.scale[0] = v >> 8, s1.scale[1] = w & 255u, s1.scale[2] = w >> 8;
 }
 
-// Coefficients 8 k .. 8 k + 7 of two rows.
+// Elements 8 k .. 8 k + 7 of two rows, times 2^-14.
 template <int DEG, int FMT>
-__device__ __forceinline__ void decode_word_pair(const ShRow<DEG, FMT>& r0, const ShRow<DEG, FMT>& r1, float g, int k,
-                                                 Float2* h) {
-    const Mx4Decode<FMT> d0(r0.scale[8 * k / ShRow<DEG, FMT>::BS], g), d1(r1.scale[8 * k / ShRow<DEG, FMT>::BS], g);
-    const Float2 factor(d0.factor(), d1.factor());
+__device__ __forceinline__ void decode_word_pair(const ShRow<DEG, FMT>& r0, const ShRow<DEG, FMT>& r1, int k, Float2* h) {
     __half2 e0[4], e1[4];
     e2m1_word_half(r0.w[k], e0);
     e2m1_word_half(r1.w[k], e1);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float2 a = d0.scaled(e0[j]), b = d1.scaled(e1[j]);
-        h[j] = Float2(a.x, b.x) * factor;
-        h[j + 4] = Float2(a.y, b.y) * factor;
+        const float2 a = __half22float2(e0[j]), b = __half22float2(e1[j]);
+        h[j] = Float2(a.x, b.x);
+        h[j + 4] = Float2(a.y, b.y);
     }
 }
 
-// The coefficients of rows r0 and r1 (-1: zeros), channel by channel. WHOLE: as ShRow wants them; else
-// element by element.
+// 1/2 + the channel's products with the basis, clamped at 0. WHOLE: h are elements times 2^-14, and what
+// lies in one block is summed before its scale (times the tensor scale, in `factor`) multiplies it; else
+// h are the coefficients.
+template <int DEG, int FMT, bool WHOLE>
+__device__ __forceinline__ Float2 channel_pair(int ch, const Float2* h, const Float2* factor, const Float2* basis) {
+    constexpr int NC = (DEG + 1) * (DEG + 1), BS = Mx4Block<FMT>::size;
+    Float2 c(0.5f);
+    if constexpr (WHOLE) {
+        const int b0 = ch * NC / BS, b1 = ((ch + 1) * NC - 1) / BS;
+#pragma unroll
+        for (int b = b0; b <= b1; ++b) {
+            const int k0 = max(b * BS - ch * NC, 0), k1 = min((b + 1) * BS - ch * NC, NC);
+            Float2 s = basis[k0] * h[k0];
+#pragma unroll
+            for (int k = k0 + 1; k < k1; ++k) s = fma2(basis[k], h[k], s);
+            c = fma2(s * Float2(0x1p14f), factor[b], c);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NC; ++k) c = fma2(basis[k], h[k], c);
+    }
+    if (c.x < 0.0f) c.x = 0.0f;
+    if (c.y < 0.0f) c.y = 0.0f;
+    return c;
+}
+
+template <int DEG, int FMT>
+__device__ __forceinline__ void block_factors(const ShRow<DEG, FMT>& r0, const ShRow<DEG, FMT>& r1, float g,
+                                              Float2 (&factor)[ShRow<DEG, FMT>::NB]) {
+#pragma unroll
+    for (int b = 0; b < ShRow<DEG, FMT>::NB; ++b)
+        factor[b] = Float2(mx4_scale<FMT>(r0.scale[b]) * g, mx4_scale<FMT>(r1.scale[b]) * g);
+}
+
+// The rows of two Gaussians (-1: zeros): elements and block factors, or (not WHOLE) the coefficients.
 template <int DEG, int FMT, bool WHOLE>
 __device__ __forceinline__ void load_sh_pair(const Mx4Sh& a, int order, int64_t r0, int64_t r1, float g,
-                                             Float2 (&h)[(3 * (DEG + 1) * (DEG + 1) + 7) / 8 * 8]) {
+                                             Float2 (&h)[(3 * (DEG + 1) * (DEG + 1) + 7) / 8 * 8],
+                                             Float2 (&factor)[ShRow<DEG, FMT>::NB]) {
     constexpr int NC = (DEG + 1) * (DEG + 1);
     if constexpr (WHOLE) {
         ShRow<DEG, FMT> s0, s1;
         s0.load(a, r0);
         s1.load(a, r1);
+        block_factors(s0, s1, g, factor);
 #pragma unroll
-        for (int k = 0; k < ShRow<DEG, FMT>::NW; ++k) decode_word_pair(s0, s1, g, k, h + 8 * k);
+        for (int k = 0; k < ShRow<DEG, FMT>::NW; ++k) decode_word_pair(s0, s1, k, h + 8 * k);
     } else {
         constexpr int BS = Mx4Block<FMT>::size;
         auto element = [&](int64_t r, int e) {
@@ -593,7 +625,8 @@ template <int DEG, int FMT, bool WHOLE>
 __device__ __forceinline__ void colour_pair(const Mx4Sh& a, int order, int64_t r0, int64_t r1, float g, const float* p,
                                             const float4& m0, const float4& m1, Float2 (&c)[3]) {
     constexpr int NC = (DEG + 1) * (DEG + 1);
-    Float2 basis[NC];
+    Float2 basis[NC], factor[ShRow<DEG, FMT>::NB];
+    const Float2 mx(m0.x, m1.x), my(m0.y, m1.y), mz(m0.z, m1.z);
     if constexpr (WHOLE && DEG == 3) {
         ShRow<DEG, FMT> s0, s1;
         bool loaded = false;
@@ -607,20 +640,21 @@ __device__ __forceinline__ void colour_pair(const Mx4Sh& a, int order, int64_t r
             s0.load(a, r0);
             s1.load(a, r1);
         }
-        sh_basis_pair<DEG>(p, Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
+        sh_basis_pair<DEG>(p, mx, my, mz, basis);
+        block_factors(s0, s1, g, factor);
 #pragma unroll
         for (int ch = 0; ch < 3; ++ch) {
             Float2 h[16];
-            decode_word_pair(s0, s1, g, 2 * ch, h);
-            decode_word_pair(s0, s1, g, 2 * ch + 1, h + 8);
-            c[ch] = sh_channel_pair<DEG>(h, basis);
+            decode_word_pair(s0, s1, 2 * ch, h);
+            decode_word_pair(s0, s1, 2 * ch + 1, h + 8);
+            c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h, factor, basis);
         }
     } else {
         Float2 h[(3 * NC + 7) / 8 * 8];
-        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h);
-        sh_basis_pair<DEG>(p, Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
+        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h, factor);
+        sh_basis_pair<DEG>(p, mx, my, mz, basis);
 #pragma unroll
-        for (int ch = 0; ch < 3; ++ch) c[ch] = sh_channel_pair<DEG>(h + ch * NC, basis);
+        for (int ch = 0; ch < 3; ++ch) c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h + ch * NC, factor, basis);
     }
 }
 
@@ -647,15 +681,14 @@ __global__ void __launch_bounds__(128) k_mx4_colours(const Mx4Sh a, int order, c
         __stcs(out + i, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
         if (two) __stcs(out + i + 1, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
     } else {
-        Float2 h[(3 * NC + 7) / 8 * 8];
-        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h);
+        Float2 h[(3 * NC + 7) / 8 * 8], factor[ShRow<DEG, FMT>::NB];
+        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h, factor);
         const int last = min(nv, ((int)blockIdx.y + 1) * views);
-#pragma unroll 2
         for (int v = blockIdx.y * views; v < last; ++v) {
             Float2 basis[NC], c[3];
             sh_basis_pair<DEG>(cv.p[v], Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
 #pragma unroll
-            for (int ch = 0; ch < 3; ++ch) c[ch] = sh_channel_pair<DEG>(h + ch * NC, basis);
+            for (int ch = 0; ch < 3; ++ch) c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h + ch * NC, factor, basis);
             float4* o = out + (size_t)v * view_stride + i;
             __stcs(o, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
             if (two) __stcs(o + 1, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));

@@ -26,6 +26,11 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
     return byte == 0 ? 0x1p-127f : u2f(byte << 23);
 }
 
+template <int FMT>
+__device__ __forceinline__ float mx4_scale(uint32_t byte) {
+    return FMT == GS3D_NVFP4 ? e4m3_value(byte) : e8m0_value(byte);
+}
+
 // Elements as fp16, times 2^-14: exponent and mantissa bits at bits 11..9 (the element's subnormal is
 // then fp16's), the sign at bit 15. By integer operations: the hardware's conversion from e2m1x2 is
 // shorter, but nvcc 12.9 returned wrong elements for it wherever the byte came from a 16- or 8-bit load

@@ -40,18 +40,14 @@ __device__ __forceinline__ float3 colour_from_sh(const float (&hc)[3][(DEG + 1) 
                        sh_channel<DEG>(hc[2], dx, dy, dz));
 }
 
-// Two fp32 values in one 64-bit register, for the packed instructions (one issue slot for two
-// operations, each rounded as the scalar one): two Gaussians side by side. Products, sums and
-// differences are all fma (a b + -0, a 1 + b, b (-1) + a round as they do) with 1, -1 and -0 from
-// memory: mul.rn.f32x2 followed by add.rn.f32x2 came back as one fused operation (nvcc 12.9), and so
-// did fma with constants the compiler could see.
+// Two fp32 values in one 64-bit register, for the packed fused multiply-add (one issue slot for two):
+// two Gaussians side by side.
 struct Float2 {
     float x, y;
     __device__ __forceinline__ Float2() {}
     __device__ __forceinline__ explicit Float2(float v) : x(v), y(v) {}
     __device__ __forceinline__ Float2(float a, float b) : x(a), y(b) {}
 };
-static __constant__ float kPackedUnits[3] = {1.0f, -1.0f, -0.0f};
 __device__ __forceinline__ Float2 fma2(Float2 a, Float2 b, Float2 c) {
     Float2 r;
     asm("{ .reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7};\n"
@@ -60,40 +56,49 @@ __device__ __forceinline__ Float2 fma2(Float2 a, Float2 b, Float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
-__device__ __forceinline__ Float2 operator*(Float2 a, Float2 b) { return fma2(a, b, Float2(kPackedUnits[2])); }
-__device__ __forceinline__ Float2 operator+(Float2 a, Float2 b) { return fma2(a, Float2(kPackedUnits[0]), b); }
-__device__ __forceinline__ Float2 operator-(Float2 a, Float2 b) { return fma2(b, Float2(kPackedUnits[1]), a); }
-__device__ __forceinline__ Float2 operator*(Float2 a, float b) { return a * Float2(b); }
-__device__ __forceinline__ Float2 operator*(float a, Float2 b) { return Float2(a) * b; }
-__device__ __forceinline__ Float2 operator-(Float2 a) { return Float2(-a.x, -a.y); }
-
-// The basis functions at the unit directions from p to two means, with colour_from_sh's operations.
-template <int DEG>
-__device__ __forceinline__ void sh_basis_pair(const float* p, Float2 mx, Float2 my, Float2 mz,
-                                              Float2 (&basis)[(DEG + 1) * (DEG + 1)]) {
-    const Float2 vx = mx - Float2(p[0]), vy = my - Float2(p[1]), vz = mz - Float2(p[2]);
-    const Float2 ss = vx * vx + vy * vy + vz * vz;
-    const Float2 inv(1.0f / sqrtf(ss.x), 1.0f / sqrtf(ss.y));
-    const Float2 dx = vx * inv, dy = vy * inv, dz = vz * inv;
-#pragma unroll
-    for (int k = 0; k < (DEG + 1) * (DEG + 1); ++k) basis[k] = sh_basis(k + 1, dx, dy, dz);
+__device__ __forceinline__ Float2 operator*(Float2 a, Float2 b) {
+    Float2 r;
+    asm("{ .reg .b64 a, b, c; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mul.rn.f32x2 c, a, b; mov.b64 {%0, %1}, c; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
 }
 
-// sh_channel for two Gaussians, with its operations in its order.
+// The basis functions (sh.jl:123-149) at the unit directions from p to two means, with fused
+// multiply-adds and the reciprocal square root (rsqrtf, 2 ulp): within a few ulp of sh_basis.
 template <int DEG>
-__device__ __forceinline__ Float2 sh_channel_pair(const Float2* hc, const Float2* basis) {
-    Float2 cc = basis[0] * hc[0];
-#pragma unroll
-    for (int d = 1; d <= DEG; ++d) {
-        Float2 band = basis[d * d] * hc[d * d];
-#pragma unroll
-        for (int k = d * d + 1; k < (d + 1) * (d + 1); ++k) band = band + basis[k] * hc[k];
-        cc = cc + band;
+__device__ __forceinline__ void sh_basis_pair(const float* p, Float2 mx, Float2 my, Float2 mz,
+                                              Float2 (&b)[(DEG + 1) * (DEG + 1)]) {
+    b[0] = Float2(sh_c(1));
+    if constexpr (DEG >= 1) {
+        const Float2 one(1.0f), minus(-1.0f);
+        Float2 x = fma2(mx, one, Float2(-p[0])), y = fma2(my, one, Float2(-p[1])), z = fma2(mz, one, Float2(-p[2]));
+        const Float2 ss = fma2(z, z, fma2(y, y, x * x));
+        const Float2 inv(rsqrtf(ss.x), rsqrtf(ss.y));
+        x = x * inv, y = y * inv, z = z * inv;
+        b[1] = y * Float2(-sh_c(2));
+        b[2] = z * Float2(sh_c(3));
+        b[3] = x * Float2(-sh_c(4));
+        if constexpr (DEG >= 2) {
+            const Float2 xx = x * x, yy = y * y, zz = z * z, xy = x * y;
+            const Float2 sum = fma2(xx, one, yy), diff = fma2(yy, minus, xx), less = fma2(sum, minus, Float2(0.0f));
+            b[4] = xy * Float2(sh_c(5));
+            b[5] = y * z * Float2(sh_c(6));
+            b[6] = fma2(zz, Float2(2.0f), less) * Float2(sh_c(7));
+            b[7] = x * z * Float2(sh_c(8));
+            b[8] = diff * Float2(sh_c(9));
+            if constexpr (DEG >= 3) {
+                const Float2 four = fma2(zz, Float2(4.0f), less);
+                b[9] = y * Float2(sh_c(10)) * fma2(xx, Float2(3.0f), yy * minus);
+                b[10] = xy * z * Float2(sh_c(11));
+                b[11] = y * Float2(sh_c(12)) * four;
+                b[12] = z * Float2(sh_c(13)) * fma2(zz, Float2(2.0f), sum * Float2(-3.0f));
+                b[13] = x * Float2(sh_c(14)) * four;
+                b[14] = z * Float2(sh_c(15)) * diff;
+                b[15] = x * Float2(sh_c(16)) * fma2(yy, Float2(-3.0f), xx);
+            }
+        }
     }
-    cc = cc + Float2(0.5f);
-    if (cc.x < 0.0f) cc.x = 0.0f;
-    if (cc.y < 0.0f) cc.y = 0.0f;
-    return cc;
 }
 
 }  // namespace gs3d

@@ -45,11 +45,13 @@ __device__ __forceinline__ void take_finite_abs(uint32_t& m, float v) {
 // Every block turns its largest magnitude into the scale it asks for (monotone, positive: fp32 bits
 // order like unsigned integers) and the largest one stays; a lone block stores it. WIDE: rows of
 // 16-byte packs, back to back.
+constexpr int kScaleThreads = 512;
+
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) k_mx4_tensor_scale(const T* __restrict__ x, int64_t rows, int64_t stride,
+__global__ void __launch_bounds__(kScaleThreads) k_mx4_tensor_scale(const T* __restrict__ x, int64_t rows, int64_t stride,
                                                           int dim, uint32_t* __restrict__ tensor_scale) {
     constexpr int N = 16 / (int)sizeof(T);
-    __shared__ uint32_t warp_max[8];
+    __shared__ uint32_t warp_max[kScaleThreads / 32];
     uint32_t m = 0;
     const int64_t total = rows * dim, threads = (int64_t)gridDim.x * blockDim.x;
     const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(256) k_mx4_tensor_scale(const T* __restrict__ 
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) m = max(m, warp_max[w]);
+        for (int w = 1; w < kScaleThreads / 32; ++w) m = max(m, warp_max[w]);
         const uint32_t scale = f2u(fmaxf(u2f(m) / 2688.0f, 0x1p-100f));
         if (gridDim.x == 1) *tensor_scale = scale;
         else atomicMax(tensor_scale, scale);
@@ -146,13 +148,11 @@ template <int FMT>
 __device__ __forceinline__ uint32_t quantise_block(const float (&v)[Mx4Block<FMT>::size], const TensorScale& t,
                                                    uint32_t (&words)[Mx4Block<FMT>::size / 8]) {
     constexpr int BS = Mx4Block<FMT>::size;
-    float a = 0.0f;
-    bool nan = false;
+    uint32_t top = 0;  // magnitudes order like unsigned integers, infinity and NaN above all
 #pragma unroll
-    for (int k = 0; k < BS; ++k) {
-        a = fmaxf(a, fabsf(v[k]));
-        nan |= v[k] != v[k];
-    }
+    for (int k = 0; k < BS; ++k) top = max(top, f2u(v[k]) & 0x7fffffffu);
+    const bool nan = top > 0x7f800000u;
+    const float a = u2f(top);
     if (FMT == GS3D_MXFP4) {
         const uint32_t byte = mxfp4_scale_byte(a);
         const float inv = u2f((254u - byte) << 23);  // 2^(127 - byte), byte <= 253
@@ -474,11 +474,11 @@ int launch_tensor_scale(const gs3d_rows* x, float* tensor_scale, cudaStream_t st
     const int64_t total = x->rows * x->dim;
     const bool wide = x->row_stride == x->dim && reinterpret_cast<uintptr_t>(in) % 16 == 0;
     uint32_t* out = reinterpret_cast<uint32_t*>(tensor_scale);
-    // up to 64 elements a thread one block is as fast as several and needs no zeroed result before it
-    const int grid = total <= 64 * 256 ? 1 : grid_for(ceil_div(total, N * 8), 256, 8);
+    // up to 128 elements a thread one block is as fast as several, which need a zeroed result first
+    const int grid = total <= 128 * kScaleThreads ? 1 : grid_for(ceil_div(total, N * 8), kScaleThreads, 4);
     if (grid > 1) GS3D_CUDA(cudaMemsetAsync(tensor_scale, 0, sizeof(float), stream), "memset tensor scale");
-    if (wide) k_mx4_tensor_scale<T, true><<<grid, 256, 0, stream>>>(in, x->rows, x->row_stride, x->dim, out);
-    else k_mx4_tensor_scale<T, false><<<grid, 256, 0, stream>>>(in, x->rows, x->row_stride, x->dim, out);
+    if (wide) k_mx4_tensor_scale<T, true><<<grid, kScaleThreads, 0, stream>>>(in, x->rows, x->row_stride, x->dim, out);
+    else k_mx4_tensor_scale<T, false><<<grid, kScaleThreads, 0, stream>>>(in, x->rows, x->row_stride, x->dim, out);
     GS3D_LAUNCHED("k_mx4_tensor_scale");
     return GS3D_OK;
 }
@@ -522,19 +522,6 @@ struct ShRow {
         for (int b = 0; b < NB; ++b) scale[b] = __ldg(a.scales + r * NB + b);
     }
 };
-
-// Rows 2 t and 2 t + 1 at degree 3 in NVFP4: 48 bytes of codes, 16-byte aligned, and 6 scales.
-__device__ __forceinline__ void load_neighbours(const Mx4Sh& a, int64_t r, ShRow<3, GS3D_NVFP4>& s0,
-                                                ShRow<3, GS3D_NVFP4>& s1) {
-    const uint4* p = reinterpret_cast<const uint4*>(a.codes + r * 24);
-    const uint4 x = __ldg(p), y = __ldg(p + 1), z = __ldg(p + 2);
-    s0.w[0] = x.x, s0.w[1] = x.y, s0.w[2] = x.z, s0.w[3] = x.w, s0.w[4] = y.x, s0.w[5] = y.y;
-    s1.w[0] = y.z, s1.w[1] = y.w, s1.w[2] = z.x, s1.w[3] = z.y, s1.w[4] = z.z, s1.w[5] = z.w;
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.scales + r * 3);
-    const uint32_t u = __ldg(q), v = __ldg(q + 1), w = __ldg(q + 2);
-    s0.scale[0] = u & 255u, s0.scale[1] = u >> 8, s0.scale[2] = v & 255u;
-    s1.scale[0] = v >> 8, s1.scale[1] = w & 255u, s1.scale[2] = w >> 8;
-}
 
 // Elements 8 k .. 8 k + 7 of two rows, times 2^-14.
 template <int DEG, int FMT>
@@ -629,17 +616,8 @@ __device__ __forceinline__ void colour_pair(const Mx4Sh& a, int order, int64_t r
     const Float2 mx(m0.x, m1.x), my(m0.y, m1.y), mz(m0.z, m1.z);
     if constexpr (WHOLE && DEG == 3) {
         ShRow<DEG, FMT> s0, s1;
-        bool loaded = false;
-        if constexpr (FMT == GS3D_NVFP4) {
-            if (a.neighbours && r1 == r0 + 1 && (r0 & 1) == 0) {
-                load_neighbours(a, r0, s0, s1);
-                loaded = true;
-            }
-        }
-        if (!loaded) {
-            s0.load(a, r0);
-            s1.load(a, r1);
-        }
+        s0.load(a, r0);
+        s1.load(a, r1);
         sh_basis_pair<DEG>(p, mx, my, mz, basis);
         block_factors(s0, s1, g, factor);
 #pragma unroll
@@ -662,24 +640,25 @@ struct Positions {
     float p[GS3D_MAX_FACTORED_VIEWS][3];
 };
 
-// Gaussians 2 t and 2 t + 1 a thread, all their operations in packed pairs. ONE: a single view; else
-// `views` of them a block, with the coefficients decoded once.
+// Gaussians i and i + 32 of a warp's 64 a thread (neighbouring lanes load and store neighbouring rows),
+// their operations in packed pairs. ONE: a single view; else `views` of them a block, with the elements
+// decoded once.
 template <int DEG, int FMT, bool WHOLE, bool ONE>
 __global__ void __launch_bounds__(128) k_mx4_colours(const Mx4Sh a, int order, const float4* __restrict__ mo4,
                                                      int n, const Positions cv, int nv, int views,
                                                      float4* __restrict__ out, int64_t view_stride) {
     constexpr int NC = (DEG + 1) * (DEG + 1);
-    const int64_t i = 2 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
+    const int64_t i = (int64_t)blockIdx.x * 256 + (threadIdx.x >> 5) * 64 + (threadIdx.x & 31);
     if (i >= n) return;
-    const bool two = i + 1 < n;
+    const bool two = i + 32 < n;
     const float g = FMT == GS3D_NVFP4 ? __ldg(a.tensor_scale) : 1.0f;
-    const int64_t r0 = sh_row(a, i), r1 = two ? sh_row(a, i + 1) : -1;
-    const float4 m0 = __ldg(mo4 + i), m1 = __ldg(mo4 + (two ? i + 1 : i));
+    const int64_t r0 = sh_row(a, i), r1 = two ? sh_row(a, i + 32) : -1;
+    const float4 m0 = __ldg(mo4 + i), m1 = __ldg(mo4 + (two ? i + 32 : i));
     if constexpr (ONE) {
         Float2 c[3];
         colour_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, cv.p[0], m0, m1, c);
         __stcs(out + i, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
-        if (two) __stcs(out + i + 1, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
+        if (two) __stcs(out + i + 32, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
     } else {
         Float2 h[(3 * NC + 7) / 8 * 8], factor[ShRow<DEG, FMT>::NB];
         load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h, factor);
@@ -691,7 +670,7 @@ __global__ void __launch_bounds__(128) k_mx4_colours(const Mx4Sh a, int order, c
             for (int ch = 0; ch < 3; ++ch) c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h + ch * NC, factor, basis);
             float4* o = out + (size_t)v * view_stride + i;
             __stcs(o, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
-            if (two) __stcs(o + 1, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
+            if (two) __stcs(o + 32, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
         }
     }
 }
@@ -705,9 +684,9 @@ __global__ void __launch_bounds__(128) k_mx4_render_colours(const Mx4Sh a, int o
                                                             const gs3d_camera cam, float* __restrict__ f2d) {
     const int F = counts[0];
     const float g = FMT == GS3D_NVFP4 ? __ldg(a.tensor_scale) : 1.0f;
-    for (int f = 2 * (blockIdx.x * blockDim.x + threadIdx.x); f < F; f += 2 * gridDim.x * blockDim.x) {
-        const bool two = f + 1 < F;
-        const int g0 = f2g[f] - 1, g1 = two ? f2g[f + 1] - 1 : g0;
+    for (int f = blockIdx.x * 256 + (threadIdx.x >> 5) * 64 + (threadIdx.x & 31); f < F; f += gridDim.x * 256) {
+        const bool two = f + 32 < F;
+        const int g0 = f2g[f] - 1, g1 = two ? f2g[f + 32] - 1 : g0;
         const float4 m0 = __ldg(mo4 + g0), m1 = __ldg(mo4 + g1);
         Float2 c[3];
         colour_pair<DEG, FMT, WHOLE>(a, order, sh_row(a, g0), sh_row(a, g1), g, cam.position, m0, m1, c);
@@ -715,7 +694,7 @@ __global__ void __launch_bounds__(128) k_mx4_render_colours(const Mx4Sh a, int o
 #pragma unroll
         for (int ch = 0; ch < 3; ++ch) {
             rr[6 + ch] = c[ch].x;
-            if (two) rr[15 + ch] = c[ch].y;
+            if (two) rr[9 * 32 + 6 + ch] = c[ch].y;
         }
     }
 }
@@ -805,10 +784,8 @@ struct RenderColoursLaunch {
 };
 
 Mx4Sh sh_source(const gs3d_mx4_rows* sh, const int32_t* indices) {
-    const bool neighbours = !indices && reinterpret_cast<uintptr_t>(sh->codes) % 16 == 0 &&
-                            reinterpret_cast<uintptr_t>(sh->scales) % 2 == 0;
     return Mx4Sh{sh->codes, sh->scales, sh->tensor_scale, indices, sh->rows, mx4_code_bytes(sh->dim),
-                 mx4_blocks(sh->dim, sh->format), neighbours};
+                 mx4_blocks(sh->dim, sh->format)};
 }
 
 }  // namespace

@@ -92,7 +92,6 @@ struct Mx4Sh {
     const int32_t* indices;
     int64_t rows;
     int code_bytes, blocks;
-    bool neighbours;  // rows in order, aligned so that two can be loaded together
 };
 
 }  // namespace gs3d

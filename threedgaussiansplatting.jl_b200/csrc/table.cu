@@ -87,21 +87,29 @@ __global__ void __launch_bounds__(256) k_table_lookup_flat(const TI* __restrict_
                                                            const int32_t* __restrict__ indices, float scale,
                                                            TO* __restrict__ out, int64_t total, int dim) {
     constexpr int N = lookup_pack<TI, TO>();
-    const int64_t e0 = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * N;
+    const int64_t block = (int64_t)blockIdx.x * (256 * N), e0 = block + threadIdx.x * N;
     if (e0 >= total) return;
-    int64_t r = e0 / dim;
-    int c = (int)(e0 - r * dim);
-    int k = __ldg(indices + r);
+    // the block's first row by one 64-bit division, the thread's from there by a 32-bit one
+    const int64_t r0 = block / dim;
+    const unsigned within = (unsigned)(block - r0 * dim) + threadIdx.x * N, dr = within / (unsigned)dim;
+    int left = dim - (int)(within - dr * dim);  // elements to the row's end
+    const int32_t* index = indices + r0 + dr;
+    auto row = [&](int c) -> const TI* {
+        const int k = __ldg(index);
+        return (unsigned)(k - 1) < (unsigned)rows ? table + (int64_t)(k - 1) * table_stride + c : nullptr;
+    };
+    const TI* p = row(dim - left);
     Pack<TO, N> o;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        float v = 0.0f;
-        if (e0 + j < total && k >= 1 && k <= rows) v = to_f32(__ldg(table + (int64_t)(k - 1) * table_stride + c)) * scale;
-        o.e[j] = from_f32<TO>(v);
-        if (++c == dim && e0 + j + 1 < total) {
-            c = 0;
-            k = __ldg(indices + ++r);
+        if (left == 0) {  // the next row, unless this was the last
+            left = dim;
+            ++index;
+            p = e0 + j < total ? row(0) : nullptr;
         }
+        o.e[j] = from_f32<TO>(p ? to_f32(__ldg(p)) * scale : 0.0f);
+        if (p) ++p;
+        --left;
     }
     if (e0 + N <= total) {
         store_streaming(out + e0, o);
@@ -490,7 +498,7 @@ template <typename T, int VB>
 __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ grads, int64_t stride, int dim,
                                                         const SegmentPlan pl, const Segments g) {
     using Unit = RowUnit<T, VB>;
-    constexpr int N = Unit::N, AHEAD = 4;
+    constexpr int N = Unit::N, AHEAD = VB == 16 ? 4 : 8;  // rows in flight a slot
     extern __shared__ __align__(16) unsigned char smem[];
     int32_t* sk = reinterpret_cast<int32_t*>(smem);  // the chunk's indices and rows
     int32_t* sv = sk + pl.chunk;
@@ -635,12 +643,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_table_join(int dim, int nch
         const int lk = long_run[q];
         if (lk < 0) continue;
         const int lb = blockIdx.x * kJoinWarps + q;
+        int end = lb + 1;  // the run's last chunk is end - 1
+        for (int more = 32 * kJoinWarps; more == 32 * kJoinWarps; end += more) {
+            const int c = end + threadIdx.x;
+            more = __syncthreads_count(c < nchunks && g.first_key[c] == lk);
+        }
         float s = 0.0f;
         if (on) {
             if (slot == 0) s = g.partial[((int64_t)lb * 2 + 1) * dim + col];
-#pragma unroll 4
-            for (int c = lb + 1 + slot; c < nchunks && g.first_key[c] == lk; c += slots)
-                s += g.partial[(int64_t)c * 2 * dim + col];
+#pragma unroll 8
+            for (int c = lb + 1 + slot; c < end; c += slots) s += g.partial[(int64_t)c * 2 * dim + col];
         }
         part[threadIdx.x] = s;
         __syncthreads();

@@ -14,6 +14,7 @@ returns and its workspace there, and does not synchronise; it can be captured in
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import numpy as np
@@ -31,31 +32,33 @@ def _rows_c(t: torch.Tensor, what: str) -> _abi.RowsC:
     kind = _TYPES.get(t.dtype)
     if kind is None:
         raise ValueError(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
-    if t.dim() < 2:
-        raise ValueError(f"{what}: need (rows, ...), got shape {tuple(t.shape)}")
-    rows, dim = t.shape[0], 1
-    for size in t.shape[1:]:
+    shape = t.shape
+    if len(shape) < 2:
+        raise ValueError(f"{what}: need (rows, ...), got shape {tuple(shape)}")
+    rows, dim = shape[0], shape[1]
+    for size in shape[2:]:
         dim *= size
     if t.is_contiguous():
-        stride = dim
-    else:
-        expect = 1
-        for size, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if size != 1 and st != expect:
-                raise ValueError(f"{what}: the elements of a row must be contiguous")
-            expect *= size
-        stride = t.stride(0) if rows > 1 else dim
-        if stride < dim:
-            raise ValueError(f"{what}: rows overlap (row stride {stride}, {dim} elements)")
+        return _abi.RowsC(rows, dim, dim, kind, t.data_ptr())
+    expect = 1
+    for size, st in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and st != expect:
+            raise ValueError(f"{what}: the elements of a row must be contiguous")
+        expect *= size
+    stride = t.stride(0) if rows > 1 else dim
+    if stride < dim:
+        raise ValueError(f"{what}: rows overlap (row stride {stride}, {dim} elements)")
     return _abi.RowsC(rows, stride, dim, kind, t.data_ptr())
 
 
-def _check_device(first: torch.Tensor, *others) -> None:
-    if first.device.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, not {first.device}")
+def _check_device(first: torch.Tensor, *others) -> torch.device:
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {device}")
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+    return device
 
 
 def _check_indices(t: torch.Tensor | None, what: str = "indices") -> None:
@@ -63,28 +66,33 @@ def _check_indices(t: torch.Tensor | None, what: str = "indices") -> None:
         raise ValueError(f"{what} must be a contiguous (n,) int32 tensor (1-based)")
 
 
-class _On:
-    """The tensors' device and the call's stream made current, so that what the call allocates
-    belongs to that stream; nothing to do when they are already."""
+def _enter(device: torch.device, stream: torch.cuda.Stream | None):
+    """(raw stream, context): makes the tensors' device and the call's stream current, so that what the
+    call allocates belongs to that stream; context None where they are already. These calls can cost
+    less on the GPU than their host side, so the raw handle is asked for without a Stream object."""
+    index = device.index
+    if stream is None:
+        if index == torch.cuda.current_device():
+            return torch._C._cuda_getCurrentRawStream(index), None
+        context = torch.cuda.device(device)
+    elif stream.device != device:
+        raise ValueError(f"stream on {stream.device} for tensors on {device}")
+    else:
+        context = torch.cuda.stream(stream)
+    context.__enter__()
+    return torch._C._cuda_getCurrentRawStream(index), context
 
-    def __init__(self, device: torch.device, stream: torch.cuda.Stream | None):
-        if stream is not None and stream.device != device:
-            raise ValueError(f"stream on {stream.device} for tensors on {device}")
-        self.ctx = None
-        if stream is not None:
-            self.ctx = torch.cuda.stream(stream)
-        elif device.index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(device)
-        self.device = device
 
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+def _leave(context) -> None:
+    if context is not None:
+        context.__exit__(None, None, None)
 
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+
+@functools.lru_cache(maxsize=256)
+def _gradient_workspace_bytes(grad_rows: int, table_rows: int, dim: int) -> int:
+    nbytes = C.c_size_t(0)
+    _abi.check(_abi.lib().gs3d_table_gradient_workspace_size(grad_rows, table_rows, dim, C.byref(nbytes)))
+    return nbytes.value
 
 
 # -- tables -----------------------------------------------------------------------------------
@@ -95,16 +103,19 @@ def table_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 1.0,
     bfloat16) for 1-based int32 `indices`; an index outside 1 .. rows gives zeros. Products are
     fp32, rounded once to `dtype` (default: the table's). `out` ((n, ...)) is filled in place."""
     _check_indices(indices)
-    _check_device(table, indices, out)
+    device = _check_device(table, indices, out)
     t = _rows_c(table, "table")
     shape = (indices.shape[0], *table.shape[1:])
-    with _On(table.device, stream) as handle:
+    handle, context = _enter(device, stream)
+    try:
         if out is None:
-            out = torch.empty(shape, dtype=dtype or table.dtype, device=table.device)
+            out = torch.empty(shape, dtype=dtype or table.dtype, device=device)
         elif out.shape != shape or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a lookup of {shape} {dtype or out.dtype}")
         o = _rows_c(out, "out")
-        _abi.check(_abi.lib().gs3d_table_lookup(C.byref(t), indices.data_ptr(), scale, C.byref(o), handle))
+        _abi.check(_abi.lib().gs3d_table_lookup(t, indices.data_ptr(), scale, o, handle))
+    finally:
+        _leave(context)
     return out
 
 
@@ -120,7 +131,7 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
     `device_counts`: only the first device_counts[0] rows take part. `accumulate`: add to `out`."""
     _check_indices(indices)
     _check_indices(fgidx_to_gidx, "fgidx_to_gidx")
-    _check_device(grads, indices, fgidx_to_gidx, device_counts, out)
+    device = _check_device(grads, indices, fgidx_to_gidx, device_counts, out)
     g = _rows_c(grads, "grads")
     if fgidx_to_gidx is not None and fgidx_to_gidx.shape[0] < g.rows:
         raise ValueError(f"{fgidx_to_gidx.shape[0]} fgidx_to_gidx entries for {g.rows} rows")
@@ -129,21 +140,22 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     shape = (int(nb_rows), *grads.shape[1:])
-    with _On(grads.device, stream) as handle:
+    handle, context = _enter(device, stream)
+    try:
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=grads.device)
+            out = torch.empty(shape, dtype=torch.float32, device=device)
         elif out.shape != shape or out.dtype != torch.float32:
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a float32 table gradient of {shape}")
         o = _rows_c(out, "out")
-        lib = _abi.lib()
-        nbytes = C.c_size_t(0)
-        _abi.check(lib.gs3d_table_gradient_workspace_size(g.rows, o.rows, g.dim, C.byref(nbytes)))
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=grads.device)
-        _abi.check(lib.gs3d_table_gradient(
-            C.byref(g), indices.data_ptr(), indices.shape[0],
+        nbytes = _gradient_workspace_bytes(g.rows, o.rows, g.dim)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _abi.check(_abi.lib().gs3d_table_gradient(
+            g, indices.data_ptr(), indices.shape[0],
             None if fgidx_to_gidx is None else fgidx_to_gidx.data_ptr(),
-            None if device_counts is None else device_counts.data_ptr(), scale, C.byref(o),
-            _abi.GS3D_TABLE_ACCUMULATE if accumulate else 0, ws.data_ptr(), nbytes.value, handle))
+            None if device_counts is None else device_counts.data_ptr(), scale, o,
+            _abi.GS3D_TABLE_ACCUMULATE if accumulate else 0, ws.data_ptr(), nbytes, handle))
+    finally:
+        _leave(context)
     return out
 
 
@@ -151,11 +163,14 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
 def mx4_tensor_scale(x: torch.Tensor, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """(1,) float32: max(largest finite |x| / 2688, 2^-100), the nvfp4 tensor scale with which no
     block of `x` ((rows, ...)) saturates."""
-    _check_device(x)
+    device = _check_device(x)
     c = _rows_c(x, "x")
-    with _On(x.device, stream) as handle:
-        scale = torch.empty(1, dtype=torch.float32, device=x.device)
-        _abi.check(_abi.lib().gs3d_mx4_tensor_scale(C.byref(c), scale.data_ptr(), handle))
+    handle, context = _enter(device, stream)
+    try:
+        scale = torch.empty(1, dtype=torch.float32, device=device)
+        _abi.check(_abi.lib().gs3d_mx4_tensor_scale(c, scale.data_ptr(), handle))
+    finally:
+        _leave(context)
     return scale
 
 
@@ -164,25 +179,36 @@ def mx4_quantise(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Ten
     """The rows of `x` ((rows, ...), float32, float16 or bfloat16) as 4-bit elements with block
     scales (gs3d_mx4_quantise). `tensor_scale` (nvfp4): (1,) float32 on the device, within 2^-100 ..
     2^100; None: mx4_tensor_scale(x)."""
-    _check_device(x, tensor_scale)
+    device = _check_device(x, tensor_scale)
     c = _rows_c(x, "x")
-    with _On(x.device, stream) as handle:
-        if format == "nvfp4" and tensor_scale is None:
-            tensor_scale = mx4_tensor_scale(x)
-        q = MX4Rows.empty(c.rows, c.dim, format, x.device, tensor_scale)
-        _abi.check(_abi.lib().gs3d_mx4_quantise(C.byref(c), C.byref(q.to_c()), handle))
+    handle, context = _enter(device, stream)
+    try:
+        if format == "nvfp4":
+            if tensor_scale is None:
+                tensor_scale = torch.empty(1, dtype=torch.float32, device=device)
+                _abi.check(_abi.lib().gs3d_mx4_tensor_scale(c, tensor_scale.data_ptr(), handle))
+            elif tensor_scale.numel() != 1 or tensor_scale.dtype != torch.float32:
+                raise ValueError("the tensor scale is (1,) float32")
+        elif tensor_scale is not None:
+            raise ValueError(f"{format} rows have no tensor scale")
+        q = MX4Rows.empty(c.rows, c.dim, format, device, tensor_scale)
+        _abi.check(_abi.lib().gs3d_mx4_quantise(c, q.to_c(), handle))
+    finally:
+        _leave(context)
     return q
 
 
 def mx4_dequantise(rows: MX4Rows, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
                    stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """The values `rows` stand for as (rows, dim) `dtype`, or into `out` ((rows, ...) of dim elements)."""
-    _check_device(rows.codes, out)
-    with _On(rows.device, stream) as handle:
+    device = _check_device(rows.codes, out)
+    handle, context = _enter(device, stream)
+    try:
         if out is None:
-            out = torch.empty((rows.rows, rows.dim), dtype=dtype, device=rows.device)
-        o = _rows_c(out, "out")
-        _abi.check(_abi.lib().gs3d_mx4_dequantise(C.byref(rows.to_c()), C.byref(o), handle))
+            out = torch.empty((rows.rows, rows.dim), dtype=dtype, device=device)
+        _abi.check(_abi.lib().gs3d_mx4_dequantise(rows.to_c(), _rows_c(out, "out"), handle))
+    finally:
+        _leave(context)
     return out
 
 
@@ -197,21 +223,24 @@ def mx4_colours(rows: MX4Rows, means: torch.Tensor, positions, sh_degree: int,
     if pos.ndim != 2 or pos.shape[1] != 3:
         raise ValueError(f"positions must be (views, 3), got {pos.shape}")
     _check_indices(indices)
-    _check_device(rows.codes, means, indices, out)
+    device = _check_device(rows.codes, means, indices, out)
     n = means.shape[0]
     if means.shape != (n, 4) or means.dtype != torch.float32 or not means.is_contiguous():
         raise ValueError("means must be a contiguous (n, 4) float32 tensor")
     if indices is not None and indices.shape[0] != n:
         raise ValueError(f"{indices.shape[0]} indices for {n} Gaussians")
     shape = (pos.shape[0], n, 4)
-    with _On(rows.device, stream) as handle:
+    handle, context = _enter(device, stream)
+    try:
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=rows.device)
+            out = torch.empty(shape, dtype=torch.float32, device=device)
         elif out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
         _abi.check(_abi.lib().gs3d_mx4_colours(
-            C.byref(rows.to_c()), int(sh_degree), None if indices is None else indices.data_ptr(),
-            means.data_ptr(), n, pos.ctypes.data, pos.shape[0], out.data_ptr(), n, handle))
+            rows.to_c(), int(sh_degree), None if indices is None else indices.data_ptr(),
+            means.data_ptr(), n, pos.__array_interface__["data"][0], pos.shape[0], out.data_ptr(), n, handle))
+    finally:
+        _leave(context)
     return out
 
 

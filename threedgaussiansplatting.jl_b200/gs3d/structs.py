@@ -410,9 +410,11 @@ class MX4Rows:
     def empty(cls, rows: int, dim: int, format: str, device, tensor_scale=None) -> "MX4Rows":
         if format not in MX4_FORMATS:
             raise ValueError(f"4-bit format {format!r} is not in {sorted(MX4_FORMATS)}")
-        blocks = -(-dim // MX4_FORMATS[format][1])
-        return cls(torch.empty((rows, (dim + 1) // 2), dtype=torch.uint8, device=device),
-                   torch.empty((rows, blocks), dtype=torch.uint8, device=device), tensor_scale, dim, format)
+        q = object.__new__(cls)  # right by construction: not checked again
+        q.codes = torch.empty((rows, (dim + 1) // 2), dtype=torch.uint8, device=device)
+        q.scales = torch.empty((rows, -(-dim // MX4_FORMATS[format][1])), dtype=torch.uint8, device=device)
+        q.tensor_scale, q.dim, q.format = tensor_scale, dim, format
+        return q
 
     @property
     def rows(self) -> int:
@@ -432,8 +434,9 @@ class MX4Rows:
                        None if ts is None else ts.to(device), self.dim, self.format)
 
     def to_c(self) -> _abi.MX4RowsC:
-        return _abi.MX4RowsC(self.codes.shape[0], self.dim, MX4_FORMATS[self.format][0],
-                             _ptr(self.codes), _ptr(self.scales), _ptr(self.tensor_scale))
+        ts = self.tensor_scale
+        return _abi.MX4RowsC(self.codes.shape[0], self.dim, MX4_FORMATS[self.format][0], self.codes.data_ptr(),
+                             self.scales.data_ptr(), None if ts is None else ts.data_ptr())
 
 
 @dataclass

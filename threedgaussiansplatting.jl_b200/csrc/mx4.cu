@@ -212,34 +212,6 @@ __global__ void __launch_bounds__(256) k_mx4_quantise_blocks(const T* __restrict
     *reinterpret_cast<Pack<uint32_t, BS / 8>*>(codes + i * (BS / 2)) = o;
 }
 
-// `bytes` bytes between global and shared memory, 16 at a time where the global side allows it (its
-// first `skip` bytes come before a 16-byte border; the shared side starts at its own offset `skip`
-// behind a border, so that both sides' packs are aligned).
-__device__ __forceinline__ int head_of(const void* p) { return (int)(reinterpret_cast<uintptr_t>(p) & 15); }
-
-__device__ __forceinline__ void copy_in(unsigned char* sh, const unsigned char* gl, int64_t bytes) {
-    // sh + head_of(gl) is where the first byte goes
-    const int h = head_of(gl);
-    const int64_t end = h + bytes;
-    const unsigned char* g0 = gl - h;
-    const int64_t first = h ? 16 : 0, last = end & ~(int64_t)15;
-    for (int64_t i = h + threadIdx.x; i < min(first, end); i += blockDim.x) sh[i] = g0[i];
-    for (int64_t i = first + 16 * (int64_t)threadIdx.x; i < last; i += 16 * (int64_t)blockDim.x)
-        *reinterpret_cast<uint4*>(sh + i) = *reinterpret_cast<const uint4*>(g0 + i);
-    for (int64_t i = max(first, last) + threadIdx.x; i < end; i += blockDim.x) sh[i] = g0[i];
-}
-
-__device__ __forceinline__ void copy_out(unsigned char* gl, const unsigned char* sh, int64_t bytes) {
-    const int h = head_of(gl);
-    const int64_t end = h + bytes;
-    unsigned char* g0 = gl - h;
-    const int64_t first = h ? 16 : 0, last = end & ~(int64_t)15;
-    for (int64_t i = h + threadIdx.x; i < min(first, end); i += blockDim.x) g0[i] = sh[i];
-    for (int64_t i = first + 16 * (int64_t)threadIdx.x; i < last; i += 16 * (int64_t)blockDim.x)
-        *reinterpret_cast<uint4*>(g0 + i) = *reinterpret_cast<const uint4*>(sh + i);
-    for (int64_t i = max(first, last) + threadIdx.x; i < end; i += blockDim.x) g0[i] = sh[i];
-}
-
 // Rows of any length (they may end inside a block): a CTA takes `per` rows, which lie back to back, as
 // one range of bytes through shared memory, and hands the codes back the same way.
 template <typename T, int FMT>
@@ -409,8 +381,6 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise(const uint8_t* __restric
         out[r * stride + k] = from_f32<T>(k & 1 ? two.y : two.x);
     }
 }
-
-constexpr int kRowsBytes = 16 << 10;  // the most that a CTA's rows take in shared memory
 
 // Rows a CTA of the *_rows kernels takes: a block for each of its 256 threads, as far as they fit.
 int rows_per_cta(int row_bytes, int row_blocks) {

@@ -38,7 +38,7 @@ inline int check_rows(const gs3d_rows* r, const char* what) {
     if (!r) return invalid("NULL %s", what);
     if (r->rows < 0 || r->rows > kMaxRows) return invalid("%s: %lld rows", what, (long long)r->rows);
     if (r->dim < 1 || r->dim > kMaxRowDim) return invalid("%s: dim = %d (1 .. %d)", what, r->dim, kMaxRowDim);
-    if (r->row_stride < r->dim || r->row_stride > ((int64_t)1 << 32))
+    if (r->row_stride < r->dim || r->row_stride > INT_MAX)
         return invalid("%s: row stride %lld with dim %d", what, (long long)r->row_stride, r->dim);
     if (r->type != GS3D_F32 && r->type != GS3D_F16 && r->type != GS3D_BF16)
         return invalid("%s: element type %d", what, r->type);
@@ -47,6 +47,35 @@ inline int check_rows(const gs3d_rows* r, const char* what) {
         return invalid("%s: data not aligned to its elements", what);
     return GS3D_OK;
 }
+
+// `bytes` bytes between global and shared memory, 16 at a time where both sides allow it: the shared
+// side's first byte is head_of(global side) bytes behind `sh`, which is 16-byte aligned, so that the
+// borders of both coincide.
+__device__ __forceinline__ int head_of(const void* p) { return (int)(reinterpret_cast<uintptr_t>(p) & 15); }
+
+__device__ __forceinline__ void copy_in(unsigned char* sh, const unsigned char* gl, int64_t bytes) {
+    const int h = head_of(gl);
+    const int64_t end = h + bytes;
+    const unsigned char* g0 = gl - h;
+    const int64_t first = h ? 16 : 0, last = end & ~(int64_t)15;
+    for (int64_t i = h + threadIdx.x; i < min(first, end); i += blockDim.x) sh[i] = g0[i];
+    for (int64_t i = first + 16 * (int64_t)threadIdx.x; i < last; i += 16 * (int64_t)blockDim.x)
+        *reinterpret_cast<uint4*>(sh + i) = __ldg(reinterpret_cast<const uint4*>(g0 + i));
+    for (int64_t i = max(first, last) + threadIdx.x; i < end; i += blockDim.x) sh[i] = g0[i];
+}
+
+__device__ __forceinline__ void copy_out(unsigned char* gl, const unsigned char* sh, int64_t bytes) {
+    const int h = head_of(gl);
+    const int64_t end = h + bytes;
+    unsigned char* g0 = gl - h;
+    const int64_t first = h ? 16 : 0, last = end & ~(int64_t)15;
+    for (int64_t i = h + threadIdx.x; i < min(first, end); i += blockDim.x) g0[i] = sh[i];
+    for (int64_t i = first + 16 * (int64_t)threadIdx.x; i < last; i += 16 * (int64_t)blockDim.x)
+        __stcs(reinterpret_cast<uint4*>(g0 + i), *reinterpret_cast<const uint4*>(sh + i));
+    for (int64_t i = max(first, last) + threadIdx.x; i < end; i += blockDim.x) g0[i] = sh[i];
+}
+
+constexpr int kRowsBytes = 16 << 10;  // the most that a CTA's rows take in shared memory
 
 // Call f(integral constant) with the element type of a checked gs3d_rows.
 template <typename F>

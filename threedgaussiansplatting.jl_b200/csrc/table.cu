@@ -11,19 +11,12 @@
 namespace gs3d {
 namespace {
 
-int grid_for(int64_t items, int threads, int per_sm) {
-    const int64_t b = std::min<int64_t>(ceil_div(items, threads), (int64_t)device_sm_count() * per_sm);
-    return (int)std::max<int64_t>(b, 1);
-}
-
 // ---- lookup ----------------------------------------------------------------------------------
-// Bound by the rows written (the table stays in L2). Three forms, by alignment:
-//   k_table_lookup_units   rows in units of N elements (16 bytes of the wider type): threads side by side on a
-//                          row's units, kLookupRows rows a thread, as many independent loads in flight
-//   k_table_lookup_flat    rows of any length, output contiguous: a thread fills N consecutive elements of the
-//                          output, across a row's end where it comes, and stores them at once
-//   k_table_lookup_scalar  everything else: an element a thread
-constexpr int kLookupRows = 4;  // 1 / 2 / 4 / 8: 129 / 103 / 94 / 117 us at 3M x 48 fp32 (a write-only fill: 79)
+// Bound by the rows written (the table stays in L2). Threads side by side on a row's units of N
+// elements, ROWS rows a thread, as many independent loads in flight. A unit is 16 bytes of the wider of
+// table and output (two half types: of both) where all rows are so aligned, else one element.
+// 3M x 48 fp32, 1 / 2 / 4 / 8 rows: 129 / 103 / 94 / 117 us (a write-only fill: 79).
+constexpr int kLookupRows = 4, kLookupColumns = 2;
 
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Pack {
@@ -31,109 +24,76 @@ struct alignas(N * sizeof(T)) Pack {
 };
 
 // A pack of 8 or 16 bytes to memory that is not read again soon: streamed, so that it does not push
-// the table out of L2 (104 us without, 94 with).
+// the table out of L2 (104 us without, 94 with). Single elements go the ordinary way: L2 joins them.
 template <typename T, int N>
 __device__ __forceinline__ void store_streaming(T* p, const Pack<T, N>& v) {
-    using W = typename std::conditional<sizeof(v) == 16, uint4, uint2>::type;
-    static_assert(sizeof(v) == sizeof(W), "packs of 8 or 16 bytes");
-    __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&v));
+    if constexpr (N == 1) {
+        *p = v.e[0];
+    } else {
+        using W = typename std::conditional<sizeof(v) == 16, uint4, uint2>::type;
+        static_assert(sizeof(v) == sizeof(W), "packs of 8 or 16 bytes");
+        __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&v));
+    }
 }
 
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
-    using W = typename std::conditional<sizeof(Pack<T, N>) == 16, uint4, uint2>::type;
-    const W w = __ldg(reinterpret_cast<const W*>(p));
-    return *reinterpret_cast<const Pack<T, N>*>(&w);
+    if constexpr (N == 1) {
+        return Pack<T, N>{__ldg(p)};
+    } else {
+        using W = typename std::conditional<sizeof(Pack<T, N>) == 16, uint4, uint2>::type;
+        const W w = __ldg(reinterpret_cast<const W*>(p));
+        return *reinterpret_cast<const Pack<T, N>*>(&w);
+    }
 }
 
 template <typename TI, typename TO>
 constexpr int lookup_pack() { return sizeof(TI) == 2 && sizeof(TO) == 2 ? 8 : 4; }
 
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(256) k_table_lookup_units(const TI* __restrict__ table, int rows,
-                                                            int64_t table_stride,
-                                                            const int32_t* __restrict__ indices, float scale,
-                                                            TO* __restrict__ out, int n, int64_t out_stride,
-                                                            int units, int tile_units, int slots) {
-    constexpr int N = lookup_pack<TI, TO>();
+template <typename TI, typename TO, int N, int ROWS, int COLS>
+__global__ void __launch_bounds__(256) k_table_lookup(const TI* __restrict__ table, int rows, int table_stride,
+                                                      const int32_t* __restrict__ indices, float scale,
+                                                      TO* __restrict__ out, int n, int64_t out_stride, int units,
+                                                      int tile_units, int slots) {
     const int slot = threadIdx.x / tile_units;
-    const int unit = blockIdx.y * tile_units + threadIdx.x - slot * tile_units;
+    const int unit = blockIdx.y * (COLS * tile_units) + threadIdx.x - slot * tile_units;  // and COLS - 1 more, tile_units apart
     if (unit >= units) return;
-    const int first = blockIdx.x * (slots * kLookupRows) + slot;
-    int k[kLookupRows];
-#pragma unroll
-    for (int q = 0; q < kLookupRows; ++q) k[q] = __ldg(indices + min(first + q * slots, n - 1));
-    Pack<TI, N> v[kLookupRows];
-#pragma unroll
-    for (int q = 0; q < kLookupRows; ++q) {
-        v[q] = Pack<TI, N>{};
-        if ((unsigned)(k[q] - 1) < (unsigned)rows)
-            v[q] = load_pack<TI, N>(table + (int64_t)(k[q] - 1) * table_stride + unit * N);
-    }
+    const int first = blockIdx.x * (slots * ROWS) + slot;
+    const TI* column = table + unit * N;
+    const int32_t* index = indices + first;
     TO* o = out + first * out_stride + unit * N;
+    const int64_t step = slots * out_stride;
+    const auto rows_of_thread = [&](auto full) {
+        int k[ROWS];
 #pragma unroll
-    for (int q = 0; q < kLookupRows; ++q) {
-        Pack<TO, N> p;
+        for (int q = 0; q < ROWS; ++q) k[q] = full || first + q * slots < n ? __ldg(index + q * slots) - 1 : -1;
+        Pack<TI, N> v[ROWS][COLS];
 #pragma unroll
-        for (int c = 0; c < N; ++c) p.e[c] = from_f32<TO>(to_f32(v[q].e[c]) * scale);
-        if ((unsigned)(k[q] - 1) >= (unsigned)rows) p = Pack<TO, N>{};  // zeros even for a NaN or infinite scale
-        if (first + q * slots < n) store_streaming(o + q * slots * out_stride, p);
-    }
-}
-
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(256) k_table_lookup_flat(const TI* __restrict__ table, int rows,
-                                                           int64_t table_stride,
-                                                           const int32_t* __restrict__ indices, float scale,
-                                                           TO* __restrict__ out, int64_t total, int dim) {
-    constexpr int N = lookup_pack<TI, TO>();
-    const int64_t block = (int64_t)blockIdx.x * (256 * N), e0 = block + threadIdx.x * N;
-    if (e0 >= total) return;
-    // the block's first row by one 64-bit division, the thread's from there by a 32-bit one
-    const int64_t r0 = block / dim;
-    const unsigned within = (unsigned)(block - r0 * dim) + threadIdx.x * N, dr = within / (unsigned)dim;
-    int left = dim - (int)(within - dr * dim);  // elements to the row's end
-    const int32_t* index = indices + r0 + dr;
-    auto row = [&](int c) -> const TI* {
-        const int k = __ldg(index);
-        return (unsigned)(k - 1) < (unsigned)rows ? table + (int64_t)(k - 1) * table_stride + c : nullptr;
-    };
-    const TI* p = row(dim - left);
-    Pack<TO, N> o;
+        for (int q = 0; q < ROWS; ++q) {
+            const TI* p = column + (int64_t)k[q] * table_stride;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        if (left == 0) {  // the next row, unless this was the last
-            left = dim;
-            ++index;
-            p = e0 + j < total ? row(0) : nullptr;
+            for (int j = 0; j < COLS; ++j) {
+                v[q][j] = Pack<TI, N>{};
+                if ((unsigned)k[q] < (unsigned)rows && (j == 0 || unit + j * tile_units < units))
+                    v[q][j] = load_pack<TI, N>(p + j * tile_units * N);
+            }
         }
-        o.e[j] = from_f32<TO>(p ? to_f32(__ldg(p)) * scale : 0.0f);
-        if (p) ++p;
-        --left;
-    }
-    if (e0 + N <= total) {
-        store_streaming(out + e0, o);
-    } else {
-        for (int j = 0; e0 + j < total; ++j) out[e0 + j] = o.e[j];
-    }
-}
-
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(256) k_table_lookup_scalar(const TI* __restrict__ table, int rows,
-                                                             int64_t table_stride,
-                                                             const int32_t* __restrict__ indices, float scale,
-                                                             TO* __restrict__ out, int64_t n, int64_t out_stride,
-                                                             int dim) {
-    const int64_t total = n * dim;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-         i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / dim;
-        const int c = (int)(i - r * dim);
-        const int k = indices[r];
-        float v = 0.0f;
-        if (k >= 1 && k <= rows) v = to_f32(table[(int64_t)(k - 1) * table_stride + c]) * scale;
-        out[r * out_stride + c] = from_f32<TO>(v);
-    }
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) {
+            const float f = (unsigned)k[q] < (unsigned)rows ? scale : 0.0f;  // zeros whatever the scale
+#pragma unroll
+            for (int j = 0; j < COLS; ++j) {
+                Pack<TO, N> p;
+#pragma unroll
+                for (int c = 0; c < N; ++c) p.e[c] = from_f32<TO>(to_f32(v[q][j].e[c]) * f);
+                if ((full || first + q * slots < n) && (j == 0 || unit + j * tile_units < units))
+                    store_streaming(o + j * tile_units * N, p);
+            }
+            o += step;
+        }
+    };
+    if ((int)(blockIdx.x + 1) * (slots * ROWS) <= n) rows_of_thread(std::true_type{});
+    else rows_of_thread(std::false_type{});
 }
 
 template <typename T>
@@ -141,29 +101,26 @@ bool packs(const gs3d_rows* r, int n) {
     return r->dim % n == 0 && r->row_stride % n == 0 && reinterpret_cast<uintptr_t>(r->data) % (n * sizeof(T)) == 0;
 }
 
+template <typename TI, typename TO, int N, int ROWS, int COLS>
+int launch_lookup_units(const gs3d_rows* table, const int32_t* indices, float scale, const gs3d_rows* out,
+                        cudaStream_t stream) {
+    const int units = out->dim / N, tile_units = std::min((int)ceil_div(units, COLS), 256);
+    const int slots = std::max(1, 256 / tile_units);
+    const dim3 grid((unsigned)ceil_div(out->rows, (int64_t)slots * ROWS), (unsigned)ceil_div(units, COLS * tile_units));
+    k_table_lookup<TI, TO, N, ROWS, COLS><<<grid, slots * tile_units, 0, stream>>>(
+        static_cast<const TI*>(table->data), (int)table->rows, (int)table->row_stride, indices, scale,
+        static_cast<TO*>(out->data), (int)out->rows, out->row_stride, units, tile_units, slots);
+    GS3D_LAUNCHED("k_table_lookup");
+    return GS3D_OK;
+}
+
 template <typename TI, typename TO>
 int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, const gs3d_rows* out,
                   cudaStream_t stream) {
     constexpr int N = lookup_pack<TI, TO>();
-    const TI* t = static_cast<const TI*>(table->data);
-    TO* o = static_cast<TO*>(out->data);
-    const int rows = (int)table->rows, dim = out->dim;
-    const int64_t n = out->rows, total = n * dim;
-    if (packs<TI>(table, N) && packs<TO>(out, N)) {
-        const int units = dim / N, tile_units = std::min(units, 256), slots = std::max(1, 256 / tile_units);
-        const dim3 grid((unsigned)ceil_div(n, (int64_t)slots * kLookupRows), (unsigned)ceil_div(units, tile_units));
-        k_table_lookup_units<TI, TO><<<grid, slots * tile_units, 0, stream>>>(
-            t, rows, table->row_stride, indices, scale, o, (int)n, out->row_stride, units, tile_units, slots);
-    } else if (out->row_stride == dim && reinterpret_cast<uintptr_t>(o) % (N * sizeof(TO)) == 0 &&
-               total / N / 256 < INT_MAX) {
-        k_table_lookup_flat<TI, TO><<<(unsigned)ceil_div(total, N * 256), 256, 0, stream>>>(
-            t, rows, table->row_stride, indices, scale, o, total, dim);
-    } else {
-        k_table_lookup_scalar<TI, TO><<<grid_for(total, 256, 8), 256, 0, stream>>>(
-            t, rows, table->row_stride, indices, scale, o, n, out->row_stride, dim);
-    }
-    GS3D_LAUNCHED("k_table_lookup");
-    return GS3D_OK;
+    if (packs<TI>(table, N) && packs<TO>(out, N))
+        return launch_lookup_units<TI, TO, N, kLookupRows, 1>(table, indices, scale, out, stream);
+    return launch_lookup_units<TI, TO, 1, kLookupRows, kLookupColumns>(table, indices, scale, out, stream);
 }
 
 // ---- gradient --------------------------------------------------------------------------------
@@ -234,11 +191,11 @@ struct ZeroRows {
     }
 };
 
+// An item: x the row's index - 1 in the table, y the row.
 struct SortPass {
-    int32_t* keys_in;  // the first pass: all rows' keys, -1 without one, written by its count kernel
-    const int32_t* vals_in;  // NULL: the first pass, values are the rows themselves
-    int32_t* keys_out;
-    int32_t* vals_out;
+    int32_t* first_keys;  // the first pass: all rows' indices, -1 without one, written by its count kernel
+    const int2* in;       // NULL: the first pass
+    int2* out;
     int32_t* hist;    // [bin][tile]: counts, then their exclusive scan over the tiles
     int32_t* totals;  // [bin]
     int32_t* valid;   // number of rows with a valid index (written by the first pass)
@@ -256,21 +213,21 @@ __global__ void __launch_bounds__(kSortThreads) k_radix_count(const SortPass p, 
     const int nbins = 1 << p.bits, tile = blockIdx.x, place = tile_place(tile);
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) bins[b] = 0;
     int key[kSortRounds];
-    if (!p.vals_in) {
+    if (!p.in) {
         src.keys(place, key);
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r)
-            if (place + 32 * r < p.n) p.keys_in[place + 32 * r] = key[r];
+            if (place + 32 * r < p.n) p.first_keys[place + 32 * r] = key[r];
     } else {
         const int m = *p.valid;
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) key[r] = place + 32 * r < m ? p.keys_in[place + 32 * r] : -1;
+        for (int r = 0; r < kSortRounds; ++r) key[r] = place + 32 * r < m ? p.in[place + 32 * r].x : -1;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r)
         if (key[r] >= 0) atomicAdd(&bins[(key[r] >> p.shift) & (nbins - 1)], 1);
-    if (!p.vals_in) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
+    if (!p.in) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
     __syncthreads();
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) p.hist[(int64_t)b * p.ntiles + tile] = bins[b];
 }
@@ -292,82 +249,123 @@ __global__ void __launch_bounds__(kSpineThreads) k_radix_spine(const SortPass p)
 }
 
 size_t radix_scatter_smem(int bits) {
-    return (size_t)kSortTile * 8 + (size_t)(1 << bits) * (8 + 2 * kSortWarps);
+    return (size_t)kSortTile * 8 + (size_t)(1 << bits) * (4 + 2 * kSortWarps);
+}
+
+// Exclusive block scan of one 64-bit value per thread of kSortThreads.
+__device__ __forceinline__ int64_t block_exclusive_scan64(int64_t v, int64_t* sm) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+    }
+    if (lane == 31) sm[w] = inc;
+    __syncthreads();
+    if (w == 0) {
+        int64_t t = lane < kSortWarps ? sm[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < kSortWarps; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += u;
+        }
+        if (lane < kSortWarps) sm[lane] = t;
+    }
+    __syncthreads();
+    return inc - v + (w ? sm[w - 1] : 0);
 }
 
 __global__ void __launch_bounds__(kSortThreads, 3) k_radix_scatter(const SortPass p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int sm[33];
+    __shared__ int64_t sm[kSortWarps];
+    constexpr int BINS = (1 << kMaxDigitBits) / kSortThreads;  // of a thread, at most
     const int nbins = 1 << p.bits, tile = blockIdx.x;
-    int32_t* keys = reinterpret_cast<int32_t*>(smem);            // the tile in digit order
-    int32_t* vals = keys + kSortTile;
-    int32_t* start = vals + kSortTile;                           // first place of a bin in the tile
-    int32_t* dest = start + nbins;                               // its place in the output, minus start
+    int2* items = reinterpret_cast<int2*>(smem);                   // the tile in digit order
+    int32_t* dest = reinterpret_cast<int32_t*>(items + kSortTile);  // a bin's place in the output, minus in the tile
     uint16_t* wcount = reinterpret_cast<uint16_t*>(dest + nbins);  // [warp][bin]
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int place = tile_place(tile), m = p.vals_in ? *p.valid : p.n;
-    int key[kSortRounds], val[kSortRounds];
+    const int place = tile_place(tile), m = p.in ? *p.valid : p.n;
+    int2 item[kSortRounds];
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
         const int i = place + 32 * r;
-        key[r] = i < m ? p.keys_in[i] : -1;
-        val[r] = p.vals_in && i < m ? p.vals_in[i] : i;
+        item[r] = make_int2(-1, i);
+        if (i < m) {
+            if (p.in) item[r] = p.in[i];
+            else item[r].x = p.first_keys[i];
+        }
+    }
+    // this thread's bins: totals over all tiles, and over the tiles before this one
+    int total[BINS], before_tile[BINS];
+    const int bins = max(1, nbins / kSortThreads), bin0 = threadIdx.x * bins;
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) {
+        const bool on = b < bins && bin0 + b < nbins;
+        total[b] = on ? p.totals[bin0 + b] : 0;
+        before_tile[b] = on ? p.hist[(int64_t)(bin0 + b) * p.ntiles + tile] : 0;
     }
     for (int i = threadIdx.x; i < nbins * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(wcount)[i] = 0;
     __syncthreads();
-    // stable rank of every key among its warp's keys of the same digit
+    // stable rank of every key among its warp's keys of the same digit: first within its 32 (all matches
+    // in flight together), then behind the 32s before
     int rank[kSortRounds];
     const unsigned below = (1u << lane) - 1u;
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
-        const int d = key[r] >= 0 ? (key[r] >> p.shift) & (nbins - 1) : nbins;
+        const int d = item[r].x >= 0 ? (item[r].x >> p.shift) & (nbins - 1) : nbins;
         const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const int before = d < nbins ? wcount[w * nbins + d] : 0;
-        rank[r] = before + __popc(peers & below);
+        rank[r] = __popc(peers & below) | __popc(peers) << 8;
+    }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+        const bool on = item[r].x >= 0;
+        uint16_t& c = wcount[w * nbins + (on ? (item[r].x >> p.shift) & (nbins - 1) : 0)];
+        const int before = c, mine = rank[r] & 255, peers = rank[r] >> 8;
+        rank[r] = before + mine;
         __syncwarp();
-        if (d < nbins && (peers & below) == 0) wcount[w * nbins + d] = (uint16_t)(before + __popc(peers));
+        if (on && mine == 0) c = (uint16_t)(before + peers);
         __syncwarp();
     }
     __syncthreads();
-    // places of the bins in the tile (over this tile's counts) and in the output (over all totals)
-    int here = 0, everywhere = 0;
-    for (int b0 = 0; b0 < nbins; b0 += kSortThreads) {
-        const int b = b0 + threadIdx.x;
-        int run = 0, total = 0, tot;
-        if (b < nbins) {
+    // places of the bins in the tile (low words, over this tile's counts) and in the output (high words,
+    // over all totals)
+    int here[BINS];
+    int64_t sum = 0;
+#pragma unroll
+    for (int b = 0; b < BINS; ++b) {
+        here[b] = 0;
+        if (b < bins && bin0 + b < nbins)
+#pragma unroll
+            for (int ww = 0; ww < kSortWarps; ++ww) here[b] += wcount[ww * nbins + bin0 + b];
+        sum += ((int64_t)total[b] << 32) + here[b];
+    }
+    int64_t base = block_exclusive_scan64(sum, sm);
+    const int64_t all = sm[kSortWarps - 1];
+#pragma unroll
+    for (int b = 0; b < BINS; ++b)
+        if (b < bins && bin0 + b < nbins) {
+            int at = (int)base;
+            dest[bin0 + b] = (int)(base >> 32) + before_tile[b] - at;
 #pragma unroll
             for (int ww = 0; ww < kSortWarps; ++ww) {
-                const int c = wcount[ww * nbins + b];
-                wcount[ww * nbins + b] = (uint16_t)run;
-                run += c;
+                uint16_t& c = wcount[ww * nbins + bin0 + b];
+                const int count = c;
+                c = (uint16_t)at;
+                at += count;
             }
-            total = p.totals[b];
+            base += ((int64_t)total[b] << 32) + here[b];
         }
-        const int st = here + block_exclusive_scan(run, sm, &tot);
-        here += tot;
-        const int base = everywhere + block_exclusive_scan(total, sm, &tot);
-        everywhere += tot;
-        if (b < nbins) {
-            start[b] = st;
-            dest[b] = base + p.hist[(int64_t)b * p.ntiles + tile] - st;
-        }
-    }
-    if (!p.vals_in && tile == 0 && threadIdx.x == 0) *p.valid = everywhere;
+    if (!p.in && tile == 0 && threadIdx.x == 0) *p.valid = (int32_t)(all >> 32);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r)
-        if (key[r] >= 0) {
-            const int d = (key[r] >> p.shift) & (nbins - 1);
-            const int at = start[d] + wcount[w * nbins + d] + rank[r];
-            keys[at] = key[r];
-            vals[at] = val[r];
-        }
+        if (item[r].x >= 0) items[wcount[w * nbins + ((item[r].x >> p.shift) & (nbins - 1))] + rank[r]] = item[r];
     __syncthreads();
-    for (int i = threadIdx.x; i < here; i += kSortThreads) {
-        const int k = keys[i];
-        const int o = dest[(k >> p.shift) & (nbins - 1)] + i;
-        p.keys_out[o] = k;
-        p.vals_out[o] = vals[i];
+    const int count = (int)all;
+    for (int i = threadIdx.x; i < count; i += kSortThreads) {
+        const int2 it = items[i];
+        p.out[dest[(it.x >> p.shift) & (nbins - 1)] + i] = it;
     }
 }
 
@@ -377,8 +375,7 @@ constexpr int kSmallWarps = kSmallThreads / 32;
 constexpr int kSmallRounds = kSortTile / kSmallThreads;
 
 __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource src, const ZeroRows zero, int bits,
-                                                              int32_t* __restrict__ keys_out,
-                                                              int32_t* __restrict__ vals_out,
+                                                              int2* __restrict__ out,
                                                               int32_t* __restrict__ valid) {
     __shared__ int keys[kSortTile], vals[kSortTile];
     __shared__ uint16_t wcount[kSmallWarps][256];
@@ -437,10 +434,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource sr
             }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < count; i += kSmallThreads) {
-        keys_out[i] = keys[i];
-        vals_out[i] = vals[i];
-    }
+    for (int i = threadIdx.x; i < count; i += kSmallThreads) out[i] = make_int2(keys[i], vals[i]);
     if (threadIdx.x == 0) *valid = count;
     if (gridDim.x == 1) zero.fill(threadIdx.x, kSmallThreads);
 }
@@ -472,8 +466,7 @@ struct SegmentPlan {
 };
 
 struct Segments {
-    const int32_t* keys;   // sorted
-    const int32_t* vals;
+    const int2* items;     // sorted
     const int32_t* valid;
     float* out;
     int64_t out_stride;
@@ -495,14 +488,13 @@ __device__ __forceinline__ void store_row(const Segments& g, int key, int col, c
 }
 
 template <typename T, int VB>
-__global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ grads, int64_t stride, int dim,
+__global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const T* __restrict__ grads, int stride, int dim,
                                                         const SegmentPlan pl, const Segments g) {
     using Unit = RowUnit<T, VB>;
     constexpr int N = Unit::N, AHEAD = VB == 16 ? 4 : 8;  // rows in flight a slot
     extern __shared__ __align__(16) unsigned char smem[];
-    int32_t* sk = reinterpret_cast<int32_t*>(smem);  // the chunk's indices and rows
-    int32_t* sv = sk + pl.chunk;
-    int32_t* pkey = sv + pl.chunk;                   // [slot][2]: the slots' first and last runs
+    int2* items = reinterpret_cast<int2*>(smem);                  // the chunk's
+    int32_t* pkey = reinterpret_cast<int32_t*>(items + pl.chunk);  // [slot][2]: the slots' first and last runs
     float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);  // [slot][2][tile_units * N]
     const int m = *g.valid;
     const int begin = blockIdx.x * pl.chunk, count = min(pl.chunk, m - begin);
@@ -511,10 +503,7 @@ __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ gr
         if (meta) g.first_key[blockIdx.x] = g.owned[blockIdx.x] = -1;
         return;
     }
-    for (int i = threadIdx.x; i < count; i += blockDim.x) {
-        sk[i] = g.keys[begin + i];
-        sv[i] = g.vals[begin + i];
-    }
+    for (int i = threadIdx.x; i < count; i += blockDim.x) items[i] = __ldg(g.items + begin + i);
     __syncthreads();
     const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
     const int unit = blockIdx.y * pl.tile_units + lane;
@@ -524,22 +513,33 @@ __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ gr
     {
         const int j1 = min((slot + 1) * pl.run, count);
         int j = slot * pl.run;
-        int cur = j < j1 ? sk[j] : -1;
+        int cur = j < j1 ? items[j].x : -1;
         bool first = true;
         float acc[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-        const T* gc = grads + col;
+        const T* gc = grads + (on ? col : 0);
         for (; j < j1; j += AHEAD) {
             Unit u[AHEAD];
+            int key[AHEAD];
 #pragma unroll
-            for (int q = 0; q < AHEAD; ++q)
-                if (on && j + q < j1) u[q].load(gc + (int64_t)sv[j + q] * stride);
+            for (int q = 0; q < AHEAD; ++q) {
+                const int2 it = items[min(j + q, j1 - 1)];
+                key[q] = it.x;
+                u[q].load(gc + (int64_t)it.y * stride);
+            }
+            const bool whole = j + AHEAD <= j1;
+            if (whole && key[AHEAD - 1] == cur) {  // sorted: all of them are
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] += to_f32(u[q].e[i]);
+                continue;
+            }
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) {
                 if (j + q >= j1) break;
-                const int k = sk[j + q];
-                if (k != cur) {
+                if (key[q] != cur) {
                     if (first) {
 #pragma unroll
                         for (int i = 0; i < N; ++i) part[(2 * slot) * width + lane * N + i] = acc[i];
@@ -548,13 +548,12 @@ __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ gr
                     } else if (on) {
                         store_row<N>(g, cur, col, acc);
                     }
-                    cur = k;
+                    cur = key[q];
 #pragma unroll
                     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
                 }
-                if (on)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) acc[i] += to_f32(u[q].e[i]);
+                for (int i = 0; i < N; ++i) acc[i] += to_f32(u[q].e[i]);
             }
         }
         const int which = 2 * slot + (first ? 0 : 1);
@@ -568,13 +567,13 @@ __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ gr
     __syncthreads();
     if (slot != 0) return;
     // the slots' open runs in order
-    const bool open_left = begin > 0 && g.keys[begin - 1] == sk[0];
-    const int last = sk[count - 1];
-    const bool open_right = begin + count < m && g.keys[begin + count] == last;
+    const bool open_left = begin > 0 && g.items[begin - 1].x == items[0].x;
+    const int last = items[count - 1].x;
+    const bool open_right = begin + count < m && g.items[begin + count].x == last;
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-    int cur = sk[0];
+    int cur = items[0].x;
     bool first = true;
     float* partial = g.partial + (int64_t)blockIdx.x * 2 * dim + col;
     for (int e = 0; e < 2 * pl.slots; ++e) {
@@ -607,7 +606,7 @@ __global__ void __launch_bounds__(256) k_table_segments(const T* __restrict__ gr
         }
     }
     if (meta) {
-        g.first_key[blockIdx.x] = sk[0];
+        g.first_key[blockIdx.x] = items[0].x;
         g.owned[blockIdx.x] = open_right && !earlier ? last : -1;
     }
 }
@@ -666,7 +665,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_table_join(int dim, int nch
 }
 
 struct GradLayout {
-    size_t keys[2], vals[2], hist, totals, valid, first_key, owned, partial, total;
+    size_t first_keys, items[2], hist, totals, valid, first_key, owned, partial, total;
     int ntiles, passes, bits, chunks_max;
 };
 
@@ -704,9 +703,9 @@ GradLayout grad_layout(int64_t n, int64_t rows, int dim) {
     for (int units = dim; units >= 1; units = units % 2 == 0 ? units / 2 : 0)
         L.chunks_max = std::max(L.chunks_max, segment_plan(n, units).nchunks);
     size_t off = 0;
+    L.first_keys = off; off += align256((size_t)n * 4);
     for (int i = 0; i < 2; ++i) {
-        L.keys[i] = off; off += align256((size_t)n * 4);
-        L.vals[i] = off; off += align256((size_t)n * 4);
+        L.items[i] = off; off += i < L.passes ? align256((size_t)n * 8) : 0;
     }
     L.hist = off; off += align256((size_t)L.ntiles * ((size_t)1 << digit) * 4);
     L.totals = off; off += align256(((size_t)1 << kMaxDigitBits) * 4);
@@ -774,6 +773,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return invalid("workspace not 256-byte aligned");
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     const auto at = [&](size_t off) { return reinterpret_cast<int32_t*>(ws + off); };
+    const auto items = [&](int i) { return reinterpret_cast<int2*>(ws + L.items[i]); };
     const bool accumulate = (flags & GS3D_TABLE_ACCUMULATE) != 0;
     float* out = static_cast<float*>(table_grads->data);
     const KeySource src{indices, fgidx_to_gidx, device_counts, n_indices, (int32_t)n, (int32_t)table_grads->rows};
@@ -784,11 +784,10 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     if (n <= kSortTile) {
         const int64_t words = accumulate ? 0 : table_grads->rows * table_grads->dim;
         const int fillers = (int)std::min<int64_t>(ceil_div(words, kSmallThreads * 8), 4 * kSMs);
-        k_sort_small<<<1 + fillers, kSmallThreads, 0, stream>>>(src, zero, L.bits, at(L.keys[0]), at(L.vals[0]),
-                                                                at(L.valid));
+        k_sort_small<<<1 + fillers, kSmallThreads, 0, stream>>>(src, zero, L.bits, items(0), at(L.valid));
         GS3D_LAUNCHED("k_sort_small");
     } else {
-        SortPass p{at(L.keys[1]), nullptr, nullptr, nullptr, at(L.hist), at(L.totals), at(L.valid), (int32_t)n, L.ntiles, 0, 0};
+        SortPass p{at(L.first_keys), nullptr, nullptr, at(L.hist), at(L.totals), at(L.valid), (int32_t)n, L.ntiles, 0, 0};
         const int digit = (L.bits + L.passes - 1) / L.passes;
         const size_t smem = radix_scatter_smem(digit);
         GS3D_CUDA(cudaFuncSetAttribute(k_radix_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -797,21 +796,19 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
         for (int i = 0; i < L.passes; ++i) {
             p.shift = i * digit;
             p.bits = digit;
-            p.keys_out = at(L.keys[i & 1]);
-            p.vals_out = at(L.vals[i & 1]);
+            p.out = items(i & 1);
             k_radix_count<<<L.ntiles, kSortThreads, 0, stream>>>(p, src, zero);
             GS3D_LAUNCHED("k_radix_count");
             k_radix_spine<<<1 << digit, kSpineThreads, 0, stream>>>(p);
             GS3D_LAUNCHED("k_radix_spine");
             k_radix_scatter<<<L.ntiles, kSortThreads, smem, stream>>>(p);
             GS3D_LAUNCHED("k_radix_scatter");
-            p.keys_in = p.keys_out;
-            p.vals_in = p.vals_out;
+            p.in = p.out;
             sorted = i & 1;
         }
     }
     if (n == 0) return GS3D_OK;
-    const Segments seg{at(L.keys[sorted]), at(L.vals[sorted]), at(L.valid), out, table_grads->row_stride, scale,
+    const Segments seg{items(sorted), at(L.valid), out, table_grads->row_stride, scale,
                        accumulate ? 1 : 0, at(L.first_key), at(L.owned), reinterpret_cast<float*>(ws + L.partial)};
     return dispatch_type(grads->type, [&](auto t) {
         using T = typename decltype(t)::T;
@@ -824,8 +821,9 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
         const size_t smem = (size_t)pl.chunk * 8 + (size_t)pl.slots * 8 + (size_t)pl.slots * 2 * pl.tile_units * per * 4;
         const dim3 grid(pl.nchunks, (unsigned)ceil_div(pl.units, pl.tile_units));
         const int threads = pl.slots * pl.tile_units;
-        if (wide) k_table_segments<T, 16><<<grid, threads, smem, stream>>>(g, grads->row_stride, grads->dim, pl, seg);
-        else k_table_segments<T, (int)sizeof(T)><<<grid, threads, smem, stream>>>(g, grads->row_stride, grads->dim, pl, seg);
+        const int stride = (int)grads->row_stride;
+        if (wide) k_table_segments<T, 16><<<grid, threads, smem, stream>>>(g, stride, grads->dim, pl, seg);
+        else k_table_segments<T, (int)sizeof(T)><<<grid, threads, smem, stream>>>(g, stride, grads->dim, pl, seg);
         GS3D_LAUNCHED("k_table_segments");
         k_table_join<<<dim3((unsigned)ceil_div(pl.nchunks, kJoinWarps), (unsigned)ceil_div(grads->dim, 256)),
                        32 * kJoinWarps, 0, stream>>>(grads->dim, pl.nchunks, seg);

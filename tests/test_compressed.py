@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 import torch
 
-from gs3d import CompressedGaussiansVector, MX4Rows, _abi
+from gs3d import CompressedGaussiansVector, MX4Rows, _abi, io, scripts
 from gs3d import compressed as gc
 
 LIB = _abi.lib()
@@ -215,3 +215,32 @@ def test_calls_need_cuda_tensors_of_the_right_kind():
         gc.SHTable(torch.zeros(4, 3, 5), i)
     with pytest.raises(ValueError):
         gc.fit_table(torch.zeros(4, 3, 16), 0)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("table", [False, True])
+def test_compressed_model_file_round_trip(tmp_path, fmt, table):
+    gen = torch.Generator().manual_seed(1)
+    n, rows = 9, 4 if table else 9
+    byte = lambda *s: torch.randint(0, 256, s, generator=gen, dtype=torch.uint8)  # noqa: E731
+    sh = MX4Rows(byte(rows, 14), byte(rows, 2 if fmt == "nvfp4" else 1),
+                 torch.tensor([0.3]) if fmt == "nvfp4" else None, 27, fmt)
+    idx = torch.randint(0, 6, (n,), generator=gen, dtype=torch.int32) if table else None
+    g = CompressedGaussiansVector(torch.randn(n, 4, generator=gen), torch.randn(n, 6, generator=gen), sh, idx)
+    io.save_compressed(tmp_path / "m.npz", g)
+    b = io.load_compressed(tmp_path / "m.npz")
+    assert (b.sh.format, b.sh.dim, b.sh_degree) == (fmt, 27, 2)
+    for x, y in ((g.means_opacities, b.means_opacities), (g.covariances, b.covariances), (sh.codes, b.sh.codes),
+                 (sh.scales, b.sh.scales)):
+        assert torch.equal(x, y)
+    assert (b.indices is None) == (not table) and (not table or torch.equal(b.indices, idx))
+    assert (b.sh.tensor_scale is None) == (fmt == "mxfp4")
+
+
+def test_compressed_model_file_refusals(tmp_path):
+    import numpy as np
+    np.savez(tmp_path / "x.npz", a=np.zeros(3))
+    with pytest.raises(ValueError, match="not a compressed"):
+        io.load_compressed(tmp_path / "x.npz")
+    with pytest.raises(ValueError, match="npz"):
+        scripts.compress(tmp_path / "m.ply", tmp_path / "m.ply", device="cpu")

@@ -654,3 +654,95 @@ def test_fit_table(cuda):
     rows = table.expand()
     assert table.coeffs.shape == (2, 3, 4) and float((rows - sh).abs().max()) < 0.2
     assert gc.fit_table(sh[:3], 10).rows == 3
+
+
+# -- training and scripts ---------------------------------------------------------------------------
+def table_scene(cuda, n=1500, rows=60):
+    g = synthetic_gaussians(SceneSpec(n, "uniform:1", -3.5, 0.4), 2).to(cuda)
+    cams = [look_at_camera(96, 64, 60.0, (2.5 * np.cos(a), 0.4, 2.5 * np.sin(a))) for a in (0.0, 2.0, 4.0)]
+    targets = [torch.rand(96, 64, 3, generator=rng(i)).to(cuda) for i in range(3)]
+    til = Tiling.for_camera(cams[0])
+    return g, gc.fit_table(g.sh_coeffs, rows, iterations=2), cams, targets, RenderOptions.for_camera(cams[0], 3), til
+
+
+def test_table_trainer_step_is_its_parts(cuda):
+    """One step against the chain of public calls it is made of, and against the plain trainer: the
+    geometry takes the same step as Trainer's on the expanded coefficients (Adam is per scalar), and the
+    table takes Adam's first step, -lr sign(gradient), on the gradient that the sums of the Gaussians'
+    SH gradients give."""
+    from gs3d.backward import FilteredGaussiansGradients, backward
+    from gs3d.loss import LossComputer
+    from gs3d.training import TableTrainer, TrainingOptions
+    g, table, cams, targets, ro, til = table_scene(cuda)
+    before, geometry = table.coeffs.clone(), [t.clone() for t in g.tensors()[:3]]
+    opts = TrainingOptions(scene_radius=2.5)
+    tr = TableTrainer(g, table, cams, targets, ro, til, opts, seed=4)
+    tr.training_step()
+    idx = tr.current_camera_index()
+    torch.cuda.synchronize()
+    # the same gradients from the parts
+    expanded = gc.table_lookup(before, table.indices)
+    model = GaussiansVector(*geometry, expanded.contiguous())
+    out, buf = RenderOutputs.create(96, 64, cuda), RenderBuffers.create(g.n, til.nb_tiles, cuda)
+    gs3d.render(out, model, cams[idx], til, ro, buf)
+    grad = torch.empty(96, 64, 3, device=cuda)
+    LossComputer(96, 64, cuda, opts.loss_dssim_vs_L1_weight)(out.rgb, targets[idx], grad)
+    fg = FilteredGaussiansGradients.create(g.n, 3, cuda)
+    backward(fg, grad, out, model, cams[idx], til, ro, buf)
+    F, _ = gs3d.counts(buf)
+    want, bound = gradient_exact(fg.sh_coeffs_grads[:F].cpu(), table.indices.cpu(), table.rows, 1.0,
+                                 buf.fgidx_to_gidx[:F].cpu())
+    # the backward's float atomics: 1e-3 of the gradient's size between two runs, as elsewhere
+    got = tr._table_gradients.sh_coeffs_grads[:table.rows].cpu().double().view(table.rows, -1)
+    assert float((got - want).norm()) <= 1e-3 * float(want.norm())
+    used = want.abs() > 1e-3 * want.abs().max()
+    step = (table.coeffs - before).cpu().double().view(table.rows, -1)
+    lr = torch.full((3, 16), opts.sh_coeffs_rest_lr, dtype=torch.float64)
+    lr[:, 0] = opts.sh_coeffs_dc_lr
+    # m / (1 - b1) = g and v / (1 - b2) = g^2 up to a few roundings each; coefficients move by lr within
+    # 16 u of that and the rounding of a coefficient below 2
+    assert ((step + lr.view(-1) * want.sign())[used].abs() <= 16 * U * lr.max() + 2 * U).all()
+    assert all(not torch.equal(a, b) for a, b in zip(g.tensors()[:3], geometry))
+    assert torch.equal(g.sh_coeffs, expanded)  # what this step rendered
+
+
+def test_table_trainer_runs(cuda):
+    from gs3d.training import TableTrainer, TrainingOptions
+    g, table, cams, targets, ro, til = table_scene(cuda)
+    n = g.n
+    tr = TableTrainer(g, table, cams, targets, ro, til,
+                      TrainingOptions(scene_radius=2.5, sh_degree_increase_interval=2, opacity_reset_interval=2,
+                                      adc_interval=1, adc_start_iteration_nb=1))
+    for _ in range(6):
+        loss = tr.training_step()
+    torch.cuda.synchronize()
+    assert g.n == n and bool(torch.isfinite(loss[:3]).all()) and bool(torch.isfinite(table.coeffs).all())
+    model = gc.compress(g, "nvfp4", table=table)  # and on to 4 bits
+    out = RenderOutputs.create(96, 64, cuda)
+    gs3d.render(out, model, cams[0], til, ro, RenderBuffers.create(n, til.nb_tiles, cuda))
+    assert bool(torch.isfinite(out.rgb).all())
+    from gs3d import io
+    with pytest.raises(ValueError):
+        io.save_checkpoint("/dev/null", tr)
+    with pytest.raises(ValueError):
+        TableTrainer(g, gc.SHTable(table.coeffs.half(), table.indices), cams, targets, ro, til,
+                     TrainingOptions(scene_radius=2.5))
+    with pytest.raises(ValueError):
+        TableTrainer(g, gc.SHTable(table.coeffs, table.indices[:-1]), cams, targets, ro, til,
+                     TrainingOptions(scene_radius=2.5))
+
+
+@pytest.mark.parametrize("table_rows", [None, 30])
+def test_compress_and_render_scripts(cuda, tmp_path, table_rows):
+    from gs3d import io, scripts
+    g = synthetic_gaussians(SceneSpec(2_000, "uniform:1", -3.5, 0.5), 7)
+    io.save_ply(tmp_path / "m.ply", g)
+    cams = [look_at_camera(64, 48, 60.0, (0, 0.3, 3))]
+    log = []
+    model = scripts.compress(tmp_path / "m.ply", tmp_path / "m.npz", table_rows=table_rows, log=log.append)
+    assert len(log) == 1 and (model.indices is None) == (table_rows is None)
+    a = scripts.render(tmp_path / "m.npz", cameras=cams)[0]
+    out, til = RenderOutputs.create(64, 48, cuda), Tiling.for_camera(cams[0])
+    gs3d.render(out, model, cams[0], til, RenderOptions.for_camera(cams[0], 3),
+                RenderBuffers.create(g.n, til.nb_tiles, cuda))
+    assert torch.equal(a, out.rgb)

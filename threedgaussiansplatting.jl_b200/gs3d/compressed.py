@@ -275,6 +275,9 @@ class SHTable:
         return table_gradient(fgradients.sh_coeffs_grads, self.indices, self.rows, self.scale, out,
                               accumulate, buffers.fgidx_to_gidx, buffers.device_counts, stream)
 
+    def to(self, device) -> "SHTable":
+        return SHTable(self.coeffs.to(device), self.indices.to(device), self.scale)
+
 
 def fit_table(sh_coeffs: torch.Tensor, nb_rows: int, iterations: int = 10, seed: int = 0) -> SHTable:
     """A table of (at most) `nb_rows` rows for `sh_coeffs` ((n, 3, order) float32 on a CUDA device)

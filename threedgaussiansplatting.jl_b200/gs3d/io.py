@@ -16,6 +16,8 @@
   (default 0.2 / inf), `rotation` = camera-to-world rotation as a list of rows, `position` = the
   camera centre. `save_cameras_json` writes the reference's `JSON.lower` fields
   (cameras.jl:508-522), plus `path` per camera when image paths are given (:1182-1190).
+* Compressed models (no counterpart in the reference): `save_compressed` / `load_compressed` keep a
+  CompressedGaussiansVector's arrays as they are in an .npz file.
 * Training checkpoints (the reference has none): parameters, Adam moments and update count,
   ADC accumulators, iteration number, render SH degree and the camera-order state, so that a
   resumed `Trainer` takes the same views and steps as the uninterrupted run (the backward's
@@ -30,7 +32,8 @@ from pathlib import Path
 import numpy as np
 import torch
 
-from .structs import DEFAULT_FAR, DEFAULT_NEAR, F32, GaussiansVector, PinholeCamera
+from .structs import (DEFAULT_FAR, DEFAULT_NEAR, F32, CompressedGaussiansVector, GaussiansVector,
+                      MX4Rows, PinholeCamera)
 
 _PLY_TYPES = {
     "char": "i1", "int8": "i1", "uchar": "u1", "uint8": "u1", "short": "i2", "int16": "i2",
@@ -177,6 +180,37 @@ def load_model_or_point_cloud(path, device="cpu") -> GaussiansVector:
     return gaussians_from_point_cloud(pts, cols, device=device)
 
 
+# -- compressed models ------------------------------------------------------------------------
+_COMPRESSED_TAG = "gs3d-compressed-1"
+
+
+def save_compressed(path, model: CompressedGaussiansVector) -> None:
+    """Write a compressed model as an .npz file."""
+    a = {"tag": np.array(_COMPRESSED_TAG), "format": np.array(model.sh.format),
+         "dim": np.array(model.sh.dim, dtype=np.int32),
+         "means_opacities": model.means_opacities, "covariances": model.covariances,
+         "codes": model.sh.codes, "scales": model.sh.scales}
+    if model.sh.tensor_scale is not None:
+        a["tensor_scale"] = model.sh.tensor_scale
+    if model.indices is not None:
+        a["indices"] = model.indices
+    with open(path, "wb") as f:  # np.savez adds a suffix to a name without one
+        np.savez(f, **{k: v.detach().cpu().numpy() if isinstance(v, torch.Tensor) else v
+                       for k, v in a.items()})
+
+
+def load_compressed(path, device="cpu") -> CompressedGaussiansVector:
+    """Read `save_compressed`'s file."""
+    with np.load(path, allow_pickle=False) as z:
+        if "tag" not in z or str(z["tag"]) != _COMPRESSED_TAG:
+            raise ValueError(f"{path}: not a compressed gs3d model")
+        t = {k: torch.from_numpy(np.ascontiguousarray(z[k])).to(device)
+             for k in ("means_opacities", "covariances", "codes", "scales", "tensor_scale", "indices")
+             if k in z}
+        sh = MX4Rows(t["codes"], t["scales"], t.get("tensor_scale"), int(z["dim"]), str(z["format"]))
+        return CompressedGaussiansVector(t["means_opacities"], t["covariances"], sh, t.get("indices"))
+
+
 # -- cameras.json -----------------------------------------------------------------------------
 def _f32(x) -> float:
     return float(F32(x))
@@ -232,6 +266,8 @@ def save_cameras_json(path, cameras, image_paths=None) -> None:
 def save_checkpoint(path, trainer) -> None:
     """Everything a Trainer needs to continue: parameters, Adam moments and update count, ADC
     accumulators, iteration number, render SH degree, camera-order state."""
+    if hasattr(trainer, "sh_table"):
+        raise ValueError("checkpoints hold a model with its own SH coefficients, not a shared table")
     if trainer.device.type == "cuda":
         torch.cuda.synchronize(trainer.device)
     if hasattr(trainer, "sync_parameters"):  # data-parallel: all-gathers still in flight

@@ -215,13 +215,16 @@ def model_path(path, iterations=None) -> Path:
 def render(path, out_dir=None, *, iterations=None, cameras=None, sh_degree=None,
            image_format: str = "ppm", device="cuda") -> list[torch.Tensor]:
     """Render the model at `path` (a .ply, or a training output directory), loaded as a
-    RenderOnlyGaussiansVector like the script does, for each camera (by
+    RenderOnlyGaussiansVector like the script does, or the compressed model of an .npz
+    (`compress`), for each camera (by
     default the output directory's cameras.json, else `default_camera()`); write
     `out_dir/render_<i>.<image_format>` when `out_dir` is given. Returns the (width, height, 3)
     images on the device."""
     device = torch.device(device)
     p = Path(path)
-    g = io.load_ply_render_only(model_path(p, iterations), device=device)  # as the script loads it
+    mp = model_path(p, iterations)
+    g = (io.load_compressed(mp, device=device) if mp.suffix == ".npz"
+         else io.load_ply_render_only(mp, device=device))  # as the script loads it
     if cameras is None:
         cameras = (io.load_cameras_json(p / "cameras.json")
                    if p.is_dir() and (p / "cameras.json").exists() else [default_camera()])
@@ -241,3 +244,24 @@ def render(path, out_dir=None, *, iterations=None, cameras=None, sh_degree=None,
         if out_dir is not None:
             write_image(Path(out_dir) / f"render_{i:05d}.{image_format}", img)
     return images
+
+
+# -- compress ---------------------------------------------------------------------------------
+def compress(path, out_path, *, iterations=None, format: str = "nvfp4", table_rows: int | None = None,
+             table_iterations: int = 10, device="cuda", seed: int = 0, log=print):
+    """Compress the model at `path` (a .ply, or a training output directory) for rendering and write it
+    to `out_path` (.npz, which `render` takes): its SH coefficients in 4 bits, every Gaussian's own
+    (`table_rows=None`) or those of a shared table of `table_rows` rows fitted to them. Returns the
+    CompressedGaussiansVector. No counterpart in the reference."""
+    from .compressed import compress as compress_model
+    from .compressed import fit_table
+    if Path(out_path).suffix != ".npz":
+        raise ValueError(f"{out_path}: compressed models are .npz files")
+    g = io.load_ply_render_only(model_path(path, iterations), device=device)
+    table = None if table_rows is None else fit_table(g.sh_coeffs, int(table_rows), table_iterations, seed)
+    model = compress_model(g, format, table)
+    io.save_compressed(out_path, model)
+    held = model.sh.nbytes + (0 if model.indices is None else 4 * g.n)
+    log(f"Compressed the SH coefficients of {g.n} Gaussians from {g.sh_coeffs.numel() * 4} to {held} "
+        f"bytes: {out_path}")
+    return model

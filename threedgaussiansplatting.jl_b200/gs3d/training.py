@@ -279,6 +279,19 @@ class Trainer:
             self._gt_ready[slot].record(cs)
         self._prefetched = (idx, t, slot)
 
+    def prepare_model(self) -> None:
+        """What a model needs before every render (nothing; TableTrainer expands its table)."""
+
+    def update_model(self, cam: PinholeCamera, rebuild: bool) -> None:
+        """The optimizer step on this iteration's gradients."""
+        rb = self.render_buffers
+        if rebuild:
+            self.optimizer.update_rebuild_sh(self.fgradients, rb.fgidx_to_gidx, rb.device_counts,
+                                             rb.f2d, cam.position, self.render_options.sh_degree)
+        else:
+            self.optimizer.update(self.fgradients, rb.fgidx_to_gidx, rb.device_counts,
+                                  self.render_options.sh_degree)
+
     def training_step(self) -> torch.Tensor:
         """One iteration; returns the device tensor [loss, L1, DSSIM, -] (no host sync)."""
         self.iteration_nb += 1
@@ -287,6 +300,7 @@ class Trainer:
         idx = self.current_camera_index()
         cam = self.cameras[idx]
         rb = self.render_buffers
+        self.prepare_model()
         render(self.render_outputs, self.gaussians, cam, self.tiling, self.render_options, rb,
                host_sync=self.render_host_sync)
         gt = self.target_for(idx)
@@ -300,14 +314,68 @@ class Trainer:
                  self.tiling, self.render_options, rb, skip_sh_grads=rebuild)
         in_adc = self.maybe_densify_and_prune()
         self.update_learning_rates()
-        if rebuild:
-            self.optimizer.update_rebuild_sh(self.fgradients, rb.fgidx_to_gidx, rb.device_counts,
-                                             rb.f2d, cam.position, self.render_options.sh_degree)
-        else:
-            self.optimizer.update(self.fgradients, rb.fgidx_to_gidx, rb.device_counts,
-                                  self.render_options.sh_degree)
+        self.update_model(cam, rebuild)
         if in_adc:
             self.complete_adc_step()
         self.maybe_opacity_reset()
         self.last_loss = loss
         return loss
+
+
+class TableTrainer(Trainer):
+    """Fine-tunes a model whose SH coefficients are rows of a shared table (no counterpart in the
+    reference): every step expands `sh_table` into the Gaussians' coefficients (table_lookup), renders
+    and back-propagates as Trainer does, sums the SH gradients of the filtered Gaussians into the
+    table's rows (table_gradient), and takes an Adam step on the table and on the Gaussians' geometry.
+    The set of Gaussians and their rows stay as they are: no densification, opacity reset or SH-degree
+    increase. `sh_table.coeffs` (float32, SH storage degree of `gaussians`) is updated in place;
+    `gaussians.sh_coeffs` is overwritten at every step."""
+
+    def __init__(self, gaussians: GaussiansVector, sh_table, cameras: list[PinholeCamera], targets,
+                 render_options: RenderOptions, tiling: Tiling, options: TrainingOptions, **kwargs):
+        coeffs = sh_table.coeffs
+        if coeffs.dtype != torch.float32 or not coeffs.is_contiguous() or coeffs.device != gaussians.device:
+            raise ValueError("the table's coefficients must be contiguous float32 on the Gaussians' device")
+        if coeffs.shape[1:] != gaussians.sh_coeffs.shape[1:] or sh_table.indices.shape[0] != gaussians.n:
+            raise ValueError(f"a table of {tuple(coeffs.shape)} with {sh_table.indices.shape[0]} indices for "
+                             f"SH coefficients of {tuple(gaussians.sh_coeffs.shape)}")
+        super().__init__(gaussians, cameras, targets, render_options, tiling, options,
+                         rebuild_sh_grads=False, **kwargs)
+        self.sh_table = sh_table
+        dev, n, rows = self.device, gaussians.n, sh_table.rows
+        # the geometry's optimizer: the Gaussians without coefficients (SH degree 0, zero gradients)
+        bare = torch.zeros((n, 3, 1), dtype=torch.float32, device=dev)
+        self.optimizer = AdamOptimizer(GaussiansVector(*gaussians.tensors()[:3], bare),
+                                       options.learning_rates())
+        self._geometry_gradients = FilteredGaussiansGradients(
+            **{**self.fgradients.__dict__, "sh_coeffs_grads": torch.zeros_like(bare)})
+        # the table's: as many Gaussians as it has rows, without geometry gradients, all of them updated
+        zeros = lambda k: torch.zeros((rows, k), dtype=torch.float32, device=dev)  # noqa: E731
+        self.table_optimizer = AdamOptimizer(GaussiansVector(zeros(4), zeros(3), zeros(4), coeffs),
+                                             options.learning_rates())
+        self._table_gradients = FilteredGaussiansGradients.create(rows, gaussians.sh_degree, dev)
+        self._table_rows = torch.arange(1, rows + 1, dtype=torch.int32, device=dev)
+        self._table_counts = torch.tensor([rows, 0, 0, 0], dtype=torch.int32, device=dev)
+
+    def maybe_increase_sh_degree(self) -> None:
+        pass
+
+    def maybe_opacity_reset(self) -> None:
+        pass
+
+    def densifies_this_iteration(self) -> bool:
+        return False
+
+    def maybe_densify_and_prune(self) -> bool:
+        return False
+
+    def prepare_model(self) -> None:
+        self.sh_table.expand(out=self.gaussians.sh_coeffs)
+
+    def update_model(self, cam: PinholeCamera, rebuild: bool) -> None:
+        rb = self.render_buffers
+        self.optimizer.update(self._geometry_gradients, rb.fgidx_to_gidx, rb.device_counts, 0)
+        self.sh_table.gradient(self.fgradients, rb,
+                               out=self._table_gradients.sh_coeffs_grads[:self.sh_table.rows])
+        self.table_optimizer.update(self._table_gradients, self._table_rows, self._table_counts,
+                                    self.render_options.sh_degree)

@@ -276,7 +276,7 @@ __device__ __forceinline__ int64_t block_exclusive_scan64(int64_t v, int64_t* sm
     return inc - v + (w ? sm[w - 1] : 0);
 }
 
-__global__ void __launch_bounds__(kSortThreads, 3) k_radix_scatter(const SortPass p) {
+__global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPass p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int64_t sm[kSortWarps];
     constexpr int BINS = (1 << kMaxDigitBits) / kSortThreads;  // of a thread, at most
@@ -307,24 +307,30 @@ __global__ void __launch_bounds__(kSortThreads, 3) k_radix_scatter(const SortPas
     }
     for (int i = threadIdx.x; i < nbins * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(wcount)[i] = 0;
     __syncthreads();
-    // stable rank of every key among its warp's keys of the same digit: first within its 32 (all matches
-    // in flight together), then behind the 32s before
+    // stable rank of every key among its warp's keys of the same digit: first within its 32, then behind the 32s
+    // before
     int rank[kSortRounds];
     const unsigned below = (1u << lane) - 1u;
+    unsigned peers[kSortRounds];  // lanes with the same digit, bit by bit
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-        const int d = item[r].x >= 0 ? (item[r].x >> p.shift) & (nbins - 1) : nbins;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        rank[r] = __popc(peers & below) | __popc(peers) << 8;
-    }
+    for (int r = 0; r < kSortRounds; ++r) peers[r] = __ballot_sync(0xffffffffu, item[r].x >= 0);
+    for (int b = p.shift; b < p.shift + p.bits; ++b)
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) {
+            const bool bit = (item[r].x >> b) & 1;
+            const unsigned ones = __ballot_sync(0xffffffffu, bit);
+            peers[r] &= bit ? ones : ~ones;
+        }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) rank[r] = __popc(peers[r] & below) | __popc(peers[r]) << 8;
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
         const bool on = item[r].x >= 0;
         uint16_t& c = wcount[w * nbins + (on ? (item[r].x >> p.shift) & (nbins - 1) : 0)];
-        const int before = c, mine = rank[r] & 255, peers = rank[r] >> 8;
+        const int before = c, mine = rank[r] & 255, all = rank[r] >> 8;
         rank[r] = before + mine;
         __syncwarp();
-        if (on && mine == 0) c = (uint16_t)(before + peers);
+        if (on && mine == 0) c = (uint16_t)(before + all);
         __syncwarp();
     }
     __syncthreads();

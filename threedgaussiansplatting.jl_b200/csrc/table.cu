@@ -3,6 +3,7 @@
 //   gs3d_table_gradient  table_grads[k] = scale * sum of grads[f] over the rows f with index k + 1,
 //                        by the rows sorted by index (stable), so the order of every sum is fixed
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 #include "internal.h"
@@ -137,6 +138,32 @@ int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, c
 // The order of every sum follows from the sorted order alone, whatever the number of rows that share
 // an index: no atomics, and a row that half of the Gaussians use is spread over the GPU like any other.
 
+// The kernels of one call follow one another with programmatic dependent launch: each starts while
+// the one before it ends, and waits in `after_predecessor` (every thread, before anything else, so
+// that the chain holds for all kernels before) until that one's writes are there. What a predecessor
+// wrote is read with ordinary loads or through L2, not as read-only data.
+__device__ __forceinline__ void after_predecessor() {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+int launch_after(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                 A&&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    GS3D_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...), what);
+    return GS3D_OK;
+}
+
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortTile = 4096;
@@ -210,6 +237,7 @@ __device__ __forceinline__ int tile_place(int tile) {
 __global__ void __launch_bounds__(kSortThreads) k_radix_count(const SortPass p, const KeySource src,
                                                               const ZeroRows zero) {
     __shared__ int bins[1 << kMaxDigitBits];
+    after_predecessor();
     const int nbins = 1 << p.bits, tile = blockIdx.x, place = tile_place(tile);
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) bins[b] = 0;
     int key[kSortRounds];
@@ -237,6 +265,7 @@ constexpr int kSpineThreads = 256;
 // Block b: exclusive scan of bin b's counts over the tiles.
 __global__ void __launch_bounds__(kSpineThreads) k_radix_spine(const SortPass p) {
     __shared__ int sm[33];
+    after_predecessor();
     int32_t* row = p.hist + (int64_t)blockIdx.x * p.ntiles;
     int carry = 0, tot;
     for (int t0 = 0; t0 < p.ntiles; t0 += kSpineThreads) {
@@ -280,6 +309,7 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPas
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int64_t sm[kSortWarps];
     constexpr int BINS = (1 << kMaxDigitBits) / kSortThreads;  // of a thread, at most
+    after_predecessor();
     const int nbins = 1 << p.bits, tile = blockIdx.x;
     int2* items = reinterpret_cast<int2*>(smem);                   // the tile in digit order
     int32_t* dest = reinterpret_cast<int32_t*>(items + kSortTile);  // a bin's place in the output, minus in the tile
@@ -386,6 +416,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource sr
     __shared__ int keys[kSortTile], vals[kSortTile];
     __shared__ uint16_t wcount[kSmallWarps][256];
     __shared__ int start[256], sm[33];
+    after_predecessor();
     if (gridDim.x > 1 && blockIdx.x > 0) {
         zero.fill((int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
         return;
@@ -494,7 +525,7 @@ __device__ __forceinline__ void store_row(const Segments& g, int key, int col, c
 }
 
 template <typename T, int VB>
-__global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const T* __restrict__ grads, int stride, int dim,
+__global__ void __launch_bounds__(256, 5) k_table_segments(const T* __restrict__ grads, int stride, int dim,
                                                         const SegmentPlan pl, const Segments g) {
     using Unit = RowUnit<T, VB>;
     constexpr int N = Unit::N, AHEAD = VB == 16 ? 4 : 8;  // rows in flight a slot
@@ -502,6 +533,7 @@ __global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const 
     int2* items = reinterpret_cast<int2*>(smem);                  // the chunk's
     int32_t* pkey = reinterpret_cast<int32_t*>(items + pl.chunk);  // [slot][2]: the slots' first and last runs
     float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);  // [slot][2][tile_units * N]
+    after_predecessor();
     const int m = *g.valid;
     const int begin = blockIdx.x * pl.chunk, count = min(pl.chunk, m - begin);
     const bool meta = threadIdx.x == 0 && blockIdx.y == 0;
@@ -509,7 +541,7 @@ __global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const 
         if (meta) g.first_key[blockIdx.x] = g.owned[blockIdx.x] = -1;
         return;
     }
-    for (int i = threadIdx.x; i < count; i += blockDim.x) items[i] = __ldg(g.items + begin + i);
+    for (int i = threadIdx.x; i < count; i += blockDim.x) items[i] = __ldcg(g.items + begin + i);
     __syncthreads();
     const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
     const int unit = blockIdx.y * pl.tile_units + lane;
@@ -527,15 +559,9 @@ __global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const 
         const T* gc = grads + (on ? col : 0);
         for (; j < j1; j += AHEAD) {
             Unit u[AHEAD];
-            int key[AHEAD];
 #pragma unroll
-            for (int q = 0; q < AHEAD; ++q) {
-                const int2 it = items[min(j + q, j1 - 1)];
-                key[q] = it.x;
-                u[q].load(gc + (int64_t)it.y * stride);
-            }
-            const bool whole = j + AHEAD <= j1;
-            if (whole && key[AHEAD - 1] == cur) {  // sorted: all of them are
+            for (int q = 0; q < AHEAD; ++q) u[q].load(gc + (int64_t)items[min(j + q, j1 - 1)].y * stride);
+            if (j + AHEAD <= j1 && items[j + AHEAD - 1].x == cur) {  // sorted: all of them are
 #pragma unroll
                 for (int q = 0; q < AHEAD; ++q)
 #pragma unroll
@@ -545,7 +571,8 @@ __global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const 
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) {
                 if (j + q >= j1) break;
-                if (key[q] != cur) {
+                const int key = items[j + q].x;
+                if (key != cur) {
                     if (first) {
 #pragma unroll
                         for (int i = 0; i < N; ++i) part[(2 * slot) * width + lane * N + i] = acc[i];
@@ -554,7 +581,7 @@ __global__ void __launch_bounds__(256, VB == 16 ? 5 : 4) k_table_segments(const 
                     } else if (on) {
                         store_row<N>(g, cur, col, acc);
                     }
-                    cur = key[q];
+                    cur = key;
 #pragma unroll
                     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
                 }
@@ -624,6 +651,7 @@ constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kJoinWarps) k_table_join(int dim, int nchunks, const Segments g) {
     __shared__ int long_run[kJoinWarps];
     __shared__ float part[32 * kJoinWarps];
+    after_predecessor();
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int b = blockIdx.x * kJoinWarps + w;
     const int k = b < nchunks ? g.owned[b] : -1;
@@ -803,12 +831,15 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
             p.shift = i * digit;
             p.bits = digit;
             p.out = items(i & 1);
-            k_radix_count<<<L.ntiles, kSortThreads, 0, stream>>>(p, src, zero);
-            GS3D_LAUNCHED("k_radix_count");
-            k_radix_spine<<<1 << digit, kSpineThreads, 0, stream>>>(p);
-            GS3D_LAUNCHED("k_radix_spine");
-            k_radix_scatter<<<L.ntiles, kSortThreads, smem, stream>>>(p);
-            GS3D_LAUNCHED("k_radix_scatter");
+            if (i == 0) {  // behind whatever wrote the inputs
+                k_radix_count<<<L.ntiles, kSortThreads, 0, stream>>>(p, src, zero);
+                GS3D_LAUNCHED("k_radix_count");
+            } else {
+                GS3D_RETURN_IF(launch_after("k_radix_count", k_radix_count, dim3(L.ntiles), kSortThreads, 0, stream, p,
+                                            src, zero));
+            }
+            GS3D_RETURN_IF(launch_after("k_radix_spine", k_radix_spine, dim3(1 << digit), kSpineThreads, 0, stream, p));
+            GS3D_RETURN_IF(launch_after("k_radix_scatter", k_radix_scatter, dim3(L.ntiles), kSortThreads, smem, stream, p));
             p.in = p.out;
             sorted = i & 1;
         }
@@ -828,12 +859,11 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
         const dim3 grid(pl.nchunks, (unsigned)ceil_div(pl.units, pl.tile_units));
         const int threads = pl.slots * pl.tile_units;
         const int stride = (int)grads->row_stride;
-        if (wide) k_table_segments<T, 16><<<grid, threads, smem, stream>>>(g, stride, grads->dim, pl, seg);
-        else k_table_segments<T, (int)sizeof(T)><<<grid, threads, smem, stream>>>(g, stride, grads->dim, pl, seg);
-        GS3D_LAUNCHED("k_table_segments");
-        k_table_join<<<dim3((unsigned)ceil_div(pl.nchunks, kJoinWarps), (unsigned)ceil_div(grads->dim, 256)),
-                       32 * kJoinWarps, 0, stream>>>(grads->dim, pl.nchunks, seg);
-        GS3D_LAUNCHED("k_table_join");
+        const auto kernel = wide ? k_table_segments<T, 16> : k_table_segments<T, (int)sizeof(T)>;
+        GS3D_RETURN_IF(launch_after("k_table_segments", kernel, grid, threads, smem, stream, g, stride, grads->dim, pl, seg));
+        GS3D_RETURN_IF(launch_after("k_table_join", k_table_join,
+                                    dim3((unsigned)ceil_div(pl.nchunks, kJoinWarps), (unsigned)ceil_div(grads->dim, 256)),
+                                    32 * kJoinWarps, 0, stream, (int)grads->dim, pl.nchunks, seg));
         return GS3D_OK;
     });
 }

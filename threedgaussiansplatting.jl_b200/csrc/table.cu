@@ -127,7 +127,7 @@ int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, c
 // ---- gradient --------------------------------------------------------------------------------
 // 1. Stable sort of the rows by table row (radix_*: 4096-row tiles, digits of up to 10 bits, three
 //    launches a pass, one pass per 10 bits of the row number; up to 4096 rows: one block sorts them in
-//    shared memory). Rows without a valid index drop out of the first pass, which also zeroes
+//    shared memory; up to 1024: k_table_gradient_tiny does everything). Rows without a valid index drop out of the first pass, which also zeroes
 //    the table's gradients.
 // 2. k_table_segments: the sorted rows are cut into chunks of equal length, a block each, and a chunk
 //    into one run of rows per slot (a slot: the threads side by side on a row's columns). A slot adds
@@ -405,40 +405,33 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPas
     }
 }
 
-// Up to kSortTile rows: block 0 sorts them in shared memory, 8 bits a pass; the others zero the table.
-constexpr int kSmallThreads = 512;
-constexpr int kSmallWarps = kSmallThreads / 32;
-constexpr int kSmallRounds = kSortTile / kSmallThreads;
-
-__global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource src, const ZeroRows zero, int bits,
-                                                              int2* __restrict__ out,
-                                                              int32_t* __restrict__ valid) {
-    __shared__ int keys[kSortTile], vals[kSortTile];
-    __shared__ uint16_t wcount[kSmallWarps][256];
-    __shared__ int start[256], sm[33];
-    after_predecessor();
-    if (gridDim.x > 1 && blockIdx.x > 0) {
-        zero.fill((int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
-        return;
-    }
+// The rows with a valid index among the first THREADS * ROUNDS, sorted by one block in shared memory,
+// 8 bits a pass; returns their number.
+template <int THREADS, int ROUNDS>
+__device__ __forceinline__ int sort_rows(const KeySource& src, int bits, int2* items, uint16_t (*wcount)[256],
+                                         int* start, int* sm) {
+    constexpr int WARPS = THREADS / 32;
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned below = (1u << lane) - 1u;
+    const int place = w * (ROUNDS * 32) + lane;
     int count = 0;
     for (int shift = 0; shift < max(bits, 1); shift += 8) {
-        const bool first = shift == 0;
-        int key[kSmallRounds], val[kSmallRounds], rank[kSmallRounds];
-        const int place = w * (kSmallRounds * 32) + lane;
-        if (first) src.keys(place, key);
+        int key[ROUNDS], row[ROUNDS], rank[ROUNDS];
+        if (shift == 0) src.keys(place, key);
 #pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r) {
+        for (int r = 0; r < ROUNDS; ++r) {
             const int i = place + 32 * r;
-            if (first) val[r] = i;
-            else key[r] = i < count ? keys[i] : -1, val[r] = vals[i];
+            row[r] = i;
+            if (shift) {
+                const int2 it = items[i];
+                key[r] = i < count ? it.x : -1;
+                row[r] = it.y;
+            }
         }
-        for (int i = threadIdx.x; i < kSmallWarps * 256; i += kSmallThreads) (&wcount[0][0])[i] = 0;
+        for (int i = threadIdx.x; i < WARPS * 256; i += THREADS) (&wcount[0][0])[i] = 0;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r) {
+        for (int r = 0; r < ROUNDS; ++r) {
             const int d = key[r] >= 0 ? (key[r] >> shift) & 255 : 256;
             const unsigned peers = __match_any_sync(0xffffffffu, d);
             const int before = d < 256 ? wcount[w][d] : 0;
@@ -451,29 +444,42 @@ __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource sr
         int run = 0;
         if (threadIdx.x < 256)
 #pragma unroll
-            for (int ww = 0; ww < kSmallWarps; ++ww) {
+            for (int ww = 0; ww < WARPS; ++ww) {
                 const int c = wcount[ww][threadIdx.x];
                 wcount[ww][threadIdx.x] = (uint16_t)run;
                 run += c;
             }
-        int tot;
-        const int st = block_exclusive_scan(run, sm, &tot);
+        const int st = block_exclusive_scan(run, sm, &count);
         if (threadIdx.x < 256) start[threadIdx.x] = st;
-        count = tot;
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSmallRounds; ++r)
+        for (int r = 0; r < ROUNDS; ++r)
             if (key[r] >= 0) {
                 const int d = (key[r] >> shift) & 255;
-                const int at = start[d] + wcount[w][d] + rank[r];
-                keys[at] = key[r];
-                vals[at] = val[r];
+                items[start[d] + wcount[w][d] + rank[r]] = make_int2(key[r], row[r]);
             }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < count; i += kSmallThreads) out[i] = make_int2(keys[i], vals[i]);
+    return count;
+}
+
+// Up to kSortTile rows: block 0 sorts them; the others zero the table.
+constexpr int kSmallThreads = 512;
+
+__global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource src, const ZeroRows zero, int bits,
+                                                              int2* __restrict__ out,
+                                                              int32_t* __restrict__ valid) {
+    __shared__ int2 items[kSortTile];
+    __shared__ uint16_t wcount[kSmallThreads / 32][256];
+    __shared__ int start[256], sm[33];
+    after_predecessor();
+    if (gridDim.x > 1 && blockIdx.x > 0) {
+        zero.fill((int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
+        return;
+    }
+    const int count = sort_rows<kSmallThreads, kSortTile / kSmallThreads>(src, bits, items, wcount, start, sm);
+    for (int i = threadIdx.x; i < count; i += kSmallThreads) out[i] = items[i];
     if (threadIdx.x == 0) *valid = count;
-    if (gridDim.x == 1) zero.fill(threadIdx.x, kSmallThreads);
 }
 
 // VB bytes of a row as VB / sizeof(T) floats.
@@ -524,33 +530,25 @@ __device__ __forceinline__ void store_row(const Segments& g, int key, int col, c
     }
 }
 
+// The sums of one chunk: `count` items in shared memory, cut into runs of `run` for the slots; every
+// thread of the block calls it (those with slot >= pl.slots only wait). open_left / open_right: the first
+// / last run goes on in the chunk before / behind, and its sum goes to partial[0 ..] / partial[dim ..]
+// (`earlier`: the whole chunk is one run that began before it, its sum at partial[0 ..]).
 template <typename T, int VB>
-__global__ void __launch_bounds__(256, 5) k_table_segments(const T* __restrict__ grads, int stride, int dim,
-                                                        const SegmentPlan pl, const Segments g) {
+__device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int stride, int dim, const SegmentPlan& pl,
+                                          int run, const Segments& g, const int2* items, int count, int32_t* pkey,
+                                          float* part, bool open_left, bool open_right, bool earlier,
+                                          float* __restrict__ partial) {
     using Unit = RowUnit<T, VB>;
-    constexpr int N = Unit::N, AHEAD = VB == 16 ? 4 : 8;  // rows in flight a slot
-    extern __shared__ __align__(16) unsigned char smem[];
-    int2* items = reinterpret_cast<int2*>(smem);                  // the chunk's
-    int32_t* pkey = reinterpret_cast<int32_t*>(items + pl.chunk);  // [slot][2]: the slots' first and last runs
-    float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);  // [slot][2][tile_units * N]
-    after_predecessor();
-    const int m = *g.valid;
-    const int begin = blockIdx.x * pl.chunk, count = min(pl.chunk, m - begin);
-    const bool meta = threadIdx.x == 0 && blockIdx.y == 0;
-    if (count <= 0) {
-        if (meta) g.first_key[blockIdx.x] = g.owned[blockIdx.x] = -1;
-        return;
-    }
-    for (int i = threadIdx.x; i < count; i += blockDim.x) items[i] = __ldcg(g.items + begin + i);
-    __syncthreads();
+    constexpr int N = Unit::N, AHEAD = VB == 16 ? 6 : 8;  // rows in flight a slot
     const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
     const int unit = blockIdx.y * pl.tile_units + lane;
     const int col = unit * N;
     const bool on = unit < pl.units;
     const int width = pl.tile_units * N;
-    {
-        const int j1 = min((slot + 1) * pl.run, count);
-        int j = slot * pl.run;
+    if (slot < pl.slots) {
+        const int j1 = min((slot + 1) * run, count);
+        int j = slot * run;
         int cur = j < j1 ? items[j].x : -1;
         bool first = true;
         float acc[N];
@@ -600,15 +598,11 @@ __global__ void __launch_bounds__(256, 5) k_table_segments(const T* __restrict__
     __syncthreads();
     if (slot != 0) return;
     // the slots' open runs in order
-    const bool open_left = begin > 0 && g.items[begin - 1].x == items[0].x;
-    const int last = items[count - 1].x;
-    const bool open_right = begin + count < m && g.items[begin + count].x == last;
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
     int cur = items[0].x;
     bool first = true;
-    float* partial = g.partial + (int64_t)blockIdx.x * 2 * dim + col;
     for (int e = 0; e < 2 * pl.slots; ++e) {
         const int k = pkey[e];
         if (k < 0) continue;
@@ -616,7 +610,7 @@ __global__ void __launch_bounds__(256, 5) k_table_segments(const T* __restrict__
             if (on) {
                 if (first && open_left) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) partial[i] = acc[i];
+                    for (int i = 0; i < N; ++i) partial[col + i] = acc[i];
                 } else {
                     store_row<N>(g, cur, col, acc);
                 }
@@ -629,19 +623,88 @@ __global__ void __launch_bounds__(256, 5) k_table_segments(const T* __restrict__
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] += part[e * width + lane * N + i];
     }
-    const bool earlier = first && open_left;  // the whole chunk goes on from the one before
-    if (on) {
-        if (earlier || open_right) {
+    if (!on) return;
+    if (earlier || open_right) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) partial[(earlier ? 0 : dim) + i] = acc[i];
-        } else {
-            store_row<N>(g, cur, col, acc);
-        }
+        for (int i = 0; i < N; ++i) partial[(earlier ? 0 : dim) + col + i] = acc[i];
+    } else {
+        store_row<N>(g, cur, col, acc);
     }
+}
+
+template <typename T, int VB>
+__global__ void __launch_bounds__(256, VB == 16 ? 4 : 5) k_table_segments(const T* __restrict__ grads, int stride, int dim,
+                                                           const SegmentPlan pl, const Segments g) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    int2* items = reinterpret_cast<int2*>(smem);                   // the chunk's
+    int32_t* pkey = reinterpret_cast<int32_t*>(items + pl.chunk);  // [slot][2]: the slots' first and last runs
+    float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);   // [slot][2][tile_units * N]
+    after_predecessor();
+    const int m = *g.valid;
+    const int begin = blockIdx.x * pl.chunk, count = min(pl.chunk, m - begin);
+    const bool meta = threadIdx.x == 0 && blockIdx.y == 0;
+    if (count <= 0) {
+        if (meta) g.first_key[blockIdx.x] = g.owned[blockIdx.x] = -1;
+        return;
+    }
+    __shared__ int outside[2];  // the keys before and behind the chunk
+    for (int i = threadIdx.x; i < count; i += blockDim.x) items[i] = __ldcg(g.items + begin + i);
+    if (threadIdx.x < 2) {
+        const int at = threadIdx.x ? begin + count : begin - 1;
+        outside[threadIdx.x] = at >= 0 && at < m ? __ldcg(g.items + at).x : -1;
+    }
+    __syncthreads();
+    const int head = items[0].x, last = items[count - 1].x;
+    const bool open_left = outside[0] == head, open_right = outside[1] == last;
+    const bool earlier = open_left && head == last;
     if (meta) {
-        g.first_key[blockIdx.x] = items[0].x;
+        g.first_key[blockIdx.x] = head;
         g.owned[blockIdx.x] = open_right && !earlier ? last : -1;
     }
+    sum_chunk<T, VB>(grads, stride, dim, pl, pl.run, g, items, count, pkey, part, open_left, open_right, earlier,
+                     g.partial + (int64_t)blockIdx.x * 2 * dim);
+}
+
+// Up to kTinyRows rows in one launch: every block sorts all of them in shared memory and takes the runs
+// that start in its share of the sorted rows; nothing crosses a border, so nothing is left to join. It
+// also zeroes, of its share of the table, the rows without gradients.
+constexpr int kTinyRows = 1024, kTinyThreads = 256;
+
+__device__ __forceinline__ int first_above(const int2* items, int n, int key) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (items[mid].x <= key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T, int VB>
+__global__ void __launch_bounds__(kTinyThreads) k_table_gradient_tiny(const T* __restrict__ grads, int stride, int dim,
+                                                                      const SegmentPlan pl, const Segments g,
+                                                                      const KeySource src, const ZeroRows zero,
+                                                                      int bits) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int2 items[kTinyRows];
+    __shared__ uint16_t wcount[kTinyThreads / 32][256];
+    __shared__ int start[256], sm[33];
+    const int count = sort_rows<kTinyThreads, kTinyRows / kTinyThreads>(src, bits, items, wcount, start, sm);
+    const int64_t b = blockIdx.x, blocks = gridDim.x;
+    if (zero.data && blockIdx.y == 0)
+        for (int64_t k = b * zero.rows / blocks + threadIdx.x; k < (b + 1) * zero.rows / blocks; k += kTinyThreads) {
+            const int p = first_above(items, count, (int)k);
+            if (p == 0 || items[p - 1].x != k)
+                for (int c = 0; c < dim; ++c) zero.data[k * zero.stride + c] = 0.0f;
+        }
+    int p0 = (int)(b * count / blocks), p1 = (int)((b + 1) * count / blocks);
+    if (p0 > 0) p0 = first_above(items, count, items[p0 - 1].x);
+    if (p1 > 0) p1 = first_above(items, count, items[p1 - 1].x);
+    if (p1 <= p0) return;
+    int32_t* pkey = reinterpret_cast<int32_t*>(smem);
+    float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);
+    sum_chunk<T, VB>(grads, stride, dim, pl, (p1 - p0 + pl.slots - 1) / pl.slots, g, items + p0, p1 - p0, pkey, part,
+                     false, false, false, nullptr);
 }
 
 // A warp per chunk for the runs of up to 32 partial sums behind the first (nearly all: an average run is
@@ -704,6 +767,10 @@ struct GradLayout {
 };
 
 constexpr int kMinRun = 4, kMaxRun = 48;  // rows a slot adds: enough blocks for few rows, few borders for many
+
+// Rows that can be read 16 bytes at a time.
+template <typename T>
+bool wide_rows(const gs3d_rows* r) { return packs<T>(r, 16 / (int)sizeof(T)); }
 
 int slots_for(int tile_units) { return std::max(1, std::min(32, 256 / tile_units)); }
 
@@ -814,6 +881,25 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     const ZeroRows zero{accumulate ? nullptr : out, table_grads->row_stride, (int32_t)table_grads->rows,
                         table_grads->dim};
     ProfScope prof("table_grad", stream);
+    if (n > 0 && n <= kTinyRows)
+        return dispatch_type(grads->type, [&](auto t) {
+            using T = typename decltype(t)::T;
+            const T* g = static_cast<const T*>(grads->data);
+            const bool wide = wide_rows<T>(grads);
+            const int per = wide ? 16 / (int)sizeof(T) : 1;
+            const SegmentPlan pl = segment_plan(n, grads->dim / per);
+            const Segments seg{nullptr, nullptr, out, table_grads->row_stride, scale, accumulate ? 1 : 0, nullptr,
+                               nullptr, nullptr};
+            const size_t smem = (size_t)pl.slots * 8 + (size_t)pl.slots * 2 * pl.tile_units * per * 4;
+            // a block for 32 rows, or for 64 KB of table to zero
+            const int64_t zeroed = accumulate ? 0 : table_grads->rows * table_grads->dim;
+            const int blocks = (int)std::max<int64_t>(ceil_div(n, 32), std::min<int64_t>(ceil_div(zeroed, 1 << 14), kSMs));
+            const dim3 grid(blocks, (unsigned)ceil_div(pl.units, pl.tile_units));
+            const auto kernel = wide ? k_table_gradient_tiny<T, 16> : k_table_gradient_tiny<T, (int)sizeof(T)>;
+            kernel<<<grid, kTinyThreads, smem, stream>>>(g, (int)grads->row_stride, grads->dim, pl, seg, src, zero, L.bits);
+            GS3D_LAUNCHED("k_table_gradient_tiny");
+            return GS3D_OK;
+        });
     int sorted = 0;
     if (n <= kSortTile) {
         const int64_t words = accumulate ? 0 : table_grads->rows * table_grads->dim;
@@ -850,10 +936,8 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     return dispatch_type(grads->type, [&](auto t) {
         using T = typename decltype(t)::T;
         const T* g = static_cast<const T*>(grads->data);
-        constexpr int N = 16 / (int)sizeof(T);
-        const bool wide = grads->dim % N == 0 && grads->row_stride % N == 0 &&
-                          (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-        const int per = wide ? N : 1;
+        const bool wide = wide_rows<T>(grads);
+        const int per = wide ? 16 / (int)sizeof(T) : 1;
         const SegmentPlan pl = segment_plan(n, grads->dim / per);
         const size_t smem = (size_t)pl.chunk * 8 + (size_t)pl.slots * 8 + (size_t)pl.slots * 2 * pl.tile_units * per * 4;
         const dim3 grid(pl.nchunks, (unsigned)ceil_div(pl.units, pl.tile_units));

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(256) k_mx4_quantise_rows(const T* __restrict__
     const unsigned char* gx = reinterpret_cast<const unsigned char*>(x + r0 * dim);
     uint8_t* gc = codes + r0 * cb;
     unsigned char* sc = smem + ((16 + (size_t)per * dim * sizeof(T) + 15) & ~(size_t)15) + head_of(gc);
-    copy_in(smem, gx, (int64_t)mine * dim * sizeof(T));
+    copy_in(smem, gx, mine * dim * (int)sizeof(T));
     __syncthreads();
     const T* sx = reinterpret_cast<const T*>(smem + head_of(gx));
     const TensorScale t = TensorScale::load<FMT>(tensor_scale);
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) k_mx4_quantise_rows(const T* __restrict__
             if (2 * k < len) o[k] = (unsigned char)(words[k / 4] >> (8 * (k % 4)));
     }
     __syncthreads();
-    copy_out(gc, sc - head_of(gc), (int64_t)mine * cb);
+    copy_out(gc, sc - head_of(gc), mine * cb);
 }
 
 // Rows apart or long: a block a thread, element by element.
@@ -324,6 +324,13 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise_blocks(const uint32_t* _
     }
 }
 
+// A word from shared memory at any byte address (reads up to 3 bytes before it and 7 behind).
+__device__ __forceinline__ uint32_t word_at(const unsigned char* p) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~(uintptr_t)3);
+    return __funnelshift_r(w[0], w[1], 8 * (int)(a & 3));
+}
+
 // Rows of any length, back to back: a CTA takes `per` rows' codes and scales through shared memory, a
 // block of a row a thread, and hands the values back as one range of bytes.
 template <typename T, int FMT>
@@ -340,7 +347,7 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise_rows(const uint8_t* __re
     const uint8_t* gc = codes + r0 * cb;
     unsigned char* go = reinterpret_cast<unsigned char*>(out + r0 * dim);
     unsigned char* so = smem + ((16 + (size_t)per * cb + 15) & ~(size_t)15);
-    copy_in(smem, gc, (int64_t)mine * cb);
+    copy_in(smem, gc, mine * cb);
     __syncthreads();
     const unsigned char* sc = smem + head_of(gc);
     T* sv = reinterpret_cast<T*>(so + head_of(go));
@@ -351,15 +358,20 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise_rows(const uint8_t* __re
         const unsigned char* c = sc + r * cb + b * (BS / 2);
         T* o = sv + r * dim + b * BS;
 #pragma unroll
-        for (int k = 0; k < BS; k += 2)
+        for (int k = 0; k < BS; k += 8)
             if (k < len) {
-                const float2 v = mx4_value(d, e2m1_pair_half(c[k / 2]));
-                o[k] = from_f32<T>(v.x);
-                if (k + 1 < len) o[k + 1] = from_f32<T>(v.y);
+                __half2 e[4];
+                e2m1_word_half(word_at(c + k / 2), e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 v = mx4_value(d, e[j]);
+                    if (k + j < len) o[k + j] = from_f32<T>(v.x);
+                    if (k + j + 4 < len) o[k + j + 4] = from_f32<T>(v.y);
+                }
             }
     }
     __syncthreads();
-    copy_out(go, so, (int64_t)mine * dim * sizeof(T));
+    copy_out(go, so, mine * dim * (int)sizeof(T));
 }
 
 // Rows apart or long: an element a thread.
@@ -426,7 +438,7 @@ int launch_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, cudaStream_t
     } else if (flat && dim * (int)sizeof(T) <= kRowsBytes) {
         const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
         const size_t smem = ((16 + (size_t)per * mx4_code_bytes(dim) + 15) & ~(size_t)15) + 16 +
-                            (size_t)per * dim * sizeof(T) + 16;
+                            (size_t)per * dim * sizeof(T) + 16 + 16;  // and what word_at reads behind the codes
         k_mx4_dequantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), 256, smem, stream>>>(
             x->codes, x->scales, x->tensor_scale, x->rows, dim, per, o);
     } else {

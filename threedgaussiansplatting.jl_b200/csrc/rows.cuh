@@ -50,29 +50,27 @@ inline int check_rows(const gs3d_rows* r, const char* what) {
 
 // `bytes` bytes between global and shared memory, 16 at a time where both sides allow it: the shared
 // side's first byte is head_of(global side) bytes behind `sh`, which is 16-byte aligned, so that the
-// borders of both coincide.
+// borders of both coincide. Blocks of 16 threads or more.
 __device__ __forceinline__ int head_of(const void* p) { return (int)(reinterpret_cast<uintptr_t>(p) & 15); }
 
-__device__ __forceinline__ void copy_in(unsigned char* sh, const unsigned char* gl, int64_t bytes) {
-    const int h = head_of(gl);
-    const int64_t end = h + bytes;
+__device__ __forceinline__ void copy_in(unsigned char* sh, const unsigned char* gl, int bytes) {
+    const int h = head_of(gl), end = h + bytes, first = h ? 16 : 0, last = max(end & ~15, first);
     const unsigned char* g0 = gl - h;
-    const int64_t first = h ? 16 : 0, last = end & ~(int64_t)15;
-    for (int64_t i = h + threadIdx.x; i < min(first, end); i += blockDim.x) sh[i] = g0[i];
-    for (int64_t i = first + 16 * (int64_t)threadIdx.x; i < last; i += 16 * (int64_t)blockDim.x)
+    const int t = threadIdx.x;
+    if (t >= h && t < min(first, end)) sh[t] = __ldg(g0 + t);
+    for (int i = first + 16 * t; i < last; i += 16 * blockDim.x)
         *reinterpret_cast<uint4*>(sh + i) = __ldg(reinterpret_cast<const uint4*>(g0 + i));
-    for (int64_t i = max(first, last) + threadIdx.x; i < end; i += blockDim.x) sh[i] = g0[i];
+    if (last + t < end) sh[last + t] = __ldg(g0 + last + t);
 }
 
-__device__ __forceinline__ void copy_out(unsigned char* gl, const unsigned char* sh, int64_t bytes) {
-    const int h = head_of(gl);
-    const int64_t end = h + bytes;
+__device__ __forceinline__ void copy_out(unsigned char* gl, const unsigned char* sh, int bytes) {
+    const int h = head_of(gl), end = h + bytes, first = h ? 16 : 0, last = max(end & ~15, first);
     unsigned char* g0 = gl - h;
-    const int64_t first = h ? 16 : 0, last = end & ~(int64_t)15;
-    for (int64_t i = h + threadIdx.x; i < min(first, end); i += blockDim.x) g0[i] = sh[i];
-    for (int64_t i = first + 16 * (int64_t)threadIdx.x; i < last; i += 16 * (int64_t)blockDim.x)
+    const int t = threadIdx.x;
+    if (t >= h && t < min(first, end)) g0[t] = sh[t];
+    for (int i = first + 16 * t; i < last; i += 16 * blockDim.x)
         __stcs(reinterpret_cast<uint4*>(g0 + i), *reinterpret_cast<const uint4*>(sh + i));
-    for (int64_t i = max(first, last) + threadIdx.x; i < end; i += blockDim.x) g0[i] = sh[i];
+    if (last + t < end) g0[last + t] = sh[last + t];
 }
 
 constexpr int kRowsBytes = 16 << 10;  // the most that a CTA's rows take in shared memory

@@ -128,6 +128,35 @@ def test_gradient(cuda, n, rows, dim, skew, kind):
     assert ((got.cpu().double() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 4095, 4096, 4097, 8193])
+@pytest.mark.parametrize("rows", [1, 2, 256, 257, 1024, 1025, 70_000, (1 << 20) + 1])
+def test_gradient_sizes_where_the_sort_changes(cuda, n, rows):
+    """One launch up to 1024 rows, one sorting block up to 4096, then tiles of 4096; digits of 8 and 10
+    bits, one to three passes."""
+    gen = rng(n + rows)
+    grads = torch.randn(n, 4, generator=gen)
+    idx = make_indices(n, rows, gen)
+    got = gc.table_gradient(grads.to(cuda), idx.to(cuda), rows)
+    want, bound = gradient_exact(grads, idx, rows, 1.0)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [5, 1000, 3000, 60_000])
+@pytest.mark.parametrize("dim", [3, 48])
+def test_gradient_of_one_row_used_by_all(cuda, n, dim):
+    """Every row of the gradients has the same index: one run over all slots, chunks and blocks."""
+    grads = torch.randn(n, dim, generator=rng(n))
+    idx = torch.full((n,), 7, dtype=torch.int32)
+    out = torch.full((9, dim), 2.0, device=cuda)
+    got = gc.table_gradient(grads.to(cuda), idx.to(cuda), 9)
+    gc.table_gradient(grads.to(cuda), idx.to(cuda), 9, out=out, accumulate=True)
+    want, bound = gradient_exact(grads, idx, 9, 1.0)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+    # the accumulation rounds once more
+    assert ((out.cpu().double() - 2.0 - want).abs() <= bound + 2 * U * (2.0 + want.abs())).all()
+    assert (out[torch.arange(9) != 6] == 2.0).all()
+
+
 @pytest.mark.parametrize("n,rows,dim,skew", [(1000, 64, 48, 0.0), (20_003, 70_000, 48, 0.0), (50_001, 1000, 27, 2.0)])
 def test_gradient_repeats_bit_for_bit(cuda, n, rows, dim, skew):
     gen = rng(2)
@@ -563,6 +592,38 @@ def test_given_colours_render(cuda):
     buf = RenderBuffers.create(g.n, til.nb_tiles, cuda)
     gs3d.render(b, plain, cam, til, opt, buf)
     assert float((a.rgb - b.rgb).abs().max()) <= pixel_bound(plain.sh_coeffs, buf)
+
+
+# -- offsets past 32 bits ---------------------------------------------------------------------------
+def test_more_than_2_31_elements(cuda):
+    """46M rows of 48 (2.2e9 elements, 4.4 GB in bf16): the rows at the end, whose element offsets do not
+    fit 31 bits, and 90M rows of 24 bytes of codes (2.1 GB). Products and sums of small whole numbers, exact."""
+    n, rows = 46_000_000, 100
+    table = (torch.arange(rows, device=cuda) % 64)[:, None].float().expand(rows, 48).contiguous().bfloat16()
+    idx = (torch.arange(n, device=cuda, dtype=torch.int32) % rows) + 1
+    out = gc.table_lookup(table, idx)
+    tail = (torch.arange(n - 3000, n, device=cuda) % rows) % 64
+    assert torch.equal(out[n - 3000:], tail[:, None].bfloat16().expand(-1, 48))
+    # only the last rows have an index: sums of values below 64 over 460 rows are exact
+    keep = torch.zeros_like(idx)
+    keep[n - rows * 460:] = idx[n - rows * 460:]
+    grad = gc.table_gradient(out, keep, rows)
+    assert torch.equal(grad, table.float() * 460)
+    q = gc.mx4_quantise(out, "mxfp4")
+    back = gc.mx4_dequantise(q, torch.bfloat16)
+    few = gc.mx4_dequantise(gc.mx4_quantise(out[n - 3000:].contiguous(), "mxfp4"), torch.bfloat16)
+    assert torch.equal(back[n - 3000:], few)
+    del out, back, q
+    m = 90_000_000
+    sh = MX4Rows(torch.zeros(m, 24, dtype=torch.uint8, device=cuda), torch.zeros(m, 2, dtype=torch.uint8, device=cuda),
+                 None, 48, "mxfp4")
+    sh.codes[m - 1000:] = 0x22
+    sh.scales[m - 1000:] = 127
+    means = torch.randn(1000, 4, generator=rng(1)).to(cuda)
+    pos = np.ones((1, 3), np.float32)
+    last = torch.arange(m - 999, m + 1, dtype=torch.int32, device=cuda)
+    small = MX4Rows(sh.codes[m - 1000:].clone(), sh.scales[m - 1000:].clone(), None, 48, "mxfp4")
+    assert torch.equal(gc.mx4_colours(sh, means, pos, 3, indices=last), gc.mx4_colours(small, means, pos, 3))
 
 
 # -- a run of them, streams and graphs -------------------------------------------------------------

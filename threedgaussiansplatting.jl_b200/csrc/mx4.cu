@@ -626,7 +626,7 @@ struct Positions {
 // their operations in packed pairs. ONE: a single view; else `views` of them a block, with the elements
 // decoded once.
 template <int DEG, int FMT, bool WHOLE, bool ONE>
-__global__ void __launch_bounds__(128) k_mx4_colours(const Mx4Sh a, int order, const float4* __restrict__ mo4,
+__global__ void __launch_bounds__(128, ONE && WHOLE ? 7 : (DEG == 3 ? 3 : 5)) k_mx4_colours(const Mx4Sh a, int order, const float4* __restrict__ mo4,
                                                      int n, const Positions cv, int nv, int views,
                                                      float4* __restrict__ out, int64_t view_stride) {
     constexpr int NC = (DEG + 1) * (DEG + 1);

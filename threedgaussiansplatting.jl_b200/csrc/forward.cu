@@ -10,6 +10,7 @@
 // F and D never leave the device unless the caller asks for them.
 #include "common.cuh"
 #include "internal.h"
+#include "mx4_colour.cuh"
 #include "sh_colour.cuh"
 
 namespace gs3d {
@@ -168,12 +169,15 @@ __device__ __forceinline__ float3 gaussian_colour(const ProjectArgs& a, const gs
     return colour_from_sh<DEG>(hc, cam.position, mx0, my0, mz0);
 }
 
-// RO: render-only input (stored opacity and 3D covariance). COL: also the colour (else left
-// for k_project_colour).
-template <int DEG, bool RO, bool COL = true>
+// What k_project does for the colour: nothing (left for k_project_colour), from the SH coefficients, or
+// from 4-bit SH rows.
+enum ProjectColour { kNoColour, kShColour, kNvfp4Colour, kNvfp4ColourWhole, kMxfp4Colour, kMxfp4ColourWhole };
+
+// RO: render-only input (stored opacity and 3D covariance).
+template <int DEG, bool RO, ProjectColour COL = kShColour>
 __global__ void __launch_bounds__(256, GS3D_PROJECT_MINB) k_project(const ProjectArgs a, const gs3d_camera cam,
                                                  const gs3d_tiling til,
-                                                 const gs3d_render_options opt) {
+                                                 const gs3d_render_options opt, const Mx4Sh mx4) {
     const int F = a.counts[0];
     for (int f = blockIdx.x * blockDim.x + threadIdx.x; f < F; f += gridDim.x * blockDim.x) {
         const int gi = a.f2g[f] - 1;
@@ -260,13 +264,22 @@ __global__ void __launch_bounds__(256, GS3D_PROJECT_MINB) k_project(const Projec
             empty = left > right || top > bottom;
         }
         float3 col = make_float3(0.0f, 0.0f, 0.0f);
-        if (COL) col = gaussian_colour<DEG>(a, cam, gi, mo.x, mo.y, mo.z);
+        if constexpr (COL == kShColour) col = gaussian_colour<DEG>(a, cam, gi, mo.x, mo.y, mo.z);
+        if constexpr (COL >= kNvfp4Colour) {
+            constexpr int FMT = COL >= kMxfp4Colour ? GS3D_MXFP4 : GS3D_NVFP4;
+            constexpr bool WHOLE = COL == kNvfp4ColourWhole || COL == kMxfp4ColourWhole;
+            const int64_t r[1] = {sh_row(mx4, gi)};
+            float c[3];
+            mx4_colour<float, DEG, FMT, WHOLE>(mx4, a.sh_stride, r, FMT == GS3D_NVFP4 ? __ldg(mx4.tensor_scale) : 1.0f,
+                                               cam.position, mo.x, mo.y, mo.z, c);
+            col = make_float3(c[0], c[1], c[2]);
+        }
 
         a.depths[f] = depth;
         float* rr = a.f2d + 9 * (size_t)f;
         rr[0] = mx; rr[1] = my; rr[2] = opacity;
         rr[3] = c22 * icov_det; rr[4] = -c21 * icov_det; rr[5] = c11 * icov_det;
-        if (COL) { rr[6] = col.x; rr[7] = col.y; rr[8] = col.z; }
+        if (COL != kNoColour) { rr[6] = col.x; rr[7] = col.y; rr[8] = col.z; }
         int4 rect;
         int count;
         if (empty) {
@@ -445,6 +458,34 @@ int check_common(const gs3d_gaussians* g, const gs3d_camera* cam, const gs3d_til
     return GS3D_OK;
 }
 
+// k_project for render-only input with 4-bit SH rows (checked: check_mx4_sh). The colour in the same
+// kernel: its 12 bytes of a 36-byte record written on their own cost 66 us at 3M Gaussians.
+template <int DEG>
+void launch_project_mx4_degree(int grid, cudaStream_t stream, const ProjectArgs& pa, const gs3d_camera& cam,
+                                      const gs3d_tiling& til, const gs3d_render_options& opt,
+                                      const gs3d_mx4_rows* sh, const int32_t* indices) {
+    const Mx4Sh mx4 = mx4_sh_source(sh, indices);
+    const bool whole = mx4_sh_whole(sh, DEG);
+    if (sh->format == GS3D_NVFP4) {
+        if (whole) k_project<DEG, true, kNvfp4ColourWhole><<<grid, 256, 0, stream>>>(pa, cam, til, opt, mx4);
+        else k_project<DEG, true, kNvfp4Colour><<<grid, 256, 0, stream>>>(pa, cam, til, opt, mx4);
+    } else {
+        if (whole) k_project<DEG, true, kMxfp4ColourWhole><<<grid, 256, 0, stream>>>(pa, cam, til, opt, mx4);
+        else k_project<DEG, true, kMxfp4Colour><<<grid, 256, 0, stream>>>(pa, cam, til, opt, mx4);
+    }
+}
+
+void launch_project_mx4(int grid, cudaStream_t stream, const ProjectArgs& pa, const gs3d_camera& cam,
+                               const gs3d_tiling& til, const gs3d_render_options& opt, const gs3d_mx4_rows* sh,
+                               const int32_t* indices) {
+    switch (opt.sh_degree) {
+        case 0: launch_project_mx4_degree<0>(grid, stream, pa, cam, til, opt, sh, indices); break;
+        case 1: launch_project_mx4_degree<1>(grid, stream, pa, cam, til, opt, sh, indices); break;
+        case 2: launch_project_mx4_degree<2>(grid, stream, pa, cam, til, opt, sh, indices); break;
+        default: launch_project_mx4_degree<3>(grid, stream, pa, cam, til, opt, sh, indices); break;
+    }
+}
+
 }  // namespace
 
 int check_render_common(const gs3d_gaussians* g, const gs3d_camera* cam, const gs3d_tiling* til,
@@ -468,7 +509,7 @@ GS3D_API int gs3d_render_forward_workspace_size(int64_t capacity_n, int64_t capa
 
 // cov != NULL: render-only input (g's means_opacity_features hold the opacities themselves).
 // mx4 != NULL (render-only input): the colours come from these 4-bit SH rows (row i, or row
-// mx4_indices[i]) in a kernel of their own before the blend; g's sh_coeffs are not read.
+// mx4_indices[i]); g's sh_coeffs are not read.
 static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_gaussians* g,
                                const float* cov, const gs3d_mx4_rows* mx4,
                                const int32_t* mx4_indices, const gs3d_camera* cam,
@@ -535,28 +576,29 @@ static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_ga
     const int pgrid = grid_for(n, 256, 8);
     {
         ProfScope prof("project", stream);
+        const Mx4Sh none{};
         if (mx4) {
-            if (n > 0) k_project<0, true, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt);
+            if (n > 0) launch_project_mx4(pgrid, stream, pa, *cam, *til, *opt, mx4, mx4_indices);
         } else if (cov) {
             switch (opt->sh_degree) {
-                case 0: k_project<0, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                case 1: k_project<1, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                case 2: k_project<2, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                default: k_project<3, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
+                case 0: k_project<0, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                case 1: k_project<1, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                case 2: k_project<2, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                default: k_project<3, true><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
             }
         } else if (flags & GS3D_RENDER_DEFER_COLOUR) {
             switch (opt->sh_degree) {
-                case 0: k_project<0, false, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                case 1: k_project<1, false, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                case 2: k_project<2, false, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                default: k_project<3, false, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
+                case 0: k_project<0, false, kNoColour><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                case 1: k_project<1, false, kNoColour><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                case 2: k_project<2, false, kNoColour><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                default: k_project<3, false, kNoColour><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
             }
         } else {
             switch (opt->sh_degree) {
-                case 0: k_project<0, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                case 1: k_project<1, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                case 2: k_project<2, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
-                default: k_project<3, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt); break;
+                case 0: k_project<0, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                case 1: k_project<1, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                case 2: k_project<2, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
+                default: k_project<3, false><<<pgrid, 256, 0, stream>>>(pa, *cam, *til, *opt, none); break;
             }
         }
         GS3D_LAUNCHED("k_project");
@@ -589,9 +631,6 @@ static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_ga
                                            buf->tiles_end_sdfgidx, buf->df2dgs_codes,
                                            buf->sdf2dgs_codes, buf->sdfgidx_to_fgidx, stream));
         }
-        if (mx4)
-            GS3D_RETURN_IF(launch_mx4_render_colours(mx4, mx4_indices, g->means_opacity_features, n,
-                                                     cam, opt->sh_degree, buf, stream));
         if (!(flags & GS3D_RENDER_DEFER_COLOUR)) {
             ProfScope prof("raster", stream);
             GS3D_RETURN_IF(launch_raster(*outputs, *cam, *til, *opt, *buf,
@@ -646,9 +685,6 @@ static int render_forward_impl(const gs3d_render_outputs* outputs, const gs3d_ga
             counts, buf->capacity_dup, buf->sdf2dgs_codes, nb_tiles, buf->tiles_end_sdfgidx);
         GS3D_LAUNCHED("k_tiles_end");
     }
-    if (mx4)
-        GS3D_RETURN_IF(launch_mx4_render_colours(mx4, mx4_indices, g->means_opacity_features, n, cam,
-                                                 opt->sh_degree, buf, stream));
     // F8 / F9
     if (!(flags & GS3D_RENDER_DEFER_COLOUR)) {
         ProfScope prof("raster", stream);

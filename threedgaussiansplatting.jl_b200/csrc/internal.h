@@ -53,12 +53,8 @@ int inclusive_scan_i32(const int32_t* in, int32_t* out, int64_t capacity, const 
 int scan_spine(int32_t* sums, int64_t capacity, const int32_t* len_dev, int64_t len_host,
                int32_t* total_dev, cudaStream_t stream);
 
-// 4-bit SH rows as the colours of a render (mx4.cu): the argument checks for n Gaussians, and the
-// colours (floats 6..8 of the filtered Gaussians' 2D records) seen from cam; means4 is 4 x n.
+// The argument checks of 4-bit SH rows as the colours of n Gaussians (mx4.cu).
 int check_mx4_sh(const gs3d_mx4_rows* sh, const int32_t* indices, int64_t n, int sh_degree);
-int launch_mx4_render_colours(const gs3d_mx4_rows* sh, const int32_t* indices, const float* means4,
-                              int n, const gs3d_camera* cam, int sh_degree,
-                              const gs3d_render_buffers* buf, cudaStream_t stream);
 
 int device_sm_count();
 

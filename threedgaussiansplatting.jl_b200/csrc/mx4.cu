@@ -20,8 +20,8 @@
 #include "common.cuh"
 #include "internal.h"
 #include "mx4.cuh"
+#include "mx4_colour.cuh"
 #include "rows.cuh"
-#include "sh_colour.cuh"
 
 namespace gs3d {
 namespace {
@@ -466,158 +466,6 @@ int launch_tensor_scale(const gs3d_rows* x, float* tensor_scale, cudaStream_t st
 }
 
 // ---- colours ---------------------------------------------------------------------------------
-// The 4-bit row of a Gaussian in registers: words of eight codes, and the block scales' bytes. Rows of
-// exactly the rendered degree, their codes aligned to 8 bytes at degree 3 (24 bytes a row) and to 2
-// below (2, 6 and 14 bytes).
-template <int DEG, int FMT>
-struct ShRow {
-    static constexpr int DIM = 3 * (DEG + 1) * (DEG + 1), CB = (DIM + 1) / 2, NW = (CB + 3) / 4;
-    static constexpr int BS = Mx4Block<FMT>::size, NB = (DIM + BS - 1) / BS;
-    uint32_t w[NW], scale[NB];
-
-    __device__ __forceinline__ void load(const Mx4Sh& a, int64_t r) {
-        if (r < 0) {  // no row: zero codes with zero scales
-#pragma unroll
-            for (int k = 0; k < NW; ++k) w[k] = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) scale[b] = 0;
-            return;
-        }
-        if constexpr (DEG == 3) {
-            const uint2* p = reinterpret_cast<const uint2*>(a.codes + r * CB);
-#pragma unroll
-            for (int k = 0; k < NW / 2; ++k) {
-                const uint2 v = __ldg(p + k);
-                w[2 * k] = v.x;
-                w[2 * k + 1] = v.y;
-            }
-        } else {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(a.codes + r * CB);
-#pragma unroll
-            for (int k = 0; k < NW; ++k) {
-                // the last word may be half: what is doubled then lies behind the row's end
-                const uint32_t lo = __ldg(p + 2 * k), hi = 4 * k + 2 < CB ? __ldg(p + 2 * k + 1) : lo;
-                w[k] = lo | (hi << 16);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) scale[b] = __ldg(a.scales + r * NB + b);
-    }
-};
-
-// Elements 8 k .. 8 k + 7 of two rows, times 2^-14.
-template <int DEG, int FMT>
-__device__ __forceinline__ void decode_word_pair(const ShRow<DEG, FMT>& r0, const ShRow<DEG, FMT>& r1, int k, Float2* h) {
-    __half2 e0[4], e1[4];
-    e2m1_word_half(r0.w[k], e0);
-    e2m1_word_half(r1.w[k], e1);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 a = __half22float2(e0[j]), b = __half22float2(e1[j]);
-        h[j] = Float2(a.x, b.x);
-        h[j + 4] = Float2(a.y, b.y);
-    }
-}
-
-// 1/2 + the channel's products with the basis, clamped at 0. WHOLE: h are elements times 2^-14, and what
-// lies in one block is summed before its scale (times the tensor scale, in `factor`) multiplies it; else
-// h are the coefficients.
-template <int DEG, int FMT, bool WHOLE>
-__device__ __forceinline__ Float2 channel_pair(int ch, const Float2* h, const Float2* factor, const Float2* basis) {
-    constexpr int NC = (DEG + 1) * (DEG + 1), BS = Mx4Block<FMT>::size;
-    Float2 c(0.5f);
-    if constexpr (WHOLE) {
-        const int b0 = ch * NC / BS, b1 = ((ch + 1) * NC - 1) / BS;
-#pragma unroll
-        for (int b = b0; b <= b1; ++b) {
-            const int k0 = max(b * BS - ch * NC, 0), k1 = min((b + 1) * BS - ch * NC, NC);
-            Float2 s = basis[k0] * h[k0];
-#pragma unroll
-            for (int k = k0 + 1; k < k1; ++k) s = fma2(basis[k], h[k], s);
-            c = fma2(s * Float2(0x1p14f), factor[b], c);
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < NC; ++k) c = fma2(basis[k], h[k], c);
-    }
-    if (c.x < 0.0f) c.x = 0.0f;
-    if (c.y < 0.0f) c.y = 0.0f;
-    return c;
-}
-
-template <int DEG, int FMT>
-__device__ __forceinline__ void block_factors(const ShRow<DEG, FMT>& r0, const ShRow<DEG, FMT>& r1, float g,
-                                              Float2 (&factor)[ShRow<DEG, FMT>::NB]) {
-#pragma unroll
-    for (int b = 0; b < ShRow<DEG, FMT>::NB; ++b)
-        factor[b] = Float2(mx4_scale<FMT>(r0.scale[b]) * g, mx4_scale<FMT>(r1.scale[b]) * g);
-}
-
-// The rows of two Gaussians (-1: zeros): elements and block factors, or (not WHOLE) the coefficients.
-template <int DEG, int FMT, bool WHOLE>
-__device__ __forceinline__ void load_sh_pair(const Mx4Sh& a, int order, int64_t r0, int64_t r1, float g,
-                                             Float2 (&h)[(3 * (DEG + 1) * (DEG + 1) + 7) / 8 * 8],
-                                             Float2 (&factor)[ShRow<DEG, FMT>::NB]) {
-    constexpr int NC = (DEG + 1) * (DEG + 1);
-    if constexpr (WHOLE) {
-        ShRow<DEG, FMT> s0, s1;
-        s0.load(a, r0);
-        s1.load(a, r1);
-        block_factors(s0, s1, g, factor);
-#pragma unroll
-        for (int k = 0; k < ShRow<DEG, FMT>::NW; ++k) decode_word_pair(s0, s1, k, h + 8 * k);
-    } else {
-        constexpr int BS = Mx4Block<FMT>::size;
-        auto element = [&](int64_t r, int e) {
-            if (r < 0) return 0.0f;
-            const Mx4Decode<FMT> d(a.scales[r * a.blocks + e / BS], g);
-            const float2 v = mx4_value(d, e2m1_pair_half(a.codes[r * a.code_bytes + e / 2]));
-            return e & 1 ? v.y : v.x;
-        };
-#pragma unroll
-        for (int c = 0; c < 3; ++c)
-#pragma unroll
-            for (int k = 0; k < NC; ++k) h[c * NC + k] = Float2(element(r0, c * order + k), element(r1, c * order + k));
-    }
-}
-
-// Row of Gaussian i, -1 where its index names none.
-__device__ __forceinline__ int64_t sh_row(const Mx4Sh& a, int64_t i) {
-    if (!a.indices) return i;
-    const int64_t r = (int64_t)__ldg(a.indices + i) - 1;
-    return r < a.rows && r >= 0 ? r : -1;
-}
-
-// The colours of two Gaussians from one position: the three channels of both. At degree 3 a channel is
-// decoded when it is summed, so that 32 coefficients are live and not 96.
-template <int DEG, int FMT, bool WHOLE>
-__device__ __forceinline__ void colour_pair(const Mx4Sh& a, int order, int64_t r0, int64_t r1, float g, const float* p,
-                                            const float4& m0, const float4& m1, Float2 (&c)[3]) {
-    constexpr int NC = (DEG + 1) * (DEG + 1);
-    Float2 basis[NC], factor[ShRow<DEG, FMT>::NB];
-    const Float2 mx(m0.x, m1.x), my(m0.y, m1.y), mz(m0.z, m1.z);
-    if constexpr (WHOLE && DEG == 3) {
-        ShRow<DEG, FMT> s0, s1;
-        s0.load(a, r0);
-        s1.load(a, r1);
-        sh_basis_pair<DEG>(p, mx, my, mz, basis);
-        block_factors(s0, s1, g, factor);
-#pragma unroll
-        for (int ch = 0; ch < 3; ++ch) {
-            Float2 h[16];
-            decode_word_pair(s0, s1, 2 * ch, h);
-            decode_word_pair(s0, s1, 2 * ch + 1, h + 8);
-            c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h, factor, basis);
-        }
-    } else {
-        Float2 h[(3 * NC + 7) / 8 * 8];
-        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h, factor);
-        sh_basis_pair<DEG>(p, mx, my, mz, basis);
-#pragma unroll
-        for (int ch = 0; ch < 3; ++ch) c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h + ch * NC, factor, basis);
-    }
-}
-
 struct Positions {
     float p[GS3D_MAX_FACTORED_VIEWS][3];
 };
@@ -636,47 +484,25 @@ __global__ void __launch_bounds__(128, ONE && WHOLE ? 7 : (DEG == 3 ? 3 : 5)) k_
     const float g = FMT == GS3D_NVFP4 ? __ldg(a.tensor_scale) : 1.0f;
     const int64_t r0 = sh_row(a, i), r1 = two ? sh_row(a, i + 32) : -1;
     const float4 m0 = __ldg(mo4 + i), m1 = __ldg(mo4 + (two ? i + 32 : i));
+    const int64_t r[2] = {r0, r1};
+    const Float2 mx(m0.x, m1.x), my(m0.y, m1.y), mz(m0.z, m1.z);
     if constexpr (ONE) {
         Float2 c[3];
-        colour_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, cv.p[0], m0, m1, c);
+        mx4_colour<Float2, DEG, FMT, WHOLE>(a, order, r, g, cv.p[0], mx, my, mz, c);
         __stcs(out + i, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
         if (two) __stcs(out + i + 32, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
     } else {
         Float2 h[(3 * NC + 7) / 8 * 8], factor[ShRow<DEG, FMT>::NB];
-        load_sh_pair<DEG, FMT, WHOLE>(a, order, r0, r1, g, h, factor);
+        load_sh<Float2, DEG, FMT, WHOLE>(a, order, r, g, h, factor);
         const int last = min(nv, ((int)blockIdx.y + 1) * views);
         for (int v = blockIdx.y * views; v < last; ++v) {
             Float2 basis[NC], c[3];
-            sh_basis_pair<DEG>(cv.p[v], Float2(m0.x, m1.x), Float2(m0.y, m1.y), Float2(m0.z, m1.z), basis);
+            sh_basis_fused<DEG>(cv.p[v], mx, my, mz, basis);
 #pragma unroll
-            for (int ch = 0; ch < 3; ++ch) c[ch] = channel_pair<DEG, FMT, WHOLE>(ch, h + ch * NC, factor, basis);
+            for (int ch = 0; ch < 3; ++ch) c[ch] = mx4_channel<Float2, DEG, FMT, WHOLE>(ch, h + ch * NC, factor, basis);
             float4* o = out + (size_t)v * view_stride + i;
             __stcs(o, make_float4(c[0].x, c[1].x, c[2].x, 0.0f));
             if (two) __stcs(o + 32, make_float4(c[0].y, c[1].y, c[2].y, 0.0f));
-        }
-    }
-}
-
-// Floats 6..8 of the filtered Gaussians' 2D records.
-template <int DEG, int FMT, bool WHOLE>
-__global__ void __launch_bounds__(128) k_mx4_render_colours(const Mx4Sh a, int order,
-                                                            const float4* __restrict__ mo4,
-                                                            const int32_t* __restrict__ f2g,
-                                                            const int32_t* __restrict__ counts,
-                                                            const gs3d_camera cam, float* __restrict__ f2d) {
-    const int F = counts[0];
-    const float g = FMT == GS3D_NVFP4 ? __ldg(a.tensor_scale) : 1.0f;
-    for (int f = blockIdx.x * 256 + (threadIdx.x >> 5) * 64 + (threadIdx.x & 31); f < F; f += gridDim.x * 256) {
-        const bool two = f + 32 < F;
-        const int g0 = f2g[f] - 1, g1 = two ? f2g[f + 32] - 1 : g0;
-        const float4 m0 = __ldg(mo4 + g0), m1 = __ldg(mo4 + g1);
-        Float2 c[3];
-        colour_pair<DEG, FMT, WHOLE>(a, order, sh_row(a, g0), sh_row(a, g1), g, cam.position, m0, m1, c);
-        float* rr = f2d + 9 * (size_t)f;
-#pragma unroll
-        for (int ch = 0; ch < 3; ++ch) {
-            rr[6 + ch] = c[ch].x;
-            if (two) rr[9 * 32 + 6 + ch] = c[ch].y;
         }
     }
 }
@@ -710,8 +536,7 @@ int dispatch_format(int format, bool whole, F&& f) {
 
 template <typename F>
 int dispatch_colours(const gs3d_mx4_rows* sh, int degree, F&& f) {
-    const bool whole = sh->dim == 3 * (degree + 1) * (degree + 1) &&
-                       reinterpret_cast<uintptr_t>(sh->codes) % (degree == 3 ? 8 : 2) == 0;
+    const bool whole = mx4_sh_whole(sh, degree);
     switch (degree) {
         case 0: return dispatch_format<0>(sh->format, whole, f);
         case 1: return dispatch_format<1>(sh->format, whole, f);
@@ -747,29 +572,6 @@ struct ColoursLaunch {
     }
 };
 
-struct RenderColoursLaunch {
-    Mx4Sh a;
-    int order;
-    const float4* mo4;
-    int n;
-    const gs3d_render_buffers* buf;
-    const gs3d_camera* cam;
-    cudaStream_t stream;
-    template <int DEG, int FMT, bool WHOLE>
-    int run() const {
-        k_mx4_render_colours<DEG, FMT, WHOLE><<<grid_for(n, 256, 16), 128, 0, stream>>>(
-            a, order, mo4, buf->fgidx_to_gidx, buf->device_counts, *cam,
-            buf->means2d_opacities_inverse_covariances_colors);
-        GS3D_LAUNCHED("k_mx4_render_colours");
-        return GS3D_OK;
-    }
-};
-
-Mx4Sh sh_source(const gs3d_mx4_rows* sh, const int32_t* indices) {
-    return Mx4Sh{sh->codes, sh->scales, sh->tensor_scale, indices, sh->rows, mx4_code_bytes(sh->dim),
-                 mx4_blocks(sh->dim, sh->format)};
-}
-
 }  // namespace
 
 int check_mx4_sh(const gs3d_mx4_rows* sh, const int32_t* indices, int64_t n, int sh_degree) {
@@ -783,16 +585,6 @@ int check_mx4_sh(const gs3d_mx4_rows* sh, const int32_t* indices, int64_t n, int
     if (!indices && sh->rows < n)
         return invalid("%lld 4-bit SH rows for %lld Gaussians", (long long)sh->rows, (long long)n);
     return GS3D_OK;
-}
-
-int launch_mx4_render_colours(const gs3d_mx4_rows* sh, const int32_t* indices, const float* means4, int n,
-                              const gs3d_camera* cam, int sh_degree, const gs3d_render_buffers* buf,
-                              cudaStream_t stream) {
-    if (n == 0) return GS3D_OK;
-    ProfScope prof("mx4_colours", stream);
-    const RenderColoursLaunch L{sh_source(sh, indices), sh->dim / 3, reinterpret_cast<const float4*>(means4), n,
-                                buf, cam, stream};
-    return dispatch_colours(sh, sh_degree, L);
 }
 
 }  // namespace gs3d
@@ -848,7 +640,7 @@ GS3D_API int gs3d_mx4_colours(const gs3d_mx4_rows* sh, int32_t sh_degree, const 
     if ((reinterpret_cast<uintptr_t>(means4) & 15) || (reinterpret_cast<uintptr_t>(colours) & 15))
         return invalid("means or colours not 16-byte aligned");
     if (n == 0) return GS3D_OK;
-    ColoursLaunch L{sh_source(sh, indices), sh->dim / 3, reinterpret_cast<const float4*>(means4), n, {}, n_views,
+    ColoursLaunch L{mx4_sh_source(sh, indices), sh->dim / 3, reinterpret_cast<const float4*>(means4), n, {}, n_views,
                     reinterpret_cast<float4*>(colours), view_stride, stream};
     for (int v = 0; v < n_views; ++v)
         for (int k = 0; k < 3; ++k) L.cv.p[v][k] = view_positions[3 * v + k];

@@ -84,14 +84,4 @@ __device__ __forceinline__ float2 mx4_value(const Mx4Decode<FMT>& d, __half2 e) 
     return make_float2(v.x * d.factor(), v.y * d.factor());
 }
 
-// 4-bit SH rows as a colour source: row i, or row indices[i].
-struct Mx4Sh {
-    const uint8_t* codes;
-    const uint8_t* scales;
-    const float* tensor_scale;
-    const int32_t* indices;
-    int64_t rows;
-    int code_bytes, blocks;
-};
-
 }  // namespace gs3d

@@ -64,38 +64,41 @@ __device__ __forceinline__ Float2 operator*(Float2 a, Float2 b) {
     return r;
 }
 
-// The basis functions (sh.jl:123-149) at the unit directions from p to two means, with fused
-// multiply-adds and the reciprocal square root (rsqrtf, 2 ulp): within a few ulp of sh_basis.
-template <int DEG>
-__device__ __forceinline__ void sh_basis_pair(const float* p, Float2 mx, Float2 my, Float2 mz,
-                                              Float2 (&b)[(DEG + 1) * (DEG + 1)]) {
-    b[0] = Float2(sh_c(1));
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float rsqrt2(float v) { return rsqrtf(v); }
+__device__ __forceinline__ Float2 rsqrt2(Float2 v) { return Float2(rsqrtf(v.x), rsqrtf(v.y)); }
+
+// The basis functions (sh.jl:123-149) at the unit direction from p to a mean (V: float) or to two
+// (Float2), with fused multiply-adds and the reciprocal square root (rsqrtf, 2 ulp): within a few ulp of
+// sh_basis.
+template <int DEG, typename V>
+__device__ __forceinline__ void sh_basis_fused(const float* p, V mx, V my, V mz, V (&b)[(DEG + 1) * (DEG + 1)]) {
+    b[0] = V(sh_c(1));
     if constexpr (DEG >= 1) {
-        const Float2 one(1.0f), minus(-1.0f);
-        Float2 x = fma2(mx, one, Float2(-p[0])), y = fma2(my, one, Float2(-p[1])), z = fma2(mz, one, Float2(-p[2]));
-        const Float2 ss = fma2(z, z, fma2(y, y, x * x));
-        const Float2 inv(rsqrtf(ss.x), rsqrtf(ss.y));
+        const V one(1.0f), minus(-1.0f);
+        V x = fma2(mx, one, V(-p[0])), y = fma2(my, one, V(-p[1])), z = fma2(mz, one, V(-p[2]));
+        const V inv = rsqrt2(fma2(z, z, fma2(y, y, x * x)));
         x = x * inv, y = y * inv, z = z * inv;
-        b[1] = y * Float2(-sh_c(2));
-        b[2] = z * Float2(sh_c(3));
-        b[3] = x * Float2(-sh_c(4));
+        b[1] = y * V(-sh_c(2));
+        b[2] = z * V(sh_c(3));
+        b[3] = x * V(-sh_c(4));
         if constexpr (DEG >= 2) {
-            const Float2 xx = x * x, yy = y * y, zz = z * z, xy = x * y;
-            const Float2 sum = fma2(xx, one, yy), diff = fma2(yy, minus, xx), less = fma2(sum, minus, Float2(0.0f));
-            b[4] = xy * Float2(sh_c(5));
-            b[5] = y * z * Float2(sh_c(6));
-            b[6] = fma2(zz, Float2(2.0f), less) * Float2(sh_c(7));
-            b[7] = x * z * Float2(sh_c(8));
-            b[8] = diff * Float2(sh_c(9));
+            const V xx = x * x, yy = y * y, zz = z * z, xy = x * y;
+            const V sum = fma2(xx, one, yy), diff = fma2(yy, minus, xx), less = sum * minus;
+            b[4] = xy * V(sh_c(5));
+            b[5] = y * z * V(sh_c(6));
+            b[6] = fma2(zz, V(2.0f), less) * V(sh_c(7));
+            b[7] = x * z * V(sh_c(8));
+            b[8] = diff * V(sh_c(9));
             if constexpr (DEG >= 3) {
-                const Float2 four = fma2(zz, Float2(4.0f), less);
-                b[9] = y * Float2(sh_c(10)) * fma2(xx, Float2(3.0f), yy * minus);
-                b[10] = xy * z * Float2(sh_c(11));
-                b[11] = y * Float2(sh_c(12)) * four;
-                b[12] = z * Float2(sh_c(13)) * fma2(zz, Float2(2.0f), sum * Float2(-3.0f));
-                b[13] = x * Float2(sh_c(14)) * four;
-                b[14] = z * Float2(sh_c(15)) * diff;
-                b[15] = x * Float2(sh_c(16)) * fma2(yy, Float2(-3.0f), xx);
+                const V four = fma2(zz, V(4.0f), less);
+                b[9] = y * V(sh_c(10)) * fma2(xx, V(3.0f), yy * minus);
+                b[10] = xy * z * V(sh_c(11));
+                b[11] = y * V(sh_c(12)) * four;
+                b[12] = z * V(sh_c(13)) * fma2(zz, V(2.0f), sum * V(-3.0f));
+                b[13] = x * V(sh_c(14)) * four;
+                b[14] = z * V(sh_c(15)) * diff;
+                b[15] = x * V(sh_c(16)) * fma2(yy, V(-3.0f), xx);
             }
         }
     }

@@ -131,9 +131,8 @@ int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, c
 //    the table's gradients.
 // 2. k_table_segments: the sorted rows are cut into chunks of equal length, a block each, and a chunk
 //    into one run of rows per slot (a slot: the threads side by side on a row's columns). A slot adds
-//    its rows in order; a run of equal indices that starts and ends inside a slot is finished and
-//    stored, the slots' first and last runs are added in slot order through shared memory, and what
-//    crosses a chunk's border is left as a partial sum.
+//    its rows in order; a run of equal indices that crosses slots is added up in slot order through
+//    shared memory, and what crosses a chunk's border is left as a partial sum.
 // 3. k_table_join: the block in whose chunk such a run starts adds its partial sums in chunk order.
 // The order of every sum follows from the sorted order alone, whatever the number of rows that share
 // an index: no atomics, and a row that half of the Gaussians use is spread over the GPU like any other.
@@ -530,15 +529,15 @@ __device__ __forceinline__ void store_row(const Segments& g, int key, int col, c
     }
 }
 
-// The sums of one chunk: `count` items in shared memory, cut into runs of `run` for the slots; every
-// thread of the block calls it (those with slot >= pl.slots only wait). open_left / open_right: the first
-// / last run goes on in the chunk before / behind, and its sum goes to partial[0 ..] / partial[dim ..]
-// (`earlier`: the whole chunk is one run that began before it, its sum at partial[0 ..]).
+// The sums of one chunk: `count` items in shared memory, `run` after the other for each slot; every thread
+// of the block calls it (those with slot >= pl.slots only wait). Where runs of equal indices cross from
+// slot to slot the slot in which one starts adds the others' sums of it, from `part`, in slot order.
+// open_left / open_right: the chunk's first / last run goes on in the chunk before / behind, and its sum
+// goes to partial[0 ..] / partial[dim ..] (to the former if it is the same run).
 template <typename T, int VB>
 __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int stride, int dim, const SegmentPlan& pl,
-                                          int run, const Segments& g, const int2* items, int count, int32_t* pkey,
-                                          float* part, bool open_left, bool open_right, bool earlier,
-                                          float* __restrict__ partial) {
+                                          int run, const Segments& g, const int2* items, int count, float* part,
+                                          bool open_left, bool open_right, float* __restrict__ partial) {
     using Unit = RowUnit<T, VB>;
     constexpr int N = Unit::N, AHEAD = VB == 16 ? 6 : 8;  // rows in flight a slot
     const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
@@ -546,16 +545,34 @@ __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int strid
     const int col = unit * N;
     const bool on = unit < pl.units;
     const int width = pl.tile_units * N;
-    if (slot < pl.slots) {
-        const int j1 = min((slot + 1) * run, count);
-        int j = slot * run;
-        int cur = j < j1 ? items[j].x : -1;
-        bool first = true;
-        float acc[N];
+    const int j0 = slot * run, j1 = min(j0 + run, count);
+    const bool some = slot < pl.slots && j0 < count;
+    float acc[N];
+    int cur = 0;
+    bool from_left = false;  // the run in acc came from the slot before
+    // a run that is complete, or goes on beyond the chunk
+    const auto emit = [&](bool at_start, bool at_end) {
+        if (!on) return;
+        if (at_start && open_left || at_end && open_right) {
+            float* p = partial + (at_start && open_left ? 0 : dim) + col;
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] = acc[i];
+        } else {
+            store_row<N>(g, cur, col, acc);
+        }
+    };
+    const auto hand_left = [&] {
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[slot * width + lane * N + i] = acc[i];
+    };
+    bool first = true;
+    if (some) {
+        cur = items[j0].x;
+        from_left = slot > 0 && items[j0 - 1].x == cur;
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.0f;
         const T* gc = grads + (on ? col : 0);
-        for (; j < j1; j += AHEAD) {
+        for (int j = j0; j < j1; j += AHEAD) {
             Unit u[AHEAD];
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) u[q].load(gc + (int64_t)items[min(j + q, j1 - 1)].y * stride);
@@ -571,14 +588,9 @@ __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int strid
                 if (j + q >= j1) break;
                 const int key = items[j + q].x;
                 if (key != cur) {
-                    if (first) {
-#pragma unroll
-                        for (int i = 0; i < N; ++i) part[(2 * slot) * width + lane * N + i] = acc[i];
-                        if (lane == 0) pkey[2 * slot] = cur;
-                        first = false;
-                    } else if (on) {
-                        store_row<N>(g, cur, col, acc);
-                    }
+                    if (first && from_left) hand_left();
+                    else emit(first && slot == 0, false);
+                    first = false;
                     cur = key;
 #pragma unroll
                     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
@@ -587,58 +599,27 @@ __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int strid
                 for (int i = 0; i < N; ++i) acc[i] += to_f32(u[q].e[i]);
             }
         }
-        const int which = 2 * slot + (first ? 0 : 1);
-#pragma unroll
-        for (int i = 0; i < N; ++i) part[which * width + lane * N + i] = acc[i];
-        if (lane == 0) {
-            pkey[which] = cur;
-            if (first) pkey[2 * slot + 1] = -1;
-        }
+        if (first && from_left) hand_left();
     }
     __syncthreads();
-    if (slot != 0) return;
-    // the slots' open runs in order
-    float acc[N];
+    if (!some || (first && from_left)) return;
+    int end = j1;
+    for (int s = slot + 1; end < count && items[end].x == cur; ++s) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-    int cur = items[0].x;
-    bool first = true;
-    for (int e = 0; e < 2 * pl.slots; ++e) {
-        const int k = pkey[e];
-        if (k < 0) continue;
-        if (k != cur) {
-            if (on) {
-                if (first && open_left) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) partial[col + i] = acc[i];
-                } else {
-                    store_row<N>(g, cur, col, acc);
-                }
-            }
-            first = false;
-            cur = k;
-#pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += part[e * width + lane * N + i];
+        for (int i = 0; i < N; ++i) acc[i] += part[s * width + lane * N + i];
+        const int next = min(end + run, count);
+        if (items[next - 1].x != cur) break;  // it ends inside that slot
+        end = next;
     }
-    if (!on) return;
-    if (earlier || open_right) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) partial[(earlier ? 0 : dim) + col + i] = acc[i];
-    } else {
-        store_row<N>(g, cur, col, acc);
-    }
+    emit(first && slot == 0, end == count);
 }
 
 template <typename T, int VB>
 __global__ void __launch_bounds__(256, VB == 16 ? 4 : 5) k_table_segments(const T* __restrict__ grads, int stride, int dim,
                                                            const SegmentPlan pl, const Segments g) {
     extern __shared__ __align__(16) unsigned char smem[];
-    int2* items = reinterpret_cast<int2*>(smem);                   // the chunk's
-    int32_t* pkey = reinterpret_cast<int32_t*>(items + pl.chunk);  // [slot][2]: the slots' first and last runs
-    float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);   // [slot][2][tile_units * N]
+    int2* items = reinterpret_cast<int2*>(smem);                // the chunk's
+    float* part = reinterpret_cast<float*>(items + pl.chunk);   // [slot][tile_units * N]
     after_predecessor();
     const int m = *g.valid;
     const int begin = blockIdx.x * pl.chunk, count = min(pl.chunk, m - begin);
@@ -661,7 +642,7 @@ __global__ void __launch_bounds__(256, VB == 16 ? 4 : 5) k_table_segments(const 
         g.first_key[blockIdx.x] = head;
         g.owned[blockIdx.x] = open_right && !earlier ? last : -1;
     }
-    sum_chunk<T, VB>(grads, stride, dim, pl, pl.run, g, items, count, pkey, part, open_left, open_right, earlier,
+    sum_chunk<T, VB>(grads, stride, dim, pl, pl.run, g, items, count, part, open_left, open_right,
                      g.partial + (int64_t)blockIdx.x * 2 * dim);
 }
 
@@ -701,10 +682,8 @@ __global__ void __launch_bounds__(kTinyThreads) k_table_gradient_tiny(const T* _
     if (p0 > 0) p0 = first_above(items, count, items[p0 - 1].x);
     if (p1 > 0) p1 = first_above(items, count, items[p1 - 1].x);
     if (p1 <= p0) return;
-    int32_t* pkey = reinterpret_cast<int32_t*>(smem);
-    float* part = reinterpret_cast<float*>(pkey + 2 * pl.slots);
-    sum_chunk<T, VB>(grads, stride, dim, pl, (p1 - p0 + pl.slots - 1) / pl.slots, g, items + p0, p1 - p0, pkey, part,
-                     false, false, false, nullptr);
+    sum_chunk<T, VB>(grads, stride, dim, pl, (p1 - p0 + pl.slots - 1) / pl.slots, g, items + p0, p1 - p0,
+                     reinterpret_cast<float*>(smem), false, false, nullptr);
 }
 
 // A warp per chunk for the runs of up to 32 partial sums behind the first (nearly all: an average run is
@@ -890,7 +869,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
             const SegmentPlan pl = segment_plan(n, grads->dim / per);
             const Segments seg{nullptr, nullptr, out, table_grads->row_stride, scale, accumulate ? 1 : 0, nullptr,
                                nullptr, nullptr};
-            const size_t smem = (size_t)pl.slots * 8 + (size_t)pl.slots * 2 * pl.tile_units * per * 4;
+            const size_t smem = (size_t)pl.slots * pl.tile_units * per * 4;
             // a block for 32 rows, or for 64 KB of table to zero
             const int64_t zeroed = accumulate ? 0 : table_grads->rows * table_grads->dim;
             const int blocks = (int)std::max<int64_t>(ceil_div(n, 32), std::min<int64_t>(ceil_div(zeroed, 1 << 14), kSMs));
@@ -939,7 +918,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
         const bool wide = wide_rows<T>(grads);
         const int per = wide ? 16 / (int)sizeof(T) : 1;
         const SegmentPlan pl = segment_plan(n, grads->dim / per);
-        const size_t smem = (size_t)pl.chunk * 8 + (size_t)pl.slots * 8 + (size_t)pl.slots * 2 * pl.tile_units * per * 4;
+        const size_t smem = (size_t)pl.chunk * 8 + (size_t)pl.slots * pl.tile_units * per * 4;
         const dim3 grid(pl.nchunks, (unsigned)ceil_div(pl.units, pl.tile_units));
         const int threads = pl.slots * pl.tile_units;
         const int stride = (int)grads->row_stride;

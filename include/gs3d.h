@@ -547,8 +547,8 @@ GS3D_API int gs3d_opacity_reset(
 #define GS3D_F16 1
 #define GS3D_BF16 2
 
-/* `rows` rows of `dim` elements; row r starts at element r * row_stride of data (row_stride >= dim;
- * data aligned to its elements). Rows of SH coefficients have dim = 3 (d+1)^2, channel by channel,
+/* `rows` (at most 2^30) rows of `dim` (at most 2^16) elements; row r starts at element r * row_stride of
+ * data (dim <= row_stride < 2^31; data aligned to its elements). Rows of SH coefficients have dim = 3 (d+1)^2, channel by channel,
  * as sh_coeffs holds them. */
 typedef struct gs3d_rows {
     int64_t rows;
@@ -573,8 +573,8 @@ GS3D_API int gs3d_table_gradient_workspace_size(int64_t grad_rows, int64_t table
                                                 size_t* bytes);
 
 /* The gradient of gs3d_table_lookup: table_grads[k] = scale * sum of grads[f] over the rows f whose
- * index is k + 1, summed in fp32 in an order that depends on the indices alone (equal inputs give
- * equal bits). Rows of the table that no index names get zeros.
+ * index is k + 1, summed in fp32 in an order fixed by the indices, the sizes and the alignment (equal
+ * calls give equal bits). Rows of the table that no index names get zeros.
  *   fgidx_to_gidx == NULL: row f has index indices[f] (grads->rows indices).
  *   fgidx_to_gidx != NULL: row f belongs to filtered Gaussian f, as gs3d_backward writes
  *     sh_coeffs_grads: its index is indices[fgidx_to_gidx[f] - 1] (n_indices indices; entries
@@ -609,8 +609,8 @@ typedef struct gs3d_mx4_rows {
     const float* tensor_scale;
 } gs3d_mx4_rows;
 
-/* tensor_scale[0] = max(largest finite |x| / (6 * 448), 2^-100): the GS3D_NVFP4 tensor scale with
- * which no block scale of x saturates. */
+/* tensor_scale[0] = max(largest finite |x| * (1 / 2688), 2^-100), 2688 = 6 * 448, the reciprocal and the
+ * product in fp32: the GS3D_NVFP4 tensor scale with which the block scales of x use their range. */
 GS3D_API int gs3d_mx4_tensor_scale(const gs3d_rows* x, float* tensor_scale, gs3d_stream_t stream);
 
 /* Quantise x into `out` (same rows and dim). Per block with largest magnitude a: GS3D_NVFP4 block

@@ -332,7 +332,7 @@ def test_quantise(cuda, n, dim, kind, fmt, spread):
     if fmt == "nvfp4":
         ts = gc.mx4_tensor_scale(x.to(cuda))
         a = x.float().abs()  # the widest spread overflows fp16: infinities do not count
-        want = max(np.float32(a[a.isfinite()].max().numpy()) / np.float32(2688.0), np.float32(2.0 ** -100))
+        want = max(np.float32(a[a.isfinite()].max().numpy()) * (np.float32(1) / np.float32(2688)), np.float32(2.0 ** -100))
         assert ts.cpu().numpy()[0] == want
         # its own scale; one that makes blocks saturate; a power of two, where borders are met exactly
         scales = [None, torch.tensor([float(want) * 0.013]), torch.tensor([2.0 ** -6])]

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kScaleThreads) k_mx4_tensor_scale(const T* __r
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kScaleThreads / 32; ++w) m = max(m, warp_max[w]);
-        const uint32_t scale = f2u(fmaxf(u2f(m) / 2688.0f, 0x1p-100f));
+        const uint32_t scale = f2u(fmaxf(u2f(m) * (1.0f / 2688.0f), 0x1p-100f));
         if (gridDim.x == 1) *tensor_scale = scale;
         else atomicMax(tensor_scale, scale);
     }

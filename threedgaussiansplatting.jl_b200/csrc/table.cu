@@ -13,10 +13,12 @@ namespace gs3d {
 namespace {
 
 // ---- lookup ----------------------------------------------------------------------------------
-// Bound by the rows written (the table stays in L2). Threads side by side on a row's units of N
-// elements, ROWS rows a thread, as many independent loads in flight. A unit is 16 bytes of the wider of
-// table and output (two half types: of both) where all rows are so aligned, else one element.
-// 3M x 48 fp32, 1 / 2 / 4 / 8 rows: 129 / 103 / 94 / 117 us (a write-only fill: 79).
+// out[i] = table[indices[i] - 1] * scale. Bound by the rows written (the table stays in L2). Threads side
+// by side on a row's units of N elements, ROWS rows a thread, as many independent loads in flight. A unit
+// is 16 bytes of the wider of table and output (two half types: of both) where all rows are so aligned
+// (3M x 48 fp32 with 1 / 2 / 4 / 8 rows: 129 / 103 / 94 / 117 us; a write-only fill of as much: 79). Else it
+// is one element, and a thread takes COLS of a row, a share of the columns apart, for one index and one
+// address (500K x 27 bf16: 17.1 us with one column, 15.3 with two; bound by the instructions).
 constexpr int kLookupRows = 4, kLookupColumns = 2;
 
 template <typename T, int N>
@@ -57,7 +59,7 @@ __global__ void __launch_bounds__(256) k_table_lookup(const TI* __restrict__ tab
                                                       TO* __restrict__ out, int n, int64_t out_stride, int units,
                                                       int tile_units, int slots) {
     const int slot = threadIdx.x / tile_units;
-    const int unit = blockIdx.y * (COLS * tile_units) + threadIdx.x - slot * tile_units;  // and COLS - 1 more, tile_units apart
+    const int unit = blockIdx.y * (COLS * tile_units) + threadIdx.x - slot * tile_units;  // the first of COLS
     if (unit >= units) return;
     const int first = blockIdx.x * (slots * ROWS) + slot;
     const TI* column = table + unit * N;
@@ -125,17 +127,20 @@ int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, c
 }
 
 // ---- gradient --------------------------------------------------------------------------------
-// 1. Stable sort of the rows by table row (radix_*: 4096-row tiles, digits of up to 10 bits, three
-//    launches a pass, one pass per 10 bits of the row number; up to 4096 rows: one block sorts them in
-//    shared memory; up to 1024: k_table_gradient_tiny does everything). Rows without a valid index drop out of the first pass, which also zeroes
-//    the table's gradients.
+// 1. Stable sort of the rows by table row (k_radix_*: tiles of 4096 rows, digits of up to 10 bits, three
+//    launches and one pass per 10 bits of the row number; up to 4096 rows k_sort_small, one block in shared
+//    memory; up to 1024 k_table_gradient_tiny does everything). Rows without a valid index drop out of
+//    the first pass, which also zeroes the table's gradients.
 // 2. k_table_segments: the sorted rows are cut into chunks of equal length, a block each, and a chunk
 //    into one run of rows per slot (a slot: the threads side by side on a row's columns). A slot adds
 //    its rows in order; a run of equal indices that crosses slots is added up in slot order through
 //    shared memory, and what crosses a chunk's border is left as a partial sum.
 // 3. k_table_join: the block in whose chunk such a run starts adds its partial sums in chunk order.
-// The order of every sum follows from the sorted order alone, whatever the number of rows that share
-// an index: no atomics, and a row that half of the Gaussians use is spread over the GPU like any other.
+// The order of every sum follows from the sorted order and the sizes, whatever the number of rows that
+// share an index: no atomics, and a row that half of the Gaussians use is spread over the GPU like any
+// other. 3M x 48 fp32 into 65,536 rows, 194 us (the bytes alone: 93): sort 61 (count 8 to 15 a pass, bound
+// by the gathers of the indices; spine 3; scatter 20, bound by ranking in shared memory: matched by
+// ballots, 30 with match_any), sums 125 (the random 192-byte gather alone: 107 to 112), join 5.
 
 // The kernels of one call follow one another with programmatic dependent launch: each starts while
 // the one before it ends, and waits in `after_predecessor` (every thread, before anything else, so
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPas
     }
     for (int i = threadIdx.x; i < nbins * kSortWarps / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(wcount)[i] = 0;
     __syncthreads();
-    // stable rank of every key among its warp's keys of the same digit: first within its 32, then behind the 32s
+    // stable rank of every key among its warp's keys of the same digit: within its 32, then behind the 32s
     // before
     int rank[kSortRounds];
     const unsigned below = (1u << lane) - 1u;
@@ -615,8 +620,8 @@ __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int strid
 }
 
 template <typename T, int VB>
-__global__ void __launch_bounds__(256, VB == 16 ? 4 : 5) k_table_segments(const T* __restrict__ grads, int stride, int dim,
-                                                           const SegmentPlan pl, const Segments g) {
+__global__ void __launch_bounds__(256, VB == 16 ? 4 : 5)
+    k_table_segments(const T* __restrict__ grads, int stride, int dim, const SegmentPlan pl, const Segments g) {
     extern __shared__ __align__(16) unsigned char smem[];
     int2* items = reinterpret_cast<int2*>(smem);                // the chunk's
     float* part = reinterpret_cast<float*>(items + pl.chunk);   // [slot][tile_units * N]
@@ -672,12 +677,15 @@ __global__ void __launch_bounds__(kTinyThreads) k_table_gradient_tiny(const T* _
     __shared__ int start[256], sm[33];
     const int count = sort_rows<kTinyThreads, kTinyRows / kTinyThreads>(src, bits, items, wcount, start, sm);
     const int64_t b = blockIdx.x, blocks = gridDim.x;
-    if (zero.data && blockIdx.y == 0)
-        for (int64_t k = b * zero.rows / blocks + threadIdx.x; k < (b + 1) * zero.rows / blocks; k += kTinyThreads) {
+    if (zero.data && blockIdx.y == 0) {
+        const int side = dim > 128 ? 32 : 1;  // a row a thread, long ones a warp
+        for (int64_t k = b * zero.rows / blocks + threadIdx.x / side; k < (b + 1) * zero.rows / blocks;
+             k += kTinyThreads / side) {
             const int p = first_above(items, count, (int)k);
             if (p == 0 || items[p - 1].x != k)
-                for (int c = 0; c < dim; ++c) zero.data[k * zero.stride + c] = 0.0f;
+                for (int c = threadIdx.x % side; c < dim; c += side) zero.data[k * zero.stride + c] = 0.0f;
         }
+    }
     int p0 = (int)(b * count / blocks), p1 = (int)((b + 1) * count / blocks);
     if (p0 > 0) p0 = first_above(items, count, items[p0 - 1].x);
     if (p1 > 0) p1 = first_above(items, count, items[p1 - 1].x);
@@ -745,7 +753,9 @@ struct GradLayout {
     int ntiles, passes, bits, chunks_max;
 };
 
-constexpr int kMinRun = 4, kMaxRun = 48;  // rows a slot adds: enough blocks for few rows, few borders for many
+// Rows a slot adds: enough blocks for few rows, few borders for many (3M: 32 / 48 / 96 rows 197 / 194 / 196 us;
+// 500K: 39.6 / 37.4 / 41.5).
+constexpr int kMinRun = 4, kMaxRun = 48;
 
 // Rows that can be read 16 bytes at a time.
 template <typename T>
@@ -770,7 +780,6 @@ int bits_of(int64_t v) {
     while (v >> b) ++b;
     return b;
 }
-
 
 GradLayout grad_layout(int64_t n, int64_t rows, int dim) {
     GradLayout L;
@@ -872,7 +881,8 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
             const size_t smem = (size_t)pl.slots * pl.tile_units * per * 4;
             // a block for 32 rows, or for 64 KB of table to zero
             const int64_t zeroed = accumulate ? 0 : table_grads->rows * table_grads->dim;
-            const int blocks = (int)std::max<int64_t>(ceil_div(n, 32), std::min<int64_t>(ceil_div(zeroed, 1 << 14), kSMs));
+            const int blocks =
+                (int)std::max<int64_t>(ceil_div(n, 32), std::min<int64_t>(ceil_div(zeroed, 1 << 14), kSMs));
             const dim3 grid(blocks, (unsigned)ceil_div(pl.units, pl.tile_units));
             const auto kernel = wide ? k_table_gradient_tiny<T, 16> : k_table_gradient_tiny<T, (int)sizeof(T)>;
             kernel<<<grid, kTinyThreads, smem, stream>>>(g, (int)grads->row_stride, grads->dim, pl, seg, src, zero, L.bits);

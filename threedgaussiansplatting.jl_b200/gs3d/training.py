@@ -329,7 +329,8 @@ class TableTrainer(Trainer):
     table's rows (table_gradient), and takes an Adam step on the table and on the Gaussians' geometry.
     The set of Gaussians and their rows stay as they are: no densification, opacity reset or SH-degree
     increase. `sh_table.coeffs` (float32, SH storage degree of `gaussians`) is updated in place;
-    `gaussians.sh_coeffs` is overwritten at every step."""
+    `gaussians.sh_coeffs` is overwritten at every step with what that step renders (prepare_model() brings
+    it up to date with the table)."""
 
     def __init__(self, gaussians: GaussiansVector, sh_table, cameras: list[PinholeCamera], targets,
                  render_options: RenderOptions, tiling: Tiling, options: TrainingOptions, **kwargs):

@@ -547,9 +547,9 @@ GS3D_API int gs3d_opacity_reset(
 #define GS3D_F16 1
 #define GS3D_BF16 2
 
-/* `rows` (at most 2^30) rows of `dim` (at most 2^16) elements; row r starts at element r * row_stride of
- * data (dim <= row_stride < 2^31; data aligned to its elements). Rows of SH coefficients have dim = 3 (d+1)^2, channel by channel,
- * as sh_coeffs holds them. */
+/* `rows` (at most 2^30) rows of `dim` (at most 2^16) elements; row r starts at element
+ * r * row_stride of data (dim <= row_stride < 2^31; data aligned to its elements). Rows of SH
+ * coefficients have dim = 3 (d+1)^2, channel by channel, as sh_coeffs holds them. */
 typedef struct gs3d_rows {
     int64_t rows;
     int64_t row_stride;
@@ -590,7 +590,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
 /* Microscaled 4-bit rows. An element is a sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (e2m1); a block
  * of consecutive elements of a row shares a scale (the last block of a row may be short).
  *   GS3D_NVFP4: blocks of 16, e4m3 block scales, one fp32 scale for all rows (*tensor_scale in
- *     device memory, within 2^-100 .. 2^100): value = element * block scale * tensor scale,
+ *     device memory, from 2^-100 to the largest fp32 / 2688): value = element * block scale * tensor scale,
  *     rounded once to fp32.
  *   GS3D_MXFP4: blocks of 32, power-of-two block scales (e8m0: 2^(byte - 127)): value = element *
  *     block scale. tensor_scale is not read.

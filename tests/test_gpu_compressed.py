@@ -401,6 +401,24 @@ def test_quantise_non_finite(cuda, fmt):
     assert float(gc.mx4_tensor_scale(torch.zeros(0, 4, device=cuda))) == 2.0 ** -100
 
 
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("dim", [48, 27])
+def test_quantise_largest_and_smallest(cuda, fmt, dim):
+    """Up to the largest fp32 values, whose tensor scale is the largest, and down to subnormal ones."""
+    gen = rng(12)
+    for top in (float(np.finfo(np.float32).max), 2.0 ** 113, 2.0 ** -110, 2.0 ** -140):
+        x = torch.from_numpy((torch.rand(50, dim, generator=gen).double() * 2 - 1).numpy() * top).float()
+        x[0, 1] = top
+        x[3] = 0.0
+        q = gc.mx4_quantise(x.to(cuda), fmt)
+        g = float(q.tensor_scale.cpu()) if fmt == "nvfp4" else 1.0
+        codes, byte, val, _ = quantise_exact(x, fmt, g)
+        assert np.array_equal(q.scales.cpu().numpy(), byte)
+        assert np.array_equal(q.codes.cpu().numpy(), codes)
+        assert np.isfinite(val).all() or fmt == "mxfp4"
+        assert np.array_equal(gc.mx4_dequantise(q).cpu().numpy(), val)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("dim,stride,offset", [(48, 64, 0), (48, 49, 1), (27, 31, 3), (16, 24, 8)])
 def test_quantise_strides(cuda, kind, dim, stride, offset):

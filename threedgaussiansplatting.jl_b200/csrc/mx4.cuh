@@ -54,7 +54,9 @@ __device__ __forceinline__ void e2m1_word_half(uint32_t word, __half2 (&e)[4]) {
 // The values of two elements: element * block scale * tensor scale, rounded once, as scaled(element *
 // 2^-14) * factor().
 // NVFP4: element * block scale has 6 significant bits and is a multiple of 2^-10 up to 2688: exact in
-// fp16 times 2^-14. MXFP4: element * 2^k, exact in fp32 up to its overflow and underflow.
+// fp16 times 2^-7, with 2^7 of the 2^14 in the scale (at most 57344). The other 2^7 is the factor's, which
+// stays finite for every tensor scale up to 2^117. MXFP4: element * 2^k, exact in fp32 up to its overflow
+// and underflow.
 template <int FMT>
 struct Mx4Decode;
 
@@ -63,7 +65,7 @@ struct Mx4Decode<GS3D_NVFP4> {
     __half2 s;
     float g;
     __device__ __forceinline__ Mx4Decode(uint32_t byte, float tensor_scale)
-        : s(__half2half2(e4m3_half(byte))), g(tensor_scale * 0x1p14f) {}
+        : s(__half2half2(__hmul(e4m3_half(byte), __ushort_as_half(0x5800)))), g(tensor_scale * 0x1p7f) {}  // 2^7
     __device__ __forceinline__ float2 scaled(__half2 e) const { return __half22float2(__hmul2(e, s)); }
     __device__ __forceinline__ float factor() const { return g; }
 };

@@ -177,8 +177,8 @@ def mx4_tensor_scale(x: torch.Tensor, stream: torch.cuda.Stream | None = None) -
 def mx4_quantise(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None,
                  stream: torch.cuda.Stream | None = None) -> MX4Rows:
     """The rows of `x` ((rows, ...), float32, float16 or bfloat16) as 4-bit elements with block
-    scales (gs3d_mx4_quantise). `tensor_scale` (nvfp4): (1,) float32 on the device, within 2^-100 ..
-    2^100; None: mx4_tensor_scale(x)."""
+    scales (gs3d_mx4_quantise). `tensor_scale` (nvfp4): (1,) float32 on the device, from 2^-100 to
+    the largest float32 / 2688; None: mx4_tensor_scale(x)."""
     device = _check_device(x, tensor_scale)
     c = _rows_c(x, "x")
     handle, context = _enter(device, stream)

@@ -128,6 +128,33 @@ def test_colour_refusals():
     assert call(n=0, means=None, out=None, stride=0) == _abi.GS3D_OK
 
 
+def test_misaligned_words_are_refused():
+    pos = (C.c_float * 3)()
+    r, out, q = rows(), rows(), mx4()
+    odd = DATA + 2
+    refused(LIB.gs3d_table_lookup(C.byref(r), odd, 1.0, C.byref(out), None), "indices", "aligned")
+    for k, what in enumerate(("indices", "fgidx_to_gidx", "device_counts")):
+        a = [DATA, DATA, DATA]
+        a[k] = odd
+        refused(LIB.gs3d_table_gradient(C.byref(r), a[0], 4, a[1], a[2], 1.0, C.byref(out), 0, DATA, BIG, None),
+                what, "aligned")
+    refused(LIB.gs3d_mx4_tensor_scale(C.byref(r), odd, None), "tensor scale", "aligned")
+    bad = mx4(ts=odd)
+    refused(LIB.gs3d_mx4_quantise(C.byref(r), C.byref(bad), None), "tensor scale", "aligned")
+    refused(LIB.gs3d_mx4_dequantise(C.byref(bad), C.byref(out), None), "tensor scale", "aligned")
+    refused(LIB.gs3d_mx4_colours(C.byref(bad), 3, None, DATA, 4, pos, 1, DATA, 4, None), "tensor scale", "aligned")
+    refused(LIB.gs3d_mx4_colours(C.byref(q), 3, odd, DATA, 4, pos, 1, DATA, 4, None), "indices", "aligned")
+
+
+def test_a_table_trainer_has_no_checkpoints(tmp_path):
+    trainer = type("Trainer", (), {"sh_table": None})()
+    torch.save({"format": "gs3d-checkpoint-1"}, tmp_path / "c.pt")
+    with pytest.raises(ValueError, match="shared table"):
+        io.load_checkpoint(tmp_path / "c.pt", trainer)
+    with pytest.raises(ValueError, match="shared table"):
+        io.save_checkpoint(tmp_path / "d.pt", trainer)
+
+
 def test_render_refusals():
     cam, til, opt = _abi.Camera(), _abi.TilingC(), _abi.RenderOptionsC()
     out, buf = _abi.RenderOutputsC(), _abi.RenderBuffersC()

@@ -514,6 +514,7 @@ int check_mx4(const gs3d_mx4_rows* q, const char* what) {
     if (q->format != GS3D_NVFP4 && q->format != GS3D_MXFP4) return invalid("%s: format %d", what, q->format);
     if (q->rows > 0 && (!q->codes || !q->scales)) return invalid("%s: NULL codes or scales", what);
     if (q->format == GS3D_NVFP4 && !q->tensor_scale) return invalid("%s: NULL tensor scale", what);
+    if (q->format == GS3D_NVFP4) GS3D_RETURN_IF(check_words(q->tensor_scale, "tensor scale"));
     return GS3D_OK;
 }
 
@@ -584,6 +585,7 @@ int check_mx4_sh(const gs3d_mx4_rows* sh, const int32_t* indices, int64_t n, int
         return invalid("SH degree %d (storage %d)", sh_degree, degree);
     if (!indices && sh->rows < n)
         return invalid("%lld 4-bit SH rows for %lld Gaussians", (long long)sh->rows, (long long)n);
+    GS3D_RETURN_IF(check_words(indices, "indices"));
     return GS3D_OK;
 }
 
@@ -597,6 +599,7 @@ GS3D_API int gs3d_mx4_tensor_scale(const gs3d_rows* x, float* tensor_scale, gs3d
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     GS3D_RETURN_IF(check_rows(x, "rows"));
     if (!tensor_scale) return invalid("NULL tensor scale");
+    GS3D_RETURN_IF(check_words(tensor_scale, "tensor scale"));
     ProfScope prof("mx4_quantise", stream);
     return dispatch_type(x->type, [&](auto t) {
         return launch_tensor_scale<typename decltype(t)::T>(x, tensor_scale, stream);

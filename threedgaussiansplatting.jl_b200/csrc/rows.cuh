@@ -34,6 +34,12 @@ inline int row_elem_bytes(int type) { return type == GS3D_F32 ? 4 : 2; }
 constexpr int64_t kMaxRows = (int64_t)1 << 30;  // row counts and indices stay within int32
 constexpr int kMaxRowDim = 1 << 16;
 
+// int32 and fp32 arrays: aligned to their elements.
+inline int check_words(const void* p, const char* what) {
+    if (reinterpret_cast<uintptr_t>(p) & 3) return invalid("%s not 4-byte aligned", what);
+    return GS3D_OK;
+}
+
 inline int check_rows(const gs3d_rows* r, const char* what) {
     if (!r) return invalid("NULL %s", what);
     if (r->rows < 0 || r->rows > kMaxRows) return invalid("%s: %lld rows", what, (long long)r->rows);

@@ -821,6 +821,7 @@ GS3D_API int gs3d_table_lookup(const gs3d_rows* table, const int32_t* indices, f
     if (table->dim != out->dim) return invalid("table dim %d, output dim %d", table->dim, out->dim);
     if (out->rows == 0) return GS3D_OK;
     if (!indices) return invalid("NULL indices");
+    GS3D_RETURN_IF(check_words(indices, "indices"));
     ProfScope prof("table_lookup", stream);
     return dispatch_type(table->type, [&](auto ti) {
         using TI = typename decltype(ti)::T;
@@ -854,6 +855,9 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     if (n_indices < 0 || (!fgidx_to_gidx && n_indices < grads->rows))
         return invalid("%lld indices for %lld rows", (long long)n_indices, (long long)grads->rows);
     if (grads->rows > 0 && !indices && n_indices > 0) return invalid("NULL indices");
+    GS3D_RETURN_IF(check_words(indices, "indices"));
+    GS3D_RETURN_IF(check_words(fgidx_to_gidx, "fgidx_to_gidx"));
+    GS3D_RETURN_IF(check_words(device_counts, "device_counts"));
     if (table_grads->rows == 0) return GS3D_OK;
     const int64_t n = grads->rows;
     const GradLayout L = grad_layout(std::max<int64_t>(n, 1), table_grads->rows, grads->dim);

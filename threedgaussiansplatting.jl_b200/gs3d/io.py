@@ -300,6 +300,8 @@ def load_checkpoint(path, trainer) -> None:
     from . import adc as adc_mod
     from .optimizer import AdamMoments
 
+    if hasattr(trainer, "sh_table"):
+        raise ValueError("checkpoints hold a model with its own SH coefficients, not a shared table")
     state = torch.load(path, map_location="cpu", weights_only=False)
     if state.get("format") != "gs3d-checkpoint-1":
         raise ValueError(f"{path}: not a gs3d checkpoint")

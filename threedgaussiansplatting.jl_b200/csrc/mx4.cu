@@ -43,13 +43,15 @@ __device__ __forceinline__ void take_finite_abs(uint32_t& m, float v) {
 }
 
 // Every block turns its largest magnitude into the scale it asks for (monotone, positive: fp32 bits
-// order like unsigned integers) and the largest one stays; a lone block stores it. WIDE: rows of
-// 16-byte packs, back to back.
+// order like unsigned integers) and the largest one stays; a lone block stores it. A maximum does not
+// depend on the order, so the atomics give equal bits. Bound by reading x: 3M x 48 fp32 104 us (5.5 TB/s).
+// WIDE: rows of 16-byte packs, back to back, eight loads a thread in flight.
 constexpr int kScaleThreads = 512;
 
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kScaleThreads) k_mx4_tensor_scale(const T* __restrict__ x, int64_t rows, int64_t stride,
-                                                          int dim, uint32_t* __restrict__ tensor_scale) {
+__global__ void __launch_bounds__(kScaleThreads) k_mx4_tensor_scale(const T* __restrict__ x, int64_t rows,
+                                                                    int64_t stride, int dim,
+                                                                    uint32_t* __restrict__ tensor_scale) {
     constexpr int N = 16 / (int)sizeof(T);
     __shared__ uint32_t warp_max[kScaleThreads / 32];
     uint32_t m = 0;
@@ -181,8 +183,10 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&v)[Mx4Block<FMT
     return nan ? 0x7fu : byte;
 }
 
-// Rows of whole blocks in 16-byte packs: a block a thread, from the last row to the first, so that
-// what a tensor-scale pass just before has left in L2 is read from there.
+// Rows of whole blocks in 16-byte packs: a block a thread, whose elements, scale and codes stay in its
+// registers; from the last row to the first, so that what a tensor-scale pass just before has left in
+// L2 is read from there. 3M x 48 fp32: 91 us behind that pass (657 MB, 100 us at the copy rate). The scale
+// is known before x is read again: one kernel for both would need all of x on the chip.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) k_mx4_quantise_blocks(const T* __restrict__ x, int64_t blocks, int64_t stride,
                                                              int nb, bool flat, uint8_t* __restrict__ codes,
@@ -213,12 +217,16 @@ __global__ void __launch_bounds__(256) k_mx4_quantise_blocks(const T* __restrict
 }
 
 // Rows of any length (they may end inside a block): a CTA takes `per` rows, which lie back to back, as
-// one range of bytes through shared memory, and hands the codes back the same way.
+// one range of bytes through shared memory, and hands the codes back the same way. 500K x 27 bf16:
+// 12.4 us (35 MB: 5.4): a CTA reads, computes and writes in turn, so small ones that overlap do better
+// (64 / 128 / 256 / 512 threads: 12.4 / 12.4 / 13.7 / 17.9); reading the elements as shifted 32-bit words
+// took 14.5.
+constexpr int kRowsThreads = 128;
+
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) k_mx4_quantise_rows(const T* __restrict__ x, int64_t rows, int dim, int per,
-                                                           uint8_t* __restrict__ codes,
-                                                           uint8_t* __restrict__ scales,
-                                                           const float* __restrict__ tensor_scale) {
+__global__ void __launch_bounds__(kRowsThreads)
+    k_mx4_quantise_rows(const T* __restrict__ x, int64_t rows, int dim, int per, uint8_t* __restrict__ codes,
+                        uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale) {
     constexpr int BS = Mx4Block<FMT>::size;
     extern __shared__ __align__(16) unsigned char smem[];
     const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2;
@@ -279,7 +287,8 @@ __global__ void __launch_bounds__(256) k_mx4_quantise(const T* __restrict__ x, i
 // ---- dequantise ------------------------------------------------------------------------------
 // Rows of whole blocks, back to back: the codes, scales and values of all rows are one run each. A
 // thread fills kDequantisePacks times 16 bytes of output, next to its neighbours' each time; the word of
-// codes that it takes its half (or all) of is read by both.
+// codes that it takes its half (or all) of is read by both. Bound by memory: 3M x 48 fp32 97 us (657 MB,
+// 6.7 TB/s); 139 with one pack a thread, 152 with the packs of a thread side by side.
 constexpr int kDequantisePacks = 4;
 
 template <typename T, int FMT>
@@ -331,13 +340,14 @@ __device__ __forceinline__ uint32_t word_at(const unsigned char* p) {
     return __funnelshift_r(w[0], w[1], 8 * (int)(a & 3));
 }
 
-// Rows of any length, back to back: a CTA takes `per` rows' codes and scales through shared memory, a
-// block of a row a thread, and hands the values back as one range of bytes.
+// Rows of any length, back to back: a CTA takes `per` rows' codes through shared memory, a block of a
+// row a thread, and hands the values back as one range of bytes. 500K x 27 bf16: 10.8 us (5.4 at the
+// copy rate), for the same reason as k_mx4_quantise_rows.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) k_mx4_dequantise_rows(const uint8_t* __restrict__ codes,
-                                                             const uint8_t* __restrict__ scales,
-                                                             const float* __restrict__ tensor_scale, int64_t rows,
-                                                             int dim, int per, T* __restrict__ out) {
+__global__ void __launch_bounds__(kRowsThreads)
+    k_mx4_dequantise_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                          const float* __restrict__ tensor_scale, int64_t rows, int dim, int per,
+                          T* __restrict__ out) {
     constexpr int BS = Mx4Block<FMT>::size;
     extern __shared__ __align__(16) unsigned char smem[];
     const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2;
@@ -394,9 +404,9 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise(const uint8_t* __restric
     }
 }
 
-// Rows a CTA of the *_rows kernels takes: a block for each of its 256 threads, as far as they fit.
+// Rows a CTA of the *_rows kernels takes: a block for each of its threads, as far as they fit.
 int rows_per_cta(int row_bytes, int row_blocks) {
-    return std::max(1, std::min(kRowsBytes / row_bytes, 256 / row_blocks));
+    return std::max(1, std::min(kRowsBytes / row_bytes, kRowsThreads / row_blocks));
 }
 
 template <typename T, int FMT>
@@ -414,7 +424,7 @@ int launch_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t s
         const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
         const size_t smem = ((16 + (size_t)per * dim * sizeof(T) + 15) & ~(size_t)15) + 16 +
                             (size_t)per * mx4_code_bytes(dim) + 16;
-        k_mx4_quantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), 256, smem, stream>>>(
+        k_mx4_quantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), kRowsThreads, smem, stream>>>(
             in, x->rows, dim, per, out->codes, out->scales, out->tensor_scale);
     } else {
         k_mx4_quantise<T, FMT><<<grid_for(blocks, 256, 8), 256, 0, stream>>>(
@@ -439,7 +449,7 @@ int launch_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, cudaStream_t
         const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
         const size_t smem = ((16 + (size_t)per * mx4_code_bytes(dim) + 15) & ~(size_t)15) + 16 +
                             (size_t)per * dim * sizeof(T) + 16 + 16;  // and what word_at reads behind the codes
-        k_mx4_dequantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), 256, smem, stream>>>(
+        k_mx4_dequantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), kRowsThreads, smem, stream>>>(
             x->codes, x->scales, x->tensor_scale, x->rows, dim, per, o);
     } else {
         k_mx4_dequantise<T, FMT><<<grid_for(x->rows * dim, 256, 8), 256, 0, stream>>>(
@@ -473,10 +483,18 @@ struct Positions {
 // Gaussians i and i + 32 of a warp's 64 a thread (neighbouring lanes load and store neighbouring rows),
 // their operations in packed pairs. ONE: a single view; else `views` of them a block, with the elements
 // decoded once.
+// Bound by instruction issue with one view (3M at degree 3: 33 us, 27 for the bytes; 74 % of the issue slots
+// used, of some 520 instructions a pair 180 decode), by the stores with several (500K at degree 2, 8 views:
+// 17 us, 11.5 for the bytes).
+// Blocks an SM: a single view in whole rows holds one channel at a time, 72 registers and 7 blocks (33.4 us;
+// 35.5 left to the compiler); several views hold all elements of both Gaussians, 3 blocks at degree 3.
+template <int DEG, bool WHOLE, bool ONE>
+constexpr int colour_blocks() { return ONE && WHOLE ? 7 : (DEG == 3 ? 3 : 5); }
+
 template <int DEG, int FMT, bool WHOLE, bool ONE>
-__global__ void __launch_bounds__(128, ONE && WHOLE ? 7 : (DEG == 3 ? 3 : 5)) k_mx4_colours(const Mx4Sh a, int order, const float4* __restrict__ mo4,
-                                                     int n, const Positions cv, int nv, int views,
-                                                     float4* __restrict__ out, int64_t view_stride) {
+__global__ void __launch_bounds__(128, colour_blocks<DEG, WHOLE, ONE>())
+    k_mx4_colours(const Mx4Sh a, int order, const float4* __restrict__ mo4, int n, const Positions cv, int nv, int views,
+                  float4* __restrict__ out, int64_t view_stride) {
     constexpr int NC = (DEG + 1) * (DEG + 1);
     const int64_t i = (int64_t)blockIdx.x * 256 + (threadIdx.x >> 5) * 64 + (threadIdx.x & 31);
     if (i >= n) return;

@@ -1,5 +1,6 @@
 // sh_colour.cuh — a Gaussian's colour from its SH coefficients (sh_coeffs_to_color, sh.jl:38-112),
-// shared by every kernel that computes colours so that they agree bit for bit.
+// shared by every kernel that computes colours from fp32 coefficients so that they agree bit for bit; and
+// the SH basis with fused multiply-adds, of the colours from 4-bit rows.
 #pragma once
 #include "common.cuh"
 

@@ -18,7 +18,8 @@ namespace {
 // is 16 bytes of the wider of table and output (two half types: of both) where all rows are so aligned
 // (3M x 48 fp32 with 1 / 2 / 4 / 8 rows: 129 / 103 / 94 / 117 us; a write-only fill of as much: 79). Else it
 // is one element, and a thread takes COLS of a row, a share of the columns apart, for one index and one
-// address (500K x 27 bf16: 17.1 us with one column, 15.3 with two; bound by the instructions).
+// address (500K x 27 bf16: 17.1 us with one column, 15.0 with two, 21 with the output's 32-bit words, whose
+// halves come from two words of the table where the rows' parities differ; bound by the instructions).
 constexpr int kLookupRows = 4, kLookupColumns = 2;
 
 template <typename T, int N>

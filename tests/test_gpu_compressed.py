@@ -31,7 +31,8 @@ def make_indices(n, rows, gen, skew=0.0, invalid=True):
 
 # -- lookup -----------------------------------------------------------------------------------
 LOOKUP_SHAPES = [(1, 1, 1), (1, 5, 48), (7, 1, 3), (33, 4, 27), (1000, 64, 48), (1001, 300, 12), (257, 9, 130),
-                 (64, 3, 1021), (5, 2, 65536), (20_003, 5000, 48)]
+                 (64, 3, 1021), (5, 2, 65536), (20_003, 5000, 48), (700, 50, 2), (700, 50, 4), (700, 50, 6), (701, 9, 54),
+             (300, 9, 514)]
 
 
 def lookup_exact(table, idx, scale, dtype):
@@ -57,7 +58,8 @@ def test_lookup(cuda, n, rows, dim, kind, out_kind):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("dim,table_stride,out_stride,offset", [(48, 48, 60, 0), (48, 64, 48, 0), (27, 31, 29, 1),
-                                                               (48, 52, 50, 3), (3, 4, 4, 1), (16, 17, 19, 0)])
+                                                               (48, 52, 50, 3), (3, 4, 4, 1), (16, 17, 19, 0),
+                                                               (20, 20, 20, 4), (20, 22, 24, 2), (54, 56, 54, 2)])
 def test_lookup_strides(cuda, kind, dim, table_stride, out_stride, offset):
     """Row strides and starts of every alignment; what lies between the rows stays as it was."""
     gen = rng(5)
@@ -126,6 +128,37 @@ def test_gradient(cuda, n, rows, dim, skew, kind):
     want, bound = gradient_exact(grads, idx, rows, 1.3)
     assert got.dtype == torch.float32 and got.shape == want.shape
     assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n", [900, 3000, 20_001])
+@pytest.mark.parametrize("dim,stride,offset", [(2, 2, 0), (4, 4, 0), (6, 6, 0), (8, 8, 2), (12, 12, 0), (12, 16, 4), (20, 22, 0),
+                                               (42, 42, 0), (42, 43, 1), (106, 106, 0), (254, 254, 0), (516, 516, 0)])
+@pytest.mark.parametrize("kind", TYPES)
+def test_gradient_units(cuda, n, dim, stride, offset, kind):
+    """Rows that are read 2, 4, 8 and 16 bytes at a time, by every path of the sizes."""
+    gen = rng(n + dim)
+    rows = 33
+    buf = torch.randn(n * stride + offset, generator=gen).to(kind).to(cuda)
+    grads = torch.as_strided(buf, (n, dim), (stride, 1), offset)
+    idx = make_indices(n, rows, gen, 1.0)
+    got = gc.table_gradient(grads, idx.to(cuda), rows, scale=-0.7)
+    want, bound = gradient_exact(grads.cpu(), idx, rows, -0.7)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n,dim", [(700_000, 119), (500_000, 260), (300_000, 1)])
+def test_gradient_of_long_runs(cuda, n, dim):
+    """Few rows used by very many: runs over hundreds and thousands of chunks, beside short ones."""
+    gen = rng(n)
+    grads = torch.randn(n, dim, generator=gen).to(torch.bfloat16)
+    idx = torch.full((n,), 4, dtype=torch.int32)
+    idx[::1000] = (torch.arange(n)[::1000] % 3).to(torch.int32) + 1
+    idx[n // 3 : n // 2] = 5
+    idx[:70] = 6
+    got = gc.table_gradient(grads.to(cuda), idx.to(cuda), 7)
+    want, bound = gradient_exact(grads, idx, 7, 1.0)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+    assert torch.equal(gc.table_gradient(grads.to(cuda), idx.to(cuda), 7), got)
 
 
 @pytest.mark.parametrize("n", [1023, 1024, 1025, 4095, 4096, 4097, 8193])
@@ -307,7 +340,8 @@ def quantise_exact(x, fmt, g):
     return codes[:, : (dim + 1) // 2], byte, val, nan
 
 
-MX_SHAPES = [(1, 1), (1, 48), (5, 3), (33, 27), (1000, 48), (257, 12), (64, 130), (7, 1021), (2, 65535), (10_001, 48)]
+MX_SHAPES = [(1, 1), (1, 48), (5, 3), (33, 27), (1000, 48), (257, 12), (64, 130), (7, 1021), (2, 65535), (10_001, 48),
+             (1031, 4), (515, 8), (777, 20), (130, 92), (301, 44), (99, 16), (65, 17), (1025, 2), (37, 72), (3, 4100)]
 
 
 def mx_input(n, dim, kind, gen, spread):
@@ -420,7 +454,8 @@ def test_quantise_largest_and_smallest(cuda, fmt, dim):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("dim,stride,offset", [(48, 64, 0), (48, 49, 1), (27, 31, 3), (16, 24, 8)])
+@pytest.mark.parametrize("dim,stride,offset", [(48, 64, 0), (48, 49, 1), (27, 31, 3), (16, 24, 8), (12, 16, 4), (92, 92, 4),
+                                               (40, 48, 0), (4, 4, 4), (48, 48, 2), (64, 72, 0)])
 def test_quantise_strides(cuda, kind, dim, stride, offset):
     gen = rng(4)
     n = 333

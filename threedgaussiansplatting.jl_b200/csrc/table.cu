@@ -15,11 +15,12 @@ namespace {
 // ---- lookup ----------------------------------------------------------------------------------
 // out[i] = table[indices[i] - 1] * scale. Bound by the rows written (the table stays in L2). Threads side
 // by side on a row's units of N elements, ROWS rows a thread, as many independent loads in flight. A unit
-// is 16 bytes of the wider of table and output (two half types: of both) where all rows are so aligned
-// (3M x 48 fp32 with 1 / 2 / 4 / 8 rows: 129 / 103 / 94 / 117 us; a write-only fill of as much: 79). Else it
-// is one element, and a thread takes COLS of a row, a share of the columns apart, for one index and one
-// address (500K x 27 bf16: 17.1 us with one column, 15.0 with two, 21 with the output's 32-bit words, whose
-// halves come from two words of the table where the rows' parities differ; bound by the instructions).
+// is 16 bytes of the wider of table and output (two half types: of both), or less as the rows' lengths and
+// starts allow (3M x 48 fp32 with 1 / 2 / 4 / 8 rows: 129 / 103 / 94 / 117 us; a write-only fill of as much: 79).
+// Of units of one or two elements a thread takes COLS of a row, a share of the columns apart, for one
+// index and one address (500K x 27 bf16: 17.1 us with one column, 15.0 with two, 19.8 with four; 1M x 54
+// bf16 by pairs: 40.0, 35.9): bound by the instructions. Odd rows by the output's 32-bit words, whose halves
+// come from two words of the table where the rows' parities differ, took 21 us.
 constexpr int kLookupRows = 4, kLookupColumns = 2;
 
 template <typename T, int N>
@@ -27,15 +28,17 @@ struct alignas(N * sizeof(T)) Pack {
     T e[N];
 };
 
-// A pack of 8 or 16 bytes to memory that is not read again soon: streamed, so that it does not push
+template <size_t BYTES>
+using PackWord = typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2, uint32_t>::type>::type;
+
+// A pack to memory that is not read again soon: streamed, so that it does not push
 // the table out of L2 (104 us without, 94 with). Single elements go the ordinary way: L2 joins them.
 template <typename T, int N>
 __device__ __forceinline__ void store_streaming(T* p, const Pack<T, N>& v) {
     if constexpr (N == 1) {
         *p = v.e[0];
     } else {
-        using W = typename std::conditional<sizeof(v) == 16, uint4, uint2>::type;
-        static_assert(sizeof(v) == sizeof(W), "packs of 8 or 16 bytes");
+        using W = PackWord<sizeof(v)>;
         __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&v));
     }
 }
@@ -45,14 +48,11 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
     if constexpr (N == 1) {
         return Pack<T, N>{__ldg(p)};
     } else {
-        using W = typename std::conditional<sizeof(Pack<T, N>) == 16, uint4, uint2>::type;
+        using W = PackWord<sizeof(Pack<T, N>)>;
         const W w = __ldg(reinterpret_cast<const W*>(p));
         return *reinterpret_cast<const Pack<T, N>*>(&w);
     }
 }
-
-template <typename TI, typename TO>
-constexpr int lookup_pack() { return sizeof(TI) == 2 && sizeof(TO) == 2 ? 8 : 4; }
 
 template <typename TI, typename TO, int N, int ROWS, int COLS>
 __global__ void __launch_bounds__(256) k_table_lookup(const TI* __restrict__ table, int rows, int table_stride,
@@ -121,9 +121,13 @@ int launch_lookup_units(const gs3d_rows* table, const int32_t* indices, float sc
 template <typename TI, typename TO>
 int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, const gs3d_rows* out,
                   cudaStream_t stream) {
-    constexpr int N = lookup_pack<TI, TO>();
-    if (packs<TI>(table, N) && packs<TO>(out, N))
-        return launch_lookup_units<TI, TO, N, kLookupRows, 1>(table, indices, scale, out, stream);
+    if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2)
+        if (packs<TI>(table, 8) && packs<TO>(out, 8))
+            return launch_lookup_units<TI, TO, 8, kLookupRows, 1>(table, indices, scale, out, stream);
+    if (packs<TI>(table, 4) && packs<TO>(out, 4))
+        return launch_lookup_units<TI, TO, 4, kLookupRows, 1>(table, indices, scale, out, stream);
+    if (packs<TI>(table, 2) && packs<TO>(out, 2))
+        return launch_lookup_units<TI, TO, 2, kLookupRows, kLookupColumns>(table, indices, scale, out, stream);
     return launch_lookup_units<TI, TO, 1, kLookupRows, kLookupColumns>(table, indices, scale, out, stream);
 }
 
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource sr
 template <typename T, int VB>
 struct RowUnit {
     static constexpr int N = VB / (int)sizeof(T);
-    T e[N];
+    alignas(VB) T e[N];
     __device__ __forceinline__ void load(const T* p) {
         // a row is read once, from a place of its own: nothing for L1, and 64 bytes a DRAM access
         // (a 3M x 192 B gather alone: 117 us plain, 107 us so)
@@ -501,6 +505,12 @@ struct RowUnit {
                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                 : "l"(p));
             *reinterpret_cast<uint4*>(e) = v;
+        } else if constexpr (VB == 8) {
+            uint2 v;
+            asm("ld.global.nc.L1::no_allocate.L2::64B.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+            *reinterpret_cast<uint2*>(e) = v;
+        } else if constexpr (VB == 4 && sizeof(T) == 2) {
+            *reinterpret_cast<uint32_t*>(e) = __ldg(reinterpret_cast<const uint32_t*>(p));
         } else {
             e[0] = __ldg(p);
         }
@@ -545,7 +555,9 @@ __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int strid
                                           int run, const Segments& g, const int2* items, int count, float* part,
                                           bool open_left, bool open_right, float* __restrict__ partial) {
     using Unit = RowUnit<T, VB>;
-    constexpr int N = Unit::N, AHEAD = VB == 16 ? 6 : 8;  // rows in flight a slot
+    // rows in flight a slot (1.2M x 119 bf16, an element a thread: 8 / 12 / 16 rows 53 / 46 / 41 us; 1M x 27
+    // fp32: 54 / 55 / 58)
+    constexpr int N = Unit::N, AHEAD = VB == 16 ? 6 : (VB < 8 && sizeof(T) == 2 ? 16 : 8);
     const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
     const int unit = blockIdx.y * pl.tile_units + lane;
     const int col = unit * N;
@@ -696,56 +708,53 @@ __global__ void __launch_bounds__(kTinyThreads) k_table_gradient_tiny(const T* _
 }
 
 // A warp per chunk for the runs of up to 32 partial sums behind the first (nearly all: an average run is
-// shorter than a chunk), the whole block for the longer ones it meets.
-constexpr int kJoinWarps = 8;
+// shorter than a chunk), 32 columns each; the whole block for a longer one, of which at most one starts in
+// a block's chunks (the chunks that it covers own none), its warps 32 partial sums apart.
+constexpr int kJoinWarps = 32;
 
 __global__ void __launch_bounds__(32 * kJoinWarps) k_table_join(int dim, int nchunks, const Segments g) {
-    __shared__ int long_run[kJoinWarps];
-    __shared__ float part[32 * kJoinWarps];
+    __shared__ int long_run[2];  // its first chunk, its key
+    __shared__ float part[kJoinWarps][32];
     after_predecessor();
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.x * kJoinWarps + w;
+    const int b = blockIdx.x * kJoinWarps + w, col = blockIdx.y * 32 + lane;
+    const bool on = col < dim;
     const int k = b < nchunks ? g.owned[b] : -1;
     const int next = b + 1 + lane;
     const unsigned same = __ballot_sync(0xffffffffu, k >= 0 && next < nchunks && g.first_key[next] == k);
-    if (lane == 0) long_run[w] = same == 0xffffffffu ? k : -1;
-    if (k >= 0 && same != 0xffffffffu) {
+    if (threadIdx.x == 0) long_run[0] = -1;
+    __syncthreads();
+    if (same == 0xffffffffu) {
+        if (lane == 0) long_run[0] = b, long_run[1] = k;
+    } else if (k >= 0 && on) {
         const int more = __ffs(~same) - 1;
-        for (int col = blockIdx.y * 256 + lane; col < min(dim, (int)blockIdx.y * 256 + 256); col += 32) {
-            float s = g.partial[((int64_t)b * 2 + 1) * dim + col];
+        float s = g.partial[((int64_t)b * 2 + 1) * dim + col];
 #pragma unroll 4
-            for (int c = 1; c <= more; ++c) s += g.partial[(int64_t)(b + c) * 2 * dim + col];
-            const float one[1] = {s};
-            store_row<1>(g, k, col, one);
-        }
+        for (int c = 1; c <= more; ++c) s += g.partial[(int64_t)(b + c) * 2 * dim + col];
+        const float one[1] = {s};
+        store_row<1>(g, k, col, one);
     }
     __syncthreads();
-    const int width = min(dim, 256), slots = 256 / width;
-    const int slot = threadIdx.x / width, col = blockIdx.y * 256 + threadIdx.x - slot * width;
-    const bool on = slot < slots && col < dim;
-    for (int q = 0; q < kJoinWarps; ++q) {
-        const int lk = long_run[q];
-        if (lk < 0) continue;
-        const int lb = blockIdx.x * kJoinWarps + q;
-        int end = lb + 1;  // the run's last chunk is end - 1
-        for (int more = 32 * kJoinWarps; more == 32 * kJoinWarps; end += more) {
-            const int c = end + threadIdx.x;
-            more = __syncthreads_count(c < nchunks && g.first_key[c] == lk);
-        }
-        float s = 0.0f;
-        if (on) {
-            if (slot == 0) s = g.partial[((int64_t)lb * 2 + 1) * dim + col];
+    const int lb = long_run[0], lk = long_run[1];
+    if (lb < 0) return;
+    int end = lb + 1;  // the run's last chunk is end - 1
+    for (int more = 32 * kJoinWarps; more == 32 * kJoinWarps; end += more) {
+        const int c = end + threadIdx.x;
+        more = __syncthreads_count(c < nchunks && g.first_key[c] == lk);
+    }
+    float s = 0.0f;
+    if (on) {
+        if (w == 0) s = g.partial[((int64_t)lb * 2 + 1) * dim + col];
 #pragma unroll 8
-            for (int c = lb + 1 + slot; c < end; c += slots) s += g.partial[(int64_t)c * 2 * dim + col];
-        }
-        part[threadIdx.x] = s;
-        __syncthreads();
-        if (slot == 0 && on) {
-            for (int t = 1; t < slots; ++t) s += part[t * width + threadIdx.x];
-            const float one[1] = {s};
-            store_row<1>(g, lk, col, one);
-        }
-        __syncthreads();
+        for (int c = lb + 1 + w; c < end; c += kJoinWarps) s += g.partial[(int64_t)c * 2 * dim + col];
+    }
+    part[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && on) {
+#pragma unroll 8
+        for (int t = 1; t < kJoinWarps; ++t) s += part[t][lane];
+        const float one[1] = {s};
+        store_row<1>(g, lk, col, one);
     }
 }
 
@@ -754,13 +763,29 @@ struct GradLayout {
     int ntiles, passes, bits, chunks_max;
 };
 
-// Rows a slot adds: enough blocks for few rows, few borders for many (3M: 32 / 48 / 96 rows 197 / 194 / 196 us;
-// 500K: 39.6 / 37.4 / 41.5).
-constexpr int kMinRun = 4, kMaxRun = 48;
+// Rows a slot adds: enough blocks for few rows, few borders for many (3M x 48 fp32: 32 / 48 / 96 rows 197 /
+// 194 / 196 us; 500K x 27 bf16: 39.6 / 37.4 / 41.5), and more for long rows, of which a block has few
+// slots, so that some 16 chunks an SM are left to join (1.2M x 119 bf16, 52 rows of which few are much
+// used: 198 us in all with 48 rows a slot and a join of 256 columns a block, 67 so).
+constexpr int kMinRun = 4, kMaxRun = 48, kMaxChunk = 2048;
 
-// Rows that can be read 16 bytes at a time.
+// Bytes of a row that a thread reads at once: 16 where the rows allow it, else 8, 4 or an element.
 template <typename T>
-bool wide_rows(const gs3d_rows* r) { return packs<T>(r, 16 / (int)sizeof(T)); }
+int unit_bytes(const gs3d_rows* r) {
+    for (int b = 16; b > (int)sizeof(T); b /= 2)
+        if (packs<T>(r, b / (int)sizeof(T))) return b;
+    return (int)sizeof(T);
+}
+
+template <typename T, typename F>
+int dispatch_unit(int bytes, F&& f) {
+    switch (bytes) {
+        case 16: return f(std::integral_constant<int, 16>{});
+        case 8: return f(std::integral_constant<int, 8>{});
+        case 4: return f(std::integral_constant<int, 4>{});
+        default: return f(std::integral_constant<int, (int)sizeof(T)>{});
+    }
+}
 
 int slots_for(int tile_units) { return std::max(1, std::min(32, 256 / tile_units)); }
 
@@ -769,8 +794,9 @@ SegmentPlan segment_plan(int64_t n, int units) {
     p.units = units;
     p.tile_units = std::min(units, 256);
     p.slots = slots_for(p.tile_units);
-    const int64_t want = ceil_div(n, (int64_t)p.slots * kSMs * 4);
-    p.run = (int)std::max<int64_t>(kMinRun, std::min<int64_t>(kMaxRun, want));
+    const int64_t want = ceil_div(n, (int64_t)p.slots * kSMs * 4), most = ceil_div(n, (int64_t)p.slots * kSMs * 16);
+    const int64_t run = std::max(most, std::max<int64_t>(kMinRun, std::min<int64_t>(kMaxRun, want)));
+    p.run = (int)std::min<int64_t>(run, kMaxChunk / p.slots);
     p.chunk = p.slots * p.run;
     p.nchunks = (int)std::max<int64_t>(1, ceil_div(n, p.chunk));
     return p;
@@ -878,8 +904,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
         return dispatch_type(grads->type, [&](auto t) {
             using T = typename decltype(t)::T;
             const T* g = static_cast<const T*>(grads->data);
-            const bool wide = wide_rows<T>(grads);
-            const int per = wide ? 16 / (int)sizeof(T) : 1;
+            const int bytes = unit_bytes<T>(grads), per = bytes / (int)sizeof(T);
             const SegmentPlan pl = segment_plan(n, grads->dim / per);
             const Segments seg{nullptr, nullptr, out, table_grads->row_stride, scale, accumulate ? 1 : 0, nullptr,
                                nullptr, nullptr};
@@ -889,10 +914,12 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
             const int blocks =
                 (int)std::max<int64_t>(ceil_div(n, 32), std::min<int64_t>(ceil_div(zeroed, 1 << 14), kSMs));
             const dim3 grid(blocks, (unsigned)ceil_div(pl.units, pl.tile_units));
-            const auto kernel = wide ? k_table_gradient_tiny<T, 16> : k_table_gradient_tiny<T, (int)sizeof(T)>;
-            kernel<<<grid, kTinyThreads, smem, stream>>>(g, (int)grads->row_stride, grads->dim, pl, seg, src, zero, L.bits);
-            GS3D_LAUNCHED("k_table_gradient_tiny");
-            return GS3D_OK;
+            return dispatch_unit<T>(bytes, [&](auto vb) {
+                k_table_gradient_tiny<T, decltype(vb)::value><<<grid, kTinyThreads, smem, stream>>>(
+                    g, (int)grads->row_stride, grads->dim, pl, seg, src, zero, L.bits);
+                GS3D_LAUNCHED("k_table_gradient_tiny");
+                return GS3D_OK;
+            });
         });
     int sorted = 0;
     if (n <= kSortTile) {
@@ -930,17 +957,18 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     return dispatch_type(grads->type, [&](auto t) {
         using T = typename decltype(t)::T;
         const T* g = static_cast<const T*>(grads->data);
-        const bool wide = wide_rows<T>(grads);
-        const int per = wide ? 16 / (int)sizeof(T) : 1;
+        const int bytes = unit_bytes<T>(grads), per = bytes / (int)sizeof(T);
         const SegmentPlan pl = segment_plan(n, grads->dim / per);
         const size_t smem = (size_t)pl.chunk * 8 + (size_t)pl.slots * pl.tile_units * per * 4;
         const dim3 grid(pl.nchunks, (unsigned)ceil_div(pl.units, pl.tile_units));
         const int threads = pl.slots * pl.tile_units;
         const int stride = (int)grads->row_stride;
-        const auto kernel = wide ? k_table_segments<T, 16> : k_table_segments<T, (int)sizeof(T)>;
-        GS3D_RETURN_IF(launch_after("k_table_segments", kernel, grid, threads, smem, stream, g, stride, grads->dim, pl, seg));
+        GS3D_RETURN_IF(dispatch_unit<T>(bytes, [&](auto vb) {
+            return launch_after("k_table_segments", k_table_segments<T, decltype(vb)::value>, grid, threads, smem, stream, g,
+                                stride, grads->dim, pl, seg);
+        }));
         GS3D_RETURN_IF(launch_after("k_table_join", k_table_join,
-                                    dim3((unsigned)ceil_div(pl.nchunks, kJoinWarps), (unsigned)ceil_div(grads->dim, 256)),
+                                    dim3((unsigned)ceil_div(pl.nchunks, kJoinWarps), (unsigned)ceil_div(grads->dim, 32)),
                                     32 * kJoinWarps, 0, stream, (int)grads->dim, pl.nchunks, seg));
         return GS3D_OK;
     });

@@ -26,6 +26,13 @@
 namespace gs3d {
 namespace {
 
+// Rows that consist of packs of BYTES bytes.
+template <typename T, int BYTES>
+bool packs_of(const gs3d_rows* r) {
+    constexpr int n = BYTES / (int)sizeof(T);
+    return r->dim % n == 0 && r->row_stride % n == 0 && reinterpret_cast<uintptr_t>(r->data) % BYTES == 0;
+}
+
 int grid_for(int64_t items, int threads, int per_sm) {
     const int64_t b = std::min<int64_t>(ceil_div(items, threads), (int64_t)device_sm_count() * per_sm);
     return (int)std::max<int64_t>(b, 1);
@@ -34,6 +41,17 @@ int grid_for(int64_t items, int threads, int per_sm) {
 template <typename T, int N>
 struct alignas(N * sizeof(T)) Pack {
     T e[N];
+};
+
+// Quotients of numbers below 2^31 by a divisor that the host knows (Granlund and Montgomery 1994).
+struct FastDiv {
+    uint32_t d, m;
+    int s;
+    explicit FastDiv(uint32_t divisor) : d(divisor), s(0) {
+        while (((uint64_t)1 << s) < d) ++s;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
 };
 
 // ---- tensor scale ----------------------------------------------------------------------------
@@ -144,22 +162,20 @@ struct TensorScale {
     }
 };
 
-// A block's scale byte and the codes of its elements v (zeros behind the row's end), two a byte,
-// in words of eight.
-template <int FMT>
-__device__ __forceinline__ uint32_t quantise_block(const float (&v)[Mx4Block<FMT>::size], const TensorScale& t,
-                                                   uint32_t (&words)[Mx4Block<FMT>::size / 8]) {
-    constexpr int BS = Mx4Block<FMT>::size;
+// A block's scale byte and the codes of its first EL elements v (zeros behind the row's end), two a byte,
+// in words of eight. EL < block size: rows of at most EL elements.
+template <int FMT, int EL>
+__device__ __forceinline__ uint32_t quantise_block(const float (&v)[EL], const TensorScale& t, uint32_t (&words)[EL / 8]) {
     uint32_t top = 0;  // magnitudes order like unsigned integers, infinity and NaN above all
 #pragma unroll
-    for (int k = 0; k < BS; ++k) top = max(top, f2u(v[k]) & 0x7fffffffu);
+    for (int k = 0; k < EL; ++k) top = max(top, f2u(v[k]) & 0x7fffffffu);
     const bool nan = top > 0x7f800000u;
     const float a = u2f(top);
     if (FMT == GS3D_MXFP4) {
         const uint32_t byte = mxfp4_scale_byte(a);
         const float inv = u2f((254u - byte) << 23);  // 2^(127 - byte), byte <= 253
 #pragma unroll
-        for (int w = 0; w < BS / 8; ++w) words[w] = e2m1_word(v + 8 * w, inv);
+        for (int w = 0; w < EL / 8; ++w) words[w] = e2m1_word(v + 8 * w, inv);
         return nan ? 0xffu : byte;
     }
     const uint32_t byte = nvfp4_scale_byte(a, t.g, t.inv6g);
@@ -168,13 +184,13 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&v)[Mx4Block<FMT
     const float lo = inv * (1.0f - 0x1p-21f), hi = inv * (1.0f + 0x1p-21f);
     uint32_t differ = 0;
 #pragma unroll
-    for (int w = 0; w < BS / 8; ++w) {
+    for (int w = 0; w < EL / 8; ++w) {
         words[w] = e2m1_word(v + 8 * w, lo);
         differ |= words[w] ^ e2m1_word(v + 8 * w, hi);
     }
     if (differ && s > 0.0f) {
 #pragma unroll
-        for (int w = 0; w < BS / 8; ++w) {
+        for (int w = 0; w < EL / 8; ++w) {
             words[w] = 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) words[w] |= e2m1_code_exact(v[8 * w + k], s, t.g) << (4 * k);
@@ -183,54 +199,76 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&v)[Mx4Block<FMT
     return nan ? 0x7fu : byte;
 }
 
-// Rows of whole blocks in 16-byte packs: a block a thread, whose elements, scale and codes stay in its
-// registers; from the last row to the first, so that what a tensor-scale pass just before has left in
-// L2 is read from there. 3M x 48 fp32: 91 us behind that pass (657 MB, 100 us at the copy rate). The scale
-// is known before x is read again: one kernel for both would need all of x on the chip.
-template <typename T, int FMT>
-__global__ void __launch_bounds__(256) k_mx4_quantise_blocks(const T* __restrict__ x, int64_t blocks, int64_t stride,
-                                                             int nb, bool flat, uint8_t* __restrict__ codes,
-                                                             uint8_t* __restrict__ scales,
-                                                             const float* __restrict__ tensor_scale) {
-    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T);
+// Rows in packs of N elements (16 bytes, or four): a block a thread, whose elements, scale and codes stay in its registers; from the
+// last row to the first, so that what a tensor-scale pass just before has left in L2 is read from there.
+// 3M x 48 fp32 in NVFP4: 91 us behind that pass (657 MB, 100 us at the rate of a plain copy). The scale is
+// known before x is read again: one kernel for both would need all of x on the chip. WHOLE: rows of whole
+// blocks, the codes stored a block at a time; else in words, or in halves of them (2.6M x 48 fp32 in MXFP4,
+// whose last block is half: 98 us, through shared memory 339).
+template <typename T, int FMT, int EL, int N, bool WHOLE>
+__global__ void __launch_bounds__(256)
+    k_mx4_quantise_blocks(const T* __restrict__ x, int64_t blocks, int64_t stride, int dim, const FastDiv nb, bool flat,
+                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                          const float* __restrict__ tensor_scale) {
+    constexpr int BS = Mx4Block<FMT>::size;
     const int64_t i = (int64_t)(gridDim.x - 1 - blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= blocks) return;
     const TensorScale t = TensorScale::load<FMT>(tensor_scale);
     const T* xb = x + i * BS;
-    if (!flat) {
-        const int64_t r = i / nb;
-        xb = x + r * stride + (i - r * nb) * BS;
+    int64_t r = 0;
+    int b = 0, len = BS;
+    if (!WHOLE || !flat) {
+        r = i < INT_MAX ? (int64_t)nb.quotient((uint32_t)i) : i / nb.d;
+        b = (int)(i - r * nb.d);
+        xb = x + r * stride + b * BS;
+        if (!WHOLE) len = min(BS, dim - b * BS);
     }
-    float v[BS];
+    float v[EL];
 #pragma unroll
-    for (int k = 0; k < BS; k += N) {
-        const Pack<T, N> p = *reinterpret_cast<const Pack<T, N>*>(xb + k);
+    for (int k = 0; k < EL; k += N) {
+        Pack<T, N> p{};
+        if (WHOLE || k < len) p = *reinterpret_cast<const Pack<T, N>*>(xb + k);
 #pragma unroll
         for (int c = 0; c < N; ++c) v[k + c] = to_f32(p.e[c]);
     }
-    uint32_t words[BS / 8];
+    uint32_t words[EL / 8];
     scales[i] = (uint8_t)quantise_block<FMT>(v, t, words);
-    Pack<uint32_t, BS / 8> o;
+    if constexpr (WHOLE) {
+        Pack<uint32_t, BS / 8> o;
 #pragma unroll
-    for (int w = 0; w < BS / 8; ++w) o.e[w] = words[w];
-    *reinterpret_cast<Pack<uint32_t, BS / 8>*>(codes + i * (BS / 2)) = o;
+        for (int w = 0; w < BS / 8; ++w) o.e[w] = words[w];
+        *reinterpret_cast<Pack<uint32_t, BS / 8>*>(codes + i * (BS / 2)) = o;
+    } else {
+        uint8_t* c = codes + r * (dim / 2) + b * (BS / 2);
+        if (dim % 8 == 0) {
+#pragma unroll
+            for (int w = 0; w < EL / 8; ++w)
+                if (8 * w < len) reinterpret_cast<uint32_t*>(c)[w] = words[w];
+        } else {  // 4 more than a multiple of 8
+#pragma unroll
+            for (int h = 0; h < EL / 4; ++h)
+                if (4 * h < len) reinterpret_cast<uint16_t*>(c)[h] = (uint16_t)(words[h / 2] >> (16 * (h & 1)));
+        }
+    }
 }
 
-// Rows of any length (they may end inside a block): a CTA takes `per` rows, which lie back to back, as
-// one range of bytes through shared memory, and hands the codes back the same way. 500K x 27 bf16:
-// 12.4 us (35 MB: 5.4): a CTA reads, computes and writes in turn, so small ones that overlap do better
-// (64 / 128 / 256 / 512 threads: 12.4 / 12.4 / 13.7 / 17.9); reading the elements as shifted 32-bit words
-// took 14.5.
-constexpr int kRowsThreads = 128;
+// Rows of any length (they may end inside a block): a CTA takes `per` (a power of two) rows, which lie back
+// to back, as one range of bytes through shared memory (asynchronous copies: 2.1M x 27 fp32 in MXFP4 49 us, 82
+// with a load and a store a turn), and hands the codes back the same way. The threads of a warp take one
+// block of neighbouring rows, so that what they read lies an odd number of elements or pairs apart (rows
+// of four-element packs do not come here) and meets few bank conflicts. 500K x 27 bf16 10.5 us (5.4 for the
+// bytes): a CTA reads, computes and writes in turn. Reading the elements as shifted 32-bit words was slower.
+// Most rows a CTA: short ones want many (2.9M x 3 fp16, 128 / 256 / 512 rows: 24 / 18 / 15.5 us).
+constexpr int kRowsThreads = 128, kRowsMost = 512;
 
-template <typename T, int FMT>
+template <typename T, int FMT, int EL>
 __global__ void __launch_bounds__(kRowsThreads)
-    k_mx4_quantise_rows(const T* __restrict__ x, int64_t rows, int dim, int per, uint8_t* __restrict__ codes,
+    k_mx4_quantise_rows(const T* __restrict__ x, int64_t rows, int dim, int log_per, uint8_t* __restrict__ codes,
                         uint8_t* __restrict__ scales, const float* __restrict__ tensor_scale) {
     constexpr int BS = Mx4Block<FMT>::size;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2;
-    const int64_t r0 = (int64_t)blockIdx.x * per;
+    const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2, per = 1 << log_per;
+    const int64_t r0 = (int64_t)blockIdx.x << log_per;
     const int mine = (int)min((int64_t)per, rows - r0);
     const unsigned char* gx = reinterpret_cast<const unsigned char*>(x + r0 * dim);
     uint8_t* gc = codes + r0 * cb;
@@ -239,17 +277,18 @@ __global__ void __launch_bounds__(kRowsThreads)
     __syncthreads();
     const T* sx = reinterpret_cast<const T*>(smem + head_of(gx));
     const TensorScale t = TensorScale::load<FMT>(tensor_scale);
-    for (int i = threadIdx.x; i < mine * nb; i += blockDim.x) {
-        const int r = i / nb, b = i - r * nb;
+    for (int i = threadIdx.x; i < nb << log_per; i += kRowsThreads) {
+        const int r = i & (per - 1), b = i >> log_per;
+        if (r >= mine) continue;
         const int len = min(BS, dim - b * BS);
-        float v[BS];
+        float v[EL];
 #pragma unroll
-        for (int k = 0; k < BS; ++k) v[k] = k < len ? to_f32(sx[r * dim + b * BS + k]) : 0.0f;
-        uint32_t words[BS / 8];
-        scales[r0 * nb + i] = (uint8_t)quantise_block<FMT>(v, t, words);
+        for (int k = 0; k < EL; ++k) v[k] = k < len ? to_f32(sx[r * dim + b * BS + k]) : 0.0f;
+        uint32_t words[EL / 8];
+        scales[(r0 + r) * nb + b] = (uint8_t)quantise_block<FMT>(v, t, words);
         unsigned char* o = sc + r * cb + b * (BS / 2);
 #pragma unroll
-        for (int k = 0; k < BS / 2; ++k)
+        for (int k = 0; k < EL / 2; ++k)
             if (2 * k < len) o[k] = (unsigned char)(words[k / 4] >> (8 * (k % 4)));
     }
     __syncthreads();
@@ -285,26 +324,35 @@ __global__ void __launch_bounds__(256) k_mx4_quantise(const T* __restrict__ x, i
 }
 
 // ---- dequantise ------------------------------------------------------------------------------
-// Rows of whole blocks, back to back: the codes, scales and values of all rows are one run each. A
-// thread fills kDequantisePacks times 16 bytes of output, next to its neighbours' each time; the word of
-// codes that it takes its half (or all) of is read by both. Bound by memory: 3M x 48 fp32 97 us (657 MB,
-// 6.7 TB/s); 139 with one pack a thread, 152 with the packs of a thread side by side.
+// Rows of packs of N elements (16 bytes, or four), back to back: the codes and values of all rows are one run each. A thread fills
+// kDequantisePacks packs of output, next to its neighbours' each time. WHOLE: rows of whole blocks,
+// whose scales are one run too. Bound by memory: 3M x 48 fp32 97 us (657 MB, 6.7 TB/s); 139 with one pack a
+// thread, 152 with the packs of a thread side by side.
 constexpr int kDequantisePacks = 4;
 
-template <typename T, int FMT>
-__global__ void __launch_bounds__(256) k_mx4_dequantise_blocks(const uint32_t* __restrict__ codes,
-                                                               const uint8_t* __restrict__ scales,
-                                                               const float* __restrict__ tensor_scale,
-                                                               int64_t packs, T* __restrict__ out) {
-    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T), R = kDequantisePacks;
+template <typename T, int FMT, int N, bool WHOLE>
+__global__ void __launch_bounds__(256)
+    k_mx4_dequantise_blocks(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                            const float* __restrict__ tensor_scale, int64_t packs, const FastDiv row_packs, int nb,
+                            T* __restrict__ out) {
+    constexpr int BS = Mx4Block<FMT>::size, R = kDequantisePacks;
+    // a pack's codes; in whole blocks a word that two packs of four share, faster (97 us, 103 by halves) but
+    // beyond the last row where the rows hold an odd number of packs
+    constexpr int SHARE = WHOLE && N == 4 ? 2 : 1;
+    using Codes = typename std::conditional<N * SHARE == 8, uint32_t, uint16_t>::type;
     const float g = FMT == GS3D_NVFP4 ? __ldg(tensor_scale) : 1.0f;
     const int64_t first = (int64_t)blockIdx.x * (256 * R) + threadIdx.x;
     uint32_t word[R], scale[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
         const int64_t i = min(first + 256 * q, packs - 1);
-        word[q] = __ldg(codes + i * N / 8);
-        scale[q] = __ldg(scales + i * N / BS);
+        word[q] = __ldg(reinterpret_cast<const Codes*>(codes) + i / SHARE);
+        int64_t block = i * N / BS;
+        if (!WHOLE) {
+            const uint32_t r = row_packs.quotient((uint32_t)i);
+            block = (int64_t)r * nb + (int)((uint32_t)i - r * row_packs.d) * N / BS;
+        }
+        scale[q] = __ldg(scales + block);
     }
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -321,7 +369,7 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise_blocks(const uint32_t* _
                 o.e[k + 4] = from_f32<T>(v.y);
             }
         } else {
-            if (threadIdx.x & 1) word[q] >>= 16;
+            if (SHARE == 2 && (threadIdx.x & 1)) word[q] >>= 16;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const float2 v = mx4_value(d, e2m1_pair_half(word[q] >> (8 * k)));
@@ -329,7 +377,8 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise_blocks(const uint32_t* _
                 o.e[2 * k + 1] = from_f32<T>(v.y);
             }
         }
-        if (i < packs) __stcs(reinterpret_cast<uint4*>(out) + i, *reinterpret_cast<const uint4*>(&o));
+        using W = typename std::conditional<sizeof(o) == 16, uint4, uint2>::type;
+        if (i < packs) __stcs(reinterpret_cast<W*>(out) + i, *reinterpret_cast<const W*>(&o));
     }
 }
 
@@ -341,18 +390,18 @@ __device__ __forceinline__ uint32_t word_at(const unsigned char* p) {
 }
 
 // Rows of any length, back to back: a CTA takes `per` rows' codes through shared memory, a block of a
-// row a thread, and hands the values back as one range of bytes. 500K x 27 bf16: 10.8 us (5.4 at the
-// copy rate), for the same reason as k_mx4_quantise_rows.
+// row a thread, and hands the values back as one range of bytes. 500K x 27 bf16: 10.0 us (5.4 for the
+// bytes), for the same reason as k_mx4_quantise_rows.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kRowsThreads)
     k_mx4_dequantise_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          const float* __restrict__ tensor_scale, int64_t rows, int dim, int per,
+                          const float* __restrict__ tensor_scale, int64_t rows, int dim, int log_per,
                           T* __restrict__ out) {
     constexpr int BS = Mx4Block<FMT>::size;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2;
+    const int nb = (dim + BS - 1) / BS, cb = (dim + 1) / 2, per = 1 << log_per;
     const float g = FMT == GS3D_NVFP4 ? __ldg(tensor_scale) : 1.0f;
-    const int64_t r0 = (int64_t)blockIdx.x * per;
+    const int64_t r0 = (int64_t)blockIdx.x << log_per;
     const int mine = (int)min((int64_t)per, rows - r0);
     const uint8_t* gc = codes + r0 * cb;
     unsigned char* go = reinterpret_cast<unsigned char*>(out + r0 * dim);
@@ -361,10 +410,11 @@ __global__ void __launch_bounds__(kRowsThreads)
     __syncthreads();
     const unsigned char* sc = smem + head_of(gc);
     T* sv = reinterpret_cast<T*>(so + head_of(go));
-    for (int i = threadIdx.x; i < mine * nb; i += blockDim.x) {
-        const int r = i / nb, b = i - r * nb;
+    for (int i = threadIdx.x; i < nb << log_per; i += kRowsThreads) {
+        const int r = i & (per - 1), b = i >> log_per;
+        if (r >= mine) continue;
         const int len = min(BS, dim - b * BS);
-        const Mx4Decode<FMT> d(__ldg(scales + r0 * nb + i), g);
+        const Mx4Decode<FMT> d(__ldg(scales + (r0 + r) * nb + b), g);
         const unsigned char* c = sc + r * cb + b * (BS / 2);
         T* o = sv + r * dim + b * BS;
 #pragma unroll
@@ -404,28 +454,36 @@ __global__ void __launch_bounds__(256) k_mx4_dequantise(const uint8_t* __restric
     }
 }
 
-// Rows a CTA of the *_rows kernels takes: a block for each of its threads, as far as they fit.
-int rows_per_cta(int row_bytes, int row_blocks) {
-    return std::max(1, std::min(kRowsBytes / row_bytes, kRowsThreads / row_blocks));
+// Rows a CTA of the *_rows kernels takes (log2): what fits, as far as it gives each of its threads few blocks.
+int log_rows_per_cta(int row_bytes) {
+    int l = 0;
+    while (2 << l <= kRowsMost && row_bytes * (2 << l) <= kRowsBytes) ++l;
+    return l;
 }
 
-template <typename T, int FMT>
-int launch_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t stream) {
+template <typename T, int FMT, int EL>
+int launch_quantise_elements(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t stream) {
     constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T);
     const T* in = static_cast<const T*>(x->data);
     const int dim = x->dim, nb = mx4_blocks(dim, FMT);
     const int64_t blocks = x->rows * nb;
     const bool flat = x->row_stride == dim;
-    if (dim % BS == 0 && x->row_stride % N == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0 &&
-        reinterpret_cast<uintptr_t>(out->codes) % (BS / 2) == 0 && blocks / 256 < INT_MAX) {
-        k_mx4_quantise_blocks<T, FMT><<<(unsigned)ceil_div(blocks, 256), 256, 0, stream>>>(
-            in, blocks, x->row_stride, nb, flat, out->codes, out->scales, out->tensor_scale);
+    if (packs_of<T, 4 * (int)sizeof(T)>(x) && blocks / 256 < INT_MAX &&
+        reinterpret_cast<uintptr_t>(out->codes) % (dim % BS ? 4 : BS / 2) == 0) {
+        auto kernel = k_mx4_quantise_blocks<T, FMT, EL, 4, false>;
+        if (packs_of<T, 16>(x)) {
+            kernel = k_mx4_quantise_blocks<T, FMT, EL, N, false>;
+            if constexpr (EL == BS)
+                if (dim % BS == 0) kernel = k_mx4_quantise_blocks<T, FMT, EL, N, true>;
+        }
+        kernel<<<(unsigned)ceil_div(blocks, 256), 256, 0, stream>>>(in, blocks, x->row_stride, dim, FastDiv(nb), flat,
+                                                                    out->codes, out->scales, out->tensor_scale);
     } else if (flat && dim * (int)sizeof(T) <= kRowsBytes) {
-        const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
-        const size_t smem = ((16 + (size_t)per * dim * sizeof(T) + 15) & ~(size_t)15) + 16 +
-                            (size_t)per * mx4_code_bytes(dim) + 16;
-        k_mx4_quantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), kRowsThreads, smem, stream>>>(
-            in, x->rows, dim, per, out->codes, out->scales, out->tensor_scale);
+        const int l = log_rows_per_cta(dim * (int)sizeof(T));
+        const size_t smem = ((16 + ((size_t)dim * sizeof(T) << l) + 15) & ~(size_t)15) + 16 +
+                            ((size_t)mx4_code_bytes(dim) << l) + 16;
+        k_mx4_quantise_rows<T, FMT, EL><<<(unsigned)ceil_div(x->rows, (int64_t)1 << l), kRowsThreads, smem, stream>>>(
+            in, x->rows, dim, l, out->codes, out->scales, out->tensor_scale);
     } else {
         k_mx4_quantise<T, FMT><<<grid_for(blocks, 256, 8), 256, 0, stream>>>(
             in, x->rows, x->row_stride, dim, out->codes, out->scales, out->tensor_scale);
@@ -434,23 +492,35 @@ int launch_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t s
     return GS3D_OK;
 }
 
+// Rows shorter than a block need not pay for all of it.
+template <typename T, int FMT>
+int launch_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, cudaStream_t stream) {
+    if (x->dim <= 8) return launch_quantise_elements<T, FMT, 8>(x, out, stream);
+    if (x->dim <= 16) return launch_quantise_elements<T, FMT, 16>(x, out, stream);
+    return launch_quantise_elements<T, FMT, Mx4Block<FMT>::size>(x, out, stream);
+}
+
 template <typename T, int FMT>
 int launch_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, cudaStream_t stream) {
-    constexpr int BS = Mx4Block<FMT>::size, N = 16 / (int)sizeof(T);
+    constexpr int BS = Mx4Block<FMT>::size;
     T* o = static_cast<T*>(out->data);
-    const int dim = x->dim;
-    const int64_t packs = x->rows * dim / N;
-    const bool flat = out->row_stride == dim;
-    if (flat && dim % BS == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0 &&
-        reinterpret_cast<uintptr_t>(x->codes) % 4 == 0 && packs / 256 < INT_MAX) {
-        k_mx4_dequantise_blocks<T, FMT><<<(unsigned)ceil_div(packs, 256 * kDequantisePacks), 256, 0, stream>>>(
-            reinterpret_cast<const uint32_t*>(x->codes), x->scales, x->tensor_scale, packs, o);
+    const int dim = x->dim, nb = mx4_blocks(dim, FMT);
+    const int n = packs_of<T, 16>(out) ? 16 / (int)sizeof(T) : 4;
+    const int64_t packs = x->rows * dim / n;
+    const bool flat = out->row_stride == dim, whole = n * sizeof(T) == 16 && dim % BS == 0;
+    if (flat && packs_of<T, 4 * (int)sizeof(T)>(out) && reinterpret_cast<uintptr_t>(x->codes) % 4 == 0 &&
+        (whole ? packs / 256 : packs) < INT_MAX) {
+        auto kernel = k_mx4_dequantise_blocks<T, FMT, 4, false>;
+        if (n * sizeof(T) == 16) kernel = k_mx4_dequantise_blocks<T, FMT, 16 / (int)sizeof(T), false>;
+        if (whole) kernel = k_mx4_dequantise_blocks<T, FMT, 16 / (int)sizeof(T), true>;
+        kernel<<<(unsigned)ceil_div(packs, 256 * kDequantisePacks), 256, 0, stream>>>(
+            x->codes, x->scales, x->tensor_scale, packs, FastDiv(dim / n), nb, o);
     } else if (flat && dim * (int)sizeof(T) <= kRowsBytes) {
-        const int per = rows_per_cta(dim * (int)sizeof(T), mx4_blocks(dim, FMT));
-        const size_t smem = ((16 + (size_t)per * mx4_code_bytes(dim) + 15) & ~(size_t)15) + 16 +
-                            (size_t)per * dim * sizeof(T) + 16 + 16;  // and what word_at reads behind the codes
-        k_mx4_dequantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, per), kRowsThreads, smem, stream>>>(
-            x->codes, x->scales, x->tensor_scale, x->rows, dim, per, o);
+        const int l = log_rows_per_cta(dim * (int)sizeof(T));
+        const size_t smem = ((16 + ((size_t)mx4_code_bytes(dim) << l) + 15) & ~(size_t)15) + 16 +
+                            ((size_t)dim * sizeof(T) << l) + 16 + 16;  // and what word_at reads behind the codes
+        k_mx4_dequantise_rows<T, FMT><<<(unsigned)ceil_div(x->rows, (int64_t)1 << l), kRowsThreads, smem, stream>>>(
+            x->codes, x->scales, x->tensor_scale, x->rows, dim, l, o);
     } else {
         k_mx4_dequantise<T, FMT><<<grid_for(x->rows * dim, 256, 8), 256, 0, stream>>>(
             x->codes, x->scales, x->tensor_scale, x->rows, out->row_stride, dim, o);

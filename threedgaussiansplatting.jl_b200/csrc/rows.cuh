@@ -64,9 +64,11 @@ __device__ __forceinline__ void copy_in(unsigned char* sh, const unsigned char* 
     const unsigned char* g0 = gl - h;
     const int t = threadIdx.x;
     if (t >= h && t < min(first, end)) sh[t] = __ldg(g0 + t);
-    for (int i = first + 16 * t; i < last; i += 16 * blockDim.x)
-        *reinterpret_cast<uint4*>(sh + i) = __ldg(reinterpret_cast<const uint4*>(g0 + i));
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(sh);
+    for (int i = first + 16 * t; i < last; i += 16 * blockDim.x)  // asynchronous: all of them in flight
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i), "l"(g0 + i) : "memory");
     if (last + t < end) sh[last + t] = __ldg(g0 + last + t);
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 __device__ __forceinline__ void copy_out(unsigned char* gl, const unsigned char* sh, int bytes) {

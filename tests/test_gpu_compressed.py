@@ -435,6 +435,36 @@ def test_quantise_non_finite(cuda, fmt):
     assert float(gc.mx4_tensor_scale(torch.zeros(0, 4, device=cuda))) == 2.0 ** -100
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [3, 50_001, 1_200_007])
+def test_tensor_scale(cuda, kind, n):
+    """The largest finite magnitude wherever it lies, among infinities and NaN."""
+    x = torch.zeros(n, 48, dtype=kind, device=cuda)
+    flat = x.view(-1)
+    for at in (0, flat.shape[0] // 2 + 1, flat.shape[0] - 1):
+        flat[at] = -3.0
+        assert float(gc.mx4_tensor_scale(x)) == float(np.float32(3.0) * (np.float32(1) / np.float32(2688)))
+        for other in (float("inf"), -float("inf"), float("nan")):
+            flat[(at + 77) % flat.shape[0]] = other
+            assert float(gc.mx4_tensor_scale(x)) == float(np.float32(3.0) * (np.float32(1) / np.float32(2688)))
+        flat[at] = 0.0
+        flat[(at + 77) % flat.shape[0]] = 0.0
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+def test_quantise_ratios_of_small_numbers(cuda, kind):
+    """16-bit elements and a power-of-two maximum: quotients that meet the borders exactly."""
+    gen = rng(3)
+    x = torch.randint(-64, 65, (4001, 48), generator=gen).float() / 8
+    x[:, 0] = torch.tensor([7.0, 10.5, 21.0, 8.0]).repeat(1001)[:4001]
+    x = x.to(kind)
+    for s in (None, torch.tensor([21.0 / 2688]), torch.tensor([2.0 ** -9]), torch.tensor([3.0 / 448])):
+        q = gc.mx4_quantise(x.to(cuda), "nvfp4", tensor_scale=None if s is None else s.to(cuda))
+        codes, byte, val, _ = quantise_exact(x, "nvfp4", float(q.tensor_scale.cpu()))
+        assert np.array_equal(q.scales.cpu().numpy(), byte)
+        assert np.array_equal(q.codes.cpu().numpy(), codes)
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("dim", [48, 27])
 def test_quantise_largest_and_smallest(cuda, fmt, dim):

@@ -10,11 +10,12 @@
 //   MXFP4: s is a power of two, so x (1 / s) is exact and one conversion decides.
 //   NVFP4: x (1 / (s g)) is not exact. Products with the reciprocal moved down and up by 2^-21 (more
 //     than the errors of s g, its reciprocal and the product) enclose q, and rounding is monotone: where
-//     both convert to the same code, q does. Else a border lies between them, and the block is decided
-//     against the borders themselves: q passes a border b iff |x| > b s g (>= where the tie goes up).
-//     b s is exact in fp32 (at most 7 significant bits); b s g is not, but no fp32 lies between it and
-//     its neighbours RD(b s g) <= b s g <= RU(b s g), so |x| > b s g iff |x| > RD(b s g) and
-//     |x| >= b s g iff |x| >= RU(b s g): exact with one directed product per border.
+//     both convert to the same code, q does. Else one border b lies between them, and q is held against it:
+//     q passes b iff |x| > b s g (>= where the tie goes up). b s is exact in fp32 (at most 7 significant
+//     bits); b s g is not, but no fp32 lies between it and its neighbours RD(b s g) <= b s g <= RU(b s g),
+//     so |x| > b s g iff |x| > RD(b s g) and |x| >= b s g iff |x| >= RU(b s g): exact with one directed
+//     product. Such borders are common where x has few bits: of 16-bit x and its own tensor scale, q is a
+//     ratio of small numbers. The block scale is decided in the same way.
 #include <type_traits>
 
 #include "common.cuh"
@@ -60,10 +61,26 @@ __device__ __forceinline__ void take_finite_abs(uint32_t& m, float v) {
     if (b < 0x7f800000u) m = max(m, b);
 }
 
+// The largest magnitude among packs, NaN left out: a word of it for each word of the packs.
+__device__ __forceinline__ float abs_max(float m, float v) { return fmaxf(m, fabsf(v)); }
+__device__ __forceinline__ __half2 abs_max(__half2 m, __half2 v) { return __hmax2(m, __habs2(v)); }
+__device__ __forceinline__ __nv_bfloat162 abs_max(__nv_bfloat162 m, __nv_bfloat162 v) { return __hmax2(m, __habs2(v)); }
+__device__ __forceinline__ float larger(float m) { return m; }
+__device__ __forceinline__ float larger(__half2 m) { return fmaxf(__low2float(m), __high2float(m)); }
+__device__ __forceinline__ float larger(__nv_bfloat162 m) { return fmaxf(__low2float(m), __high2float(m)); }
+template <typename T>
+using Word = typename std::conditional<
+    sizeof(T) == 4, float, typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type>::type;
+
 // Every block turns its largest magnitude into the scale it asks for (monotone, positive: fp32 bits
 // order like unsigned integers) and the largest one stays; a lone block stores it. A maximum does not
-// depend on the order, so the atomics give equal bits. Bound by reading x: 3M x 48 fp32 104 us (5.5 TB/s).
-// WIDE: rows of 16-byte packs, back to back, eight loads a thread in flight.
+// depend on the order, so the atomics give equal bits.
+// WIDE: rows of 16-byte packs, back to back, eight loads a thread in flight, of 16-bit elements two a
+// comparison. Bound by reading x: 3M x 48 fp32 95 us (6.0 TB/s), 1.5M x 48 bf16 29 (39 with the elements one by
+// one in fp32). All but the last 96 MB are read as data that L2 need not keep, so that what k_mx4_quantise_blocks
+// begins with is there: with its own loads so marked too the two and the dequantisation behind them take
+// 281 us at 3M x 48 fp32, 298 with plain loads.
+constexpr int64_t kScaleKept = (int64_t)96 << 20;
 constexpr int kScaleThreads = 512;
 
 template <typename T, bool WIDE>
@@ -76,12 +93,40 @@ __global__ void __launch_bounds__(kScaleThreads) k_mx4_tensor_scale(const T* __r
     const int64_t total = rows * dim, threads = (int64_t)gridDim.x * blockDim.x;
     const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (WIDE) {
-        const Pack<T, N>* p = reinterpret_cast<const Pack<T, N>*>(x);
-#pragma unroll 8
-        for (int64_t i = t; i < total / N; i += threads) {
-            const Pack<T, N> v = p[i];
+        using W = Word<T>;
+        const int64_t packs = total / N;
+        const uint4* p = reinterpret_cast<const uint4*>(x);
+        W top{};
+        constexpr int AHEAD = 8;
+        const int64_t streamed = packs - max(kScaleKept / 16, AHEAD * threads);
+        const auto batch = [&](int64_t i, auto full) {
+            uint4 v[AHEAD];
 #pragma unroll
-            for (int c = 0; c < N; ++c) take_finite_abs(m, to_f32(v.e[c]));
+            for (int q = 0; q < AHEAD; ++q) {
+                v[q] = make_uint4(0u, 0u, 0u, 0u);
+                if (i < streamed) v[q] = __ldcs(p + i + q * threads);
+                else if (full || i + q * threads < packs) v[q] = __ldg(p + i + q * threads);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                top = abs_max(top, *reinterpret_cast<const W*>(&v[q].x));
+                top = abs_max(top, *reinterpret_cast<const W*>(&v[q].y));
+                top = abs_max(top, *reinterpret_cast<const W*>(&v[q].z));
+                top = abs_max(top, *reinterpret_cast<const W*>(&v[q].w));
+            }
+        };
+        int64_t i = t;
+        for (; i + (AHEAD - 1) * threads < packs; i += AHEAD * threads) batch(i, std::true_type{});
+        if (i < packs) batch(i, std::false_type{});
+        const float a = larger(top);
+        if (f2u(a) < 0x7f800000u) {
+            m = f2u(a);
+        } else {  // infinities do not count: once more without them
+            for (int64_t i = t; i < packs; i += threads) {
+                const Pack<T, N> v = reinterpret_cast<const Pack<T, N>*>(x)[i];
+#pragma unroll
+                for (int c = 0; c < N; ++c) take_finite_abs(m, to_f32(v.e[c]));
+            }
         }
         const int64_t tail = total / N * N + t;
         if (tail < total) take_finite_abs(m, to_f32(x[tail]));
@@ -105,7 +150,7 @@ __global__ void __launch_bounds__(kScaleThreads) k_mx4_tensor_scale(const T* __r
 // ---- quantise --------------------------------------------------------------------------------
 // a / (6 g) to the nearest e4m3 value, ties to even, at most 448 (0x7e): an estimate (within a step),
 // corrected against the exact borders around it.
-__device__ __forceinline__ uint32_t nvfp4_scale_byte(float a, float g, float inv6g) {
+__device__ __noinline__ uint32_t nvfp4_scale_byte_exact(float a, float g, float inv6g) {
     const float est = fminf(a * inv6g, 448.0f);
     uint32_t u = __nv_cvt_float_to_fp8(est, __NV_SATFINITE, __NV_E4M3) & 0x7fu;
     const float v = e4m3_value(u);
@@ -118,6 +163,14 @@ __device__ __forceinline__ uint32_t nvfp4_scale_byte(float a, float g, float inv
         if ((u & 1u) ? a <= __fmul_rd(border, g) : a < __fmul_ru(border, g)) return u - 1;
     }
     return u;
+}
+
+// The same: enclosed, where both ends convert to the same value (0x7f for a NaN).
+__device__ __forceinline__ uint32_t nvfp4_scale_byte(float a, float g, float inv6g) {
+    const uint32_t both = __nv_cvt_float2_to_fp8x2(
+        make_float2(a * (inv6g * (1.0f - 0x1p-21f)), a * (inv6g * (1.0f + 0x1p-21f))), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = both & 0xffu;
+    return lo == both >> 8 ? lo : nvfp4_scale_byte_exact(a, g, inv6g);
 }
 
 // 2^(floor(log2 a) - 2) as its e8m0 byte.
@@ -136,17 +189,25 @@ __device__ __forceinline__ uint32_t e2m1_word(const float* x, float f) {
     return w;
 }
 
-// The code of x against the borders themselves.
-__device__ __noinline__ uint32_t e2m1_code_exact(float x, float s, float g) {
-    const float b[7] = {0.25f, 0.75f, 1.25f, 1.75f, 2.5f, 3.5f, 5.0f};
-    const float a = fabsf(x);
-    uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < 7; ++j) {
-        const float bs = b[j] * s;
-        c += ((j & 1) ? a >= __fmul_ru(bs, g) : a > __fmul_rd(bs, g)) ? 1u : 0u;
-    }
-    return c | ((f2u(x) >> 28) & 8u);
+// Whether a magnitude lies beyond the border between codes c and c + 1, ties to the even code.
+__device__ __forceinline__ bool beyond_border(float a, uint32_t c, float s, float g) {
+    const float2 e = __half22float2(e2m1_pair_half(c | (c + 1) << 4));
+    const float bs = (e.x + e.y) * 0x1p13f * s;  // border * s, exact
+    return (c & 1u) ? a >= __fmul_ru(bs, g) : a > __fmul_rd(bs, g);
+}
+
+// 1 / v within one unit in the last place, for v and 1 / v within the normal numbers.
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// The larger magnitude, NaN if one is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
 }
 
 struct TensorScale {
@@ -156,7 +217,7 @@ struct TensorScale {
         TensorScale t{1.0f, 0.0f};
         if (FMT == GS3D_NVFP4) {
             t.g = __ldg(p);
-            t.inv6g = 1.0f / (6.0f * t.g);
+            t.inv6g = reciprocal(6.0f * t.g);
         }
         return t;
     }
@@ -166,11 +227,10 @@ struct TensorScale {
 // in words of eight. EL < block size: rows of at most EL elements.
 template <int FMT, int EL>
 __device__ __forceinline__ uint32_t quantise_block(const float (&v)[EL], const TensorScale& t, uint32_t (&words)[EL / 8]) {
-    uint32_t top = 0;  // magnitudes order like unsigned integers, infinity and NaN above all
+    float a = fabsf(v[0]);
 #pragma unroll
-    for (int k = 0; k < EL; ++k) top = max(top, f2u(v[k]) & 0x7fffffffu);
-    const bool nan = top > 0x7f800000u;
-    const float a = u2f(top);
+    for (int k = 1; k < EL; ++k) a = max_abs(a, v[k]);
+    const bool nan = a != a;
     if (FMT == GS3D_MXFP4) {
         const uint32_t byte = mxfp4_scale_byte(a);
         const float inv = u2f((254u - byte) << 23);  // 2^(127 - byte), byte <= 253
@@ -180,31 +240,32 @@ __device__ __forceinline__ uint32_t quantise_block(const float (&v)[EL], const T
     }
     const uint32_t byte = nvfp4_scale_byte(a, t.g, t.inv6g);
     const float s = e4m3_value(byte);
-    const float inv = s > 0.0f ? 1.0f / (s * t.g) : 0.0f;
+    const float inv = s > 0.0f ? reciprocal(s * t.g) : 0.0f;
     const float lo = inv * (1.0f - 0x1p-21f), hi = inv * (1.0f + 0x1p-21f);
-    uint32_t differ = 0;
+    uint32_t differ = 0, upper[EL / 8];
 #pragma unroll
     for (int w = 0; w < EL / 8; ++w) {
         words[w] = e2m1_word(v + 8 * w, lo);
-        differ |= words[w] ^ e2m1_word(v + 8 * w, hi);
+        upper[w] = e2m1_word(v + 8 * w, hi) ^ words[w];
+        differ |= upper[w];
     }
-    if (differ && s > 0.0f) {
+    if (differ)
 #pragma unroll
-        for (int w = 0; w < EL / 8; ++w) {
-            words[w] = 0;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) words[w] |= e2m1_code_exact(v[8 * w + k], s, t.g) << (4 * k);
+        for (int k = 0; k < EL; ++k) {
+            const uint32_t d = (upper[k / 8] >> (4 * (k % 8))) & 15u, c = (words[k / 8] >> (4 * (k % 8))) & 7u;
+            if (d && beyond_border(fabsf(v[k]), c, s, t.g)) words[k / 8] ^= d << (4 * (k % 8));
         }
-    }
     return nan ? 0x7fu : byte;
 }
 
-// Rows in packs of N elements (16 bytes, or four): a block a thread, whose elements, scale and codes stay in its registers; from the
-// last row to the first, so that what a tensor-scale pass just before has left in L2 is read from there.
-// 3M x 48 fp32 in NVFP4: 91 us behind that pass (657 MB, 100 us at the rate of a plain copy). The scale is
-// known before x is read again: one kernel for both would need all of x on the chip. WHOLE: rows of whole
-// blocks, the codes stored a block at a time; else in words, or in halves of them (2.6M x 48 fp32 in MXFP4,
-// whose last block is half: 98 us, through shared memory 339).
+// Rows in packs of N elements (16 bytes, or four): a block a thread, whose elements, scale and codes stay
+// in its registers; from the last row to the first, so that what a tensor-scale pass just before has left
+// in L2 is read from there. Bound by memory with fp32 (3M x 48 in NVFP4 87 us behind that pass; 657 MB, 100 us
+// at the rate of a plain copy; 2.6M x 48 in MXFP4, whose last block is half, 98 us, through shared memory
+// 339), by the instructions with 16-bit elements in NVFP4 (1.5M x 48 bf16 40 us, 26 for the bytes; 78 with all
+// elements of a block held against all borders where one might lie between two codes). The tensor scale
+// is known before x is read again: one kernel for both would need all of x on the chip.
+// WHOLE: rows of whole blocks, the codes stored a block at a time; else in words, or in halves of them.
 template <typename T, int FMT, int EL, int N, bool WHOLE>
 __global__ void __launch_bounds__(256)
     k_mx4_quantise_blocks(const T* __restrict__ x, int64_t blocks, int64_t stride, int dim, const FastDiv nb, bool flat,
@@ -227,7 +288,11 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int k = 0; k < EL; k += N) {
         Pack<T, N> p{};
-        if (WHOLE || k < len) p = *reinterpret_cast<const Pack<T, N>*>(xb + k);
+        if (WHOLE || k < len) {
+            using W = typename std::conditional<sizeof(p) == 16, uint4, uint2>::type;
+            const W w = __ldcs(reinterpret_cast<const W*>(xb + k));
+            p = *reinterpret_cast<const Pack<T, N>*>(&w);
+        }
 #pragma unroll
         for (int c = 0; c < N; ++c) v[k + c] = to_f32(p.e[c]);
     }

@@ -146,6 +146,18 @@ def test_gradient_units(cuda, n, dim, stride, offset, kind):
     assert ((got.cpu().double() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("n", [303_104, 303_105, 606_208, 606_209])
+@pytest.mark.parametrize("rows", [700, 90_000])
+def test_gradient_sizes_where_the_tiles_change(cuda, n, rows):
+    """Tiles of 1024, 2048 and 4096 rows; few of them leave blocks that zero the table."""
+    gen = rng(n + rows)
+    grads = torch.randn(n, 3, generator=gen)
+    idx = make_indices(n, rows, gen, 1.0)
+    got = gc.table_gradient(grads.to(cuda), idx.to(cuda), rows)
+    want, bound = gradient_exact(grads, idx, rows, 1.0)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("n,dim", [(700_000, 119), (500_000, 260), (300_000, 1)])
 def test_gradient_of_long_runs(cuda, n, dim):
     """Few rows used by very many: runs over hundreds and thousands of chunks, beside short ones."""

@@ -132,10 +132,10 @@ int launch_lookup(const gs3d_rows* table, const int32_t* indices, float scale, c
 }
 
 // ---- gradient --------------------------------------------------------------------------------
-// 1. Stable sort of the rows by table row (k_radix_*: tiles of 4096 rows, digits of up to 10 bits, three
-//    launches and one pass per 10 bits of the row number; up to 4096 rows k_sort_small, one block in shared
-//    memory; up to 1024 k_table_gradient_tiny does everything). Rows without a valid index drop out of
-//    the first pass, which also zeroes the table's gradients.
+// 1. Stable sort of the rows by table row (k_radix_*: tiles of 1024 to 4096 rows, digits of up to 10 bits,
+//    three launches and one pass per 10 bits of the row number; up to 4096 rows k_sort_small, one block in
+//    shared memory; up to 1024 k_table_gradient_tiny does everything). Rows without a valid index drop
+//    out of the first pass, which also zeroes the table's gradients.
 // 2. k_table_segments: the sorted rows are cut into chunks of equal length, a block each, and a chunk
 //    into one run of rows per slot (a slot: the threads side by side on a row's columns). A slot adds
 //    its rows in order; a run of equal indices that crosses slots is added up in slot order through
@@ -175,8 +175,7 @@ int launch_after(const char* what, void (*kernel)(P...), dim3 grid, int threads,
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortTile = 4096;
-constexpr int kSortRounds = kSortTile / kSortThreads;
+constexpr int kSmallSort = 4096;  // rows that one block sorts
 constexpr int kMaxDigitBits = 10;
 
 // Row f's table row 0 .. rows - 1, or -1 where it takes no part.
@@ -239,32 +238,39 @@ struct SortPass {
 };
 
 // A thread's place in a tile: its rows are place, place + 32, ..., warp after warp in row order.
+template <int ROUNDS>
 __device__ __forceinline__ int tile_place(int tile) {
-    return tile * kSortTile + (threadIdx.x >> 5) * (kSortRounds * 32) + (threadIdx.x & 31);
+    return tile * (kSortThreads * ROUNDS) + (threadIdx.x >> 5) * (ROUNDS * 32) + (threadIdx.x & 31);
 }
 
+template <int ROUNDS>
 __global__ void __launch_bounds__(kSortThreads) k_radix_count(const SortPass p, const KeySource src,
                                                               const ZeroRows zero) {
     __shared__ int bins[1 << kMaxDigitBits];
     after_predecessor();
-    const int nbins = 1 << p.bits, tile = blockIdx.x, place = tile_place(tile);
+    const int fillers = gridDim.x - p.ntiles;  // blocks behind the tiles', which zero the table
+    if ((int)blockIdx.x >= p.ntiles) {
+        zero.fill((int64_t)(blockIdx.x - p.ntiles) * kSortThreads + threadIdx.x, (int64_t)fillers * kSortThreads);
+        return;
+    }
+    const int nbins = 1 << p.bits, tile = blockIdx.x, place = tile_place<ROUNDS>(tile);
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) bins[b] = 0;
-    int key[kSortRounds];
+    int key[ROUNDS];
     if (!p.in) {
         src.keys(place, key);
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r)
+        for (int r = 0; r < ROUNDS; ++r)
             if (place + 32 * r < p.n) p.first_keys[place + 32 * r] = key[r];
     } else {
         const int m = *p.valid;
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) key[r] = place + 32 * r < m ? p.in[place + 32 * r].x : -1;
+        for (int r = 0; r < ROUNDS; ++r) key[r] = place + 32 * r < m ? p.in[place + 32 * r].x : -1;
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)
+    for (int r = 0; r < ROUNDS; ++r)
         if (key[r] >= 0) atomicAdd(&bins[(key[r] >> p.shift) & (nbins - 1)], 1);
-    if (!p.in) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)gridDim.x * kSortThreads);
+    if (!p.in && fillers == 0) zero.fill((int64_t)tile * kSortThreads + threadIdx.x, (int64_t)p.ntiles * kSortThreads);
     __syncthreads();
     for (int b = threadIdx.x; b < nbins; b += kSortThreads) p.hist[(int64_t)b * p.ntiles + tile] = bins[b];
 }
@@ -286,8 +292,8 @@ __global__ void __launch_bounds__(kSpineThreads) k_radix_spine(const SortPass p)
     if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
 }
 
-size_t radix_scatter_smem(int bits) {
-    return (size_t)kSortTile * 8 + (size_t)(1 << bits) * (4 + 2 * kSortWarps);
+size_t radix_scatter_smem(int rounds, int bits) {
+    return (size_t)rounds * kSortThreads * 8 + (size_t)(1 << bits) * (4 + 2 * kSortWarps);
 }
 
 // Exclusive block scan of one 64-bit value per thread of kSortThreads.
@@ -314,6 +320,7 @@ __device__ __forceinline__ int64_t block_exclusive_scan64(int64_t v, int64_t* sm
     return inc - v + (w ? sm[w - 1] : 0);
 }
 
+template <int ROUNDS>
 __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPass p) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int64_t sm[kSortWarps];
@@ -321,13 +328,13 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPas
     after_predecessor();
     const int nbins = 1 << p.bits, tile = blockIdx.x;
     int2* items = reinterpret_cast<int2*>(smem);                   // the tile in digit order
-    int32_t* dest = reinterpret_cast<int32_t*>(items + kSortTile);  // a bin's place in the output, minus in the tile
+    int32_t* dest = reinterpret_cast<int32_t*>(items + ROUNDS * kSortThreads);  // a bin's place in the output, minus in the tile
     uint16_t* wcount = reinterpret_cast<uint16_t*>(dest + nbins);  // [warp][bin]
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int place = tile_place(tile), m = p.in ? *p.valid : p.n;
-    int2 item[kSortRounds];
+    const int place = tile_place<ROUNDS>(tile), m = p.in ? *p.valid : p.n;
+    int2 item[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         const int i = place + 32 * r;
         item[r] = make_int2(-1, i);
         if (i < m) {
@@ -348,22 +355,22 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPas
     __syncthreads();
     // stable rank of every key among its warp's keys of the same digit: within its 32, then behind the 32s
     // before
-    int rank[kSortRounds];
+    int rank[ROUNDS];
     const unsigned below = (1u << lane) - 1u;
-    unsigned peers[kSortRounds];  // lanes with the same digit, bit by bit
+    unsigned peers[ROUNDS];  // lanes with the same digit, bit by bit
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) peers[r] = __ballot_sync(0xffffffffu, item[r].x >= 0);
+    for (int r = 0; r < ROUNDS; ++r) peers[r] = __ballot_sync(0xffffffffu, item[r].x >= 0);
     for (int b = p.shift; b < p.shift + p.bits; ++b)
 #pragma unroll
-        for (int r = 0; r < kSortRounds; ++r) {
+        for (int r = 0; r < ROUNDS; ++r) {
             const bool bit = (item[r].x >> b) & 1;
             const unsigned ones = __ballot_sync(0xffffffffu, bit);
             peers[r] &= bit ? ones : ~ones;
         }
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) rank[r] = __popc(peers[r] & below) | __popc(peers[r]) << 8;
+    for (int r = 0; r < ROUNDS; ++r) rank[r] = __popc(peers[r] & below) | __popc(peers[r]) << 8;
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         const bool on = item[r].x >= 0;
         uint16_t& c = wcount[w * nbins + (on ? (item[r].x >> p.shift) & (nbins - 1) : 0)];
         const int before = c, mine = rank[r] & 255, all = rank[r] >> 8;
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kSortThreads, 2) k_radix_scatter(const SortPas
     if (!p.in && tile == 0 && threadIdx.x == 0) *p.valid = (int32_t)(all >> 32);
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)
+    for (int r = 0; r < ROUNDS; ++r)
         if (item[r].x >= 0) items[wcount[w * nbins + ((item[r].x >> p.shift) & (nbins - 1))] + rank[r]] = item[r];
     __syncthreads();
     const int count = (int)all;
@@ -472,13 +479,13 @@ __device__ __forceinline__ int sort_rows(const KeySource& src, int bits, int2* i
     return count;
 }
 
-// Up to kSortTile rows: block 0 sorts them; the others zero the table.
+// Up to kSmallSort rows: block 0 sorts them; the others zero the table.
 constexpr int kSmallThreads = 512;
 
 __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource src, const ZeroRows zero, int bits,
                                                               int2* __restrict__ out,
                                                               int32_t* __restrict__ valid) {
-    __shared__ int2 items[kSortTile];
+    __shared__ int2 items[kSmallSort];
     __shared__ uint16_t wcount[kSmallThreads / 32][256];
     __shared__ int start[256], sm[33];
     after_predecessor();
@@ -486,7 +493,7 @@ __global__ void __launch_bounds__(kSmallThreads) k_sort_small(const KeySource sr
         zero.fill((int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
         return;
     }
-    const int count = sort_rows<kSmallThreads, kSortTile / kSmallThreads>(src, bits, items, wcount, start, sm);
+    const int count = sort_rows<kSmallThreads, kSmallSort / kSmallThreads>(src, bits, items, wcount, start, sm);
     for (int i = threadIdx.x; i < count; i += kSmallThreads) out[i] = items[i];
     if (threadIdx.x == 0) *valid = count;
 }
@@ -802,6 +809,21 @@ SegmentPlan segment_plan(int64_t n, int units) {
     return p;
 }
 
+// Rows a thread of the sort's tiles takes: small tiles for few rows, so that all SMs have some (300K rows into
+// 60,000 of the table, 2 / 4 / 8 rows: 41 / 43 / 51 us in all; 450K: - / 49 / 56).
+int sort_rounds(int64_t n) {
+    return n <= 2 * kSMs * 2 * kSortThreads ? 2 : (n <= 2 * kSMs * 4 * kSortThreads ? 4 : 8);
+}
+
+template <typename F>
+int dispatch_rounds(int rounds, F&& f) {
+    switch (rounds) {
+        case 2: return f(std::integral_constant<int, 2>{});
+        case 4: return f(std::integral_constant<int, 4>{});
+        default: return f(std::integral_constant<int, 8>{});
+    }
+}
+
 int bits_of(int64_t v) {
     int b = 0;
     while (v >> b) ++b;
@@ -810,7 +832,7 @@ int bits_of(int64_t v) {
 
 GradLayout grad_layout(int64_t n, int64_t rows, int dim) {
     GradLayout L;
-    L.ntiles = (int)ceil_div(n, kSortTile);
+    L.ntiles = (int)ceil_div(n, sort_rounds(n) * kSortThreads);
     L.bits = bits_of(std::max<int64_t>(rows, 1) - 1);
     L.passes = std::max(1, (L.bits + kMaxDigitBits - 1) / kMaxDigitBits);
     const int digit = (L.bits + L.passes - 1) / L.passes;
@@ -922,7 +944,7 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
             });
         });
     int sorted = 0;
-    if (n <= kSortTile) {
+    if (n <= kSmallSort) {
         const int64_t words = accumulate ? 0 : table_grads->rows * table_grads->dim;
         const int fillers = (int)std::min<int64_t>(ceil_div(words, kSmallThreads * 8), 4 * kSMs);
         k_sort_small<<<1 + fillers, kSmallThreads, 0, stream>>>(src, zero, L.bits, items(0), at(L.valid));
@@ -930,26 +952,36 @@ GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices,
     } else {
         SortPass p{at(L.first_keys), nullptr, nullptr, at(L.hist), at(L.totals), at(L.valid), (int32_t)n, L.ntiles, 0, 0};
         const int digit = (L.bits + L.passes - 1) / L.passes;
-        const size_t smem = radix_scatter_smem(digit);
-        GS3D_CUDA(cudaFuncSetAttribute(k_radix_scatter, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)radix_scatter_smem(kMaxDigitBits)),
-                  "scatter smem attribute");
-        for (int i = 0; i < L.passes; ++i) {
-            p.shift = i * digit;
-            p.bits = digit;
-            p.out = items(i & 1);
-            if (i == 0) {  // behind whatever wrote the inputs
-                k_radix_count<<<L.ntiles, kSortThreads, 0, stream>>>(p, src, zero);
-                GS3D_LAUNCHED("k_radix_count");
-            } else {
-                GS3D_RETURN_IF(launch_after("k_radix_count", k_radix_count, dim3(L.ntiles), kSortThreads, 0, stream, p,
-                                            src, zero));
+        GS3D_RETURN_IF(dispatch_rounds(sort_rounds(n), [&](auto rounds) {
+            constexpr int R = decltype(rounds)::value;
+            const size_t smem = radix_scatter_smem(R, digit);
+            if (smem > (48u << 10))
+                GS3D_CUDA(cudaFuncSetAttribute(k_radix_scatter<R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)radix_scatter_smem(R, kMaxDigitBits)),
+                          "scatter smem attribute");
+            // few tiles leave SMs that zero the table: a block for 16 KB of it
+            const int64_t zeroed = accumulate ? 0 : table_grads->rows * table_grads->dim;
+            const int fillers = (int)std::min<int64_t>(ceil_div(zeroed, 1 << 12), std::max(0, 4 * kSMs - L.ntiles));
+            for (int i = 0; i < L.passes; ++i) {
+                p.shift = i * digit;
+                p.bits = digit;
+                p.out = items(i & 1);
+                if (i == 0) {  // behind whatever wrote the inputs
+                    k_radix_count<R><<<L.ntiles + fillers, kSortThreads, 0, stream>>>(p, src, zero);
+                    GS3D_LAUNCHED("k_radix_count");
+                } else {
+                    GS3D_RETURN_IF(launch_after("k_radix_count", k_radix_count<R>, dim3(L.ntiles), kSortThreads, 0,
+                                                stream, p, src, zero));
+                }
+                GS3D_RETURN_IF(
+                    launch_after("k_radix_spine", k_radix_spine, dim3(1 << digit), kSpineThreads, 0, stream, p));
+                GS3D_RETURN_IF(launch_after("k_radix_scatter", k_radix_scatter<R>, dim3(L.ntiles), kSortThreads, smem,
+                                            stream, p));
+                p.in = p.out;
+                sorted = i & 1;
             }
-            GS3D_RETURN_IF(launch_after("k_radix_spine", k_radix_spine, dim3(1 << digit), kSpineThreads, 0, stream, p));
-            GS3D_RETURN_IF(launch_after("k_radix_scatter", k_radix_scatter, dim3(L.ntiles), kSortThreads, smem, stream, p));
-            p.in = p.out;
-            sorted = i & 1;
-        }
+            return GS3D_OK;
+        }));
     }
     if (n == 0) return GS3D_OK;
     const Segments seg{items(sorted), at(L.valid), out, table_grads->row_stride, scale,

@@ -109,7 +109,7 @@ def table_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 1.0,
     handle, context = _enter(device, stream)
     try:
         if out is None:
-            out = torch.empty(shape, dtype=dtype or table.dtype, device=device)
+            out = table.new_empty(shape, dtype=dtype)
         elif out.shape != shape or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a lookup of {shape} {dtype or out.dtype}")
         o = _rows_c(out, "out")
@@ -143,12 +143,12 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
     handle, context = _enter(device, stream)
     try:
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=device)
+            out = grads.new_empty(shape, dtype=torch.float32)
         elif out.shape != shape or out.dtype != torch.float32:
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a float32 table gradient of {shape}")
         o = _rows_c(out, "out")
         nbytes = _gradient_workspace_bytes(g.rows, o.rows, g.dim)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = grads.new_empty(nbytes, dtype=torch.uint8)
         _abi.check(_abi.lib().gs3d_table_gradient(
             g, indices.data_ptr(), indices.shape[0],
             None if fgidx_to_gidx is None else fgidx_to_gidx.data_ptr(),
@@ -167,7 +167,7 @@ def mx4_tensor_scale(x: torch.Tensor, stream: torch.cuda.Stream | None = None) -
     c = _rows_c(x, "x")
     handle, context = _enter(device, stream)
     try:
-        scale = torch.empty(1, dtype=torch.float32, device=device)
+        scale = x.new_empty(1, dtype=torch.float32)
         _abi.check(_abi.lib().gs3d_mx4_tensor_scale(c, scale.data_ptr(), handle))
     finally:
         _leave(context)
@@ -185,13 +185,13 @@ def mx4_quantise(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Ten
     try:
         if format == "nvfp4":
             if tensor_scale is None:
-                tensor_scale = torch.empty(1, dtype=torch.float32, device=device)
+                tensor_scale = x.new_empty(1, dtype=torch.float32)
                 _abi.check(_abi.lib().gs3d_mx4_tensor_scale(c, tensor_scale.data_ptr(), handle))
             elif tensor_scale.numel() != 1 or tensor_scale.dtype != torch.float32:
                 raise ValueError("the tensor scale is (1,) float32")
         elif tensor_scale is not None:
             raise ValueError(f"{format} rows have no tensor scale")
-        q = MX4Rows.empty(c.rows, c.dim, format, device, tensor_scale)
+        q = MX4Rows.empty_beside(x, c.rows, c.dim, format, tensor_scale)
         _abi.check(_abi.lib().gs3d_mx4_quantise(c, q.to_c(), handle))
     finally:
         _leave(context)
@@ -205,7 +205,7 @@ def mx4_dequantise(rows: MX4Rows, dtype: torch.dtype = torch.float32, out: torch
     handle, context = _enter(device, stream)
     try:
         if out is None:
-            out = torch.empty((rows.rows, rows.dim), dtype=dtype, device=device)
+            out = rows.codes.new_empty((rows.rows, rows.dim), dtype=dtype)
         _abi.check(_abi.lib().gs3d_mx4_dequantise(rows.to_c(), _rows_c(out, "out"), handle))
     finally:
         _leave(context)
@@ -233,7 +233,7 @@ def mx4_colours(rows: MX4Rows, means: torch.Tensor, positions, sh_degree: int,
     handle, context = _enter(device, stream)
     try:
         if out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=device)
+            out = means.new_empty(shape)
         elif out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous float32 tensor of shape {shape}")
         _abi.check(_abi.lib().gs3d_mx4_colours(

@@ -408,11 +408,16 @@ class MX4Rows:
 
     @classmethod
     def empty(cls, rows: int, dim: int, format: str, device, tensor_scale=None) -> "MX4Rows":
+        return cls.empty_beside(torch.empty(0, device=device), rows, dim, format, tensor_scale)
+
+    @classmethod
+    def empty_beside(cls, t: torch.Tensor, rows: int, dim: int, format: str, tensor_scale=None) -> "MX4Rows":
+        """`empty` on `t`'s device."""
         if format not in MX4_FORMATS:
             raise ValueError(f"4-bit format {format!r} is not in {sorted(MX4_FORMATS)}")
         q = object.__new__(cls)  # right by construction: not checked again
-        q.codes = torch.empty((rows, (dim + 1) // 2), dtype=torch.uint8, device=device)
-        q.scales = torch.empty((rows, -(-dim // MX4_FORMATS[format][1])), dtype=torch.uint8, device=device)
+        q.codes = t.new_empty((rows, (dim + 1) // 2), dtype=torch.uint8)
+        q.scales = t.new_empty((rows, -(-dim // MX4_FORMATS[format][1])), dtype=torch.uint8)
         q.tensor_scale, q.dim, q.format = tensor_scale, dim, format
         return q
 

@@ -146,6 +146,31 @@ def test_gradient_units(cuda, n, dim, stride, offset, kind):
     assert ((got.cpu().double() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("n", [1, 30, 1000])
+@pytest.mark.parametrize("rows,dim,out_stride", [(3, 1, 1), (60_000, 48, 48), (60_000, 48, 52), (5_000, 27, 29),
+                                                 (17_000_000, 2, 2), (900, 130, 132), (40_000, 3, 4)])
+def test_gradient_of_few_rows_zeroes_the_rest(cuda, n, rows, dim, out_stride):
+    gen = rng(n + rows)
+    grads = torch.randn(n, dim, generator=gen)
+    idx = make_indices(n, rows, gen)
+    idx[-1] = rows
+    buf = torch.full((rows * out_stride,), 5.0, device=cuda)
+    out = torch.as_strided(buf, (rows, dim), (out_stride, 1))
+    gc.table_gradient(grads.to(cuda), idx.to(cuda), rows, out=out)
+    named = idx[(idx >= 1) & (idx <= rows)].long().unique() - 1
+    assert int((out != 0).any(dim=1).sum()) <= len(named)
+    keep = torch.ones(rows, dtype=torch.bool, device=cuda)
+    keep[named.to(cuda)] = False
+    assert (out[keep] == 0).all()
+    order = torch.full((rows + 1,), 0, dtype=torch.int64)
+    order[named + 1] = torch.arange(1, len(named) + 1)
+    safe = torch.where((idx >= 1) & (idx <= rows), idx.long(), 0)
+    want, bound = gradient_exact(grads, order[safe].to(torch.int32), len(named), 1.0)
+    assert ((out[named.to(cuda)].cpu().double() - want).abs() <= bound).all()
+    if out_stride > dim:
+        assert (torch.as_strided(buf, (rows, out_stride - dim), (out_stride, 1), dim) == 5.0).all()
+
+
 @pytest.mark.parametrize("n", [303_104, 303_105, 606_208, 606_209])
 @pytest.mark.parametrize("rows", [700, 90_000])
 def test_gradient_sizes_where_the_tiles_change(cuda, n, rows):

@@ -676,6 +676,37 @@ __global__ void __launch_bounds__(256, VB == 16 ? 4 : 5)
 // also zeroes, of its share of the table, the rows without gradients.
 constexpr int kTinyRows = 1024, kTinyThreads = 256;
 
+// Zeroes the rows first .. last - 1 of the table that no item names: marks those that are named, kZeroRows
+// rows a turn, and leaves each row to 16 bytes (or an element) a thread of as many threads side by side
+// (1,000 rows into 60,000 of 48: 12.6 us, 24.7 with a search and a thread a row).
+constexpr int kZeroRows = 16384;
+
+__device__ __forceinline__ void zero_unused(const ZeroRows& z, const int2* items, int count, int64_t first,
+                                            int64_t last, uint32_t* used) {
+    const bool wide = ((z.stride | z.dim) & 3) == 0 && (reinterpret_cast<uintptr_t>(z.data) & 15) == 0;
+    const int units = wide ? z.dim / 4 : z.dim, side = min(32, 1 << (32 - __clz(units - 1 | 1)));
+    const int lane = threadIdx.x & (side - 1);
+    for (int64_t r = first; r < last; r += kZeroRows) {
+        const int m = (int)min((int64_t)kZeroRows, last - r);
+        for (int i = threadIdx.x; i < (m + 31) / 32; i += kTinyThreads) used[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += kTinyThreads) {
+            const int64_t k = items[i].x - r;
+            if (k >= 0 && k < m) atomicOr(used + (k >> 5), 1u << (k & 31));
+        }
+        __syncthreads();
+        for (int k = threadIdx.x / side; k < m; k += kTinyThreads / side) {
+            if ((used[k >> 5] >> (k & 31)) & 1u) continue;
+            float* row = z.data + (r + k) * z.stride;
+            for (int c = lane; c < units; c += side) {
+                if (wide) reinterpret_cast<float4*>(row)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                else row[c] = 0.0f;
+            }
+        }
+        __syncthreads();
+    }
+}
+
 __device__ __forceinline__ int first_above(const int2* items, int n, int key) {
     int lo = 0, hi = n;
     while (lo < hi) {
@@ -695,17 +726,11 @@ __global__ void __launch_bounds__(kTinyThreads) k_table_gradient_tiny(const T* _
     __shared__ int2 items[kTinyRows];
     __shared__ uint16_t wcount[kTinyThreads / 32][256];
     __shared__ int start[256], sm[33];
+    __shared__ uint32_t used[kZeroRows / 32];
     const int count = sort_rows<kTinyThreads, kTinyRows / kTinyThreads>(src, bits, items, wcount, start, sm);
     const int64_t b = blockIdx.x, blocks = gridDim.x;
-    if (zero.data && blockIdx.y == 0) {
-        const int side = dim > 128 ? 32 : 1;  // a row a thread, long ones a warp
-        for (int64_t k = b * zero.rows / blocks + threadIdx.x / side; k < (b + 1) * zero.rows / blocks;
-             k += kTinyThreads / side) {
-            const int p = first_above(items, count, (int)k);
-            if (p == 0 || items[p - 1].x != k)
-                for (int c = threadIdx.x % side; c < dim; c += side) zero.data[k * zero.stride + c] = 0.0f;
-        }
-    }
+    if (zero.data && blockIdx.y == 0)
+        zero_unused(zero, items, count, b * zero.rows / blocks, (b + 1) * zero.rows / blocks, used);
     int p0 = (int)(b * count / blocks), p1 = (int)((b + 1) * count / blocks);
     if (p0 > 0) p0 = first_above(items, count, items[p0 - 1].x);
     if (p1 > 0) p1 = first_above(items, count, items[p1 - 1].x);

@@ -86,6 +86,21 @@ def test_gradient_workspace_grows_with_the_rows():
         last = size.value
 
 
+@pytest.mark.parametrize("dim", [1, 3, 27, 48, 119, 130, 1021, 65536])
+@pytest.mark.parametrize("table_rows", [1, 1000, 65_536, 3_000_000])
+def test_gradient_workspace_serves_fewer_rows(dim, table_rows):
+    """A workspace for n rows is large enough for any smaller number: tiles and chunks change with n."""
+    sizes, size = [], C.c_size_t(0)
+    steps = sorted({max(0, a + d) for a in [*range(0, 30_000, 501), *(1024 * k for k in range(1, 1300, 7)), 303_104, 606_208,
+                                            *(592 * 4 * s for s in (1, 2, 21, 32)), *(2368 * 48 * s for s in (1, 2, 5, 18, 21)),
+                                            *(2368 * 49 * s for s in (1, 2, 5, 18, 21)), 3_000_000, 1 << 24, 1 << 30]
+                    for d in (-1, 0, 1) if a + d <= 1 << 30})
+    for n in steps:
+        _abi.check(LIB.gs3d_table_gradient_workspace_size(n, table_rows, dim, C.byref(size)))
+        sizes.append(size.value)
+    assert sizes == sorted(sizes)
+
+
 @pytest.mark.parametrize("bad,word", [(dict(n=-1), "rows"), (dict(n=BIG), "rows"), (dict(dim=0), "dim"),
                                       (dict(fmt=2), "format"), (dict(codes=None), "NULL"),
                                       (dict(scales=None), "NULL"), (dict(ts=None), "NULL tensor scale")])

@@ -840,6 +840,16 @@ int sort_rounds(int64_t n) {
     return n <= 2 * kSMs * 2 * kSortThreads ? 2 : (n <= 2 * kSMs * 4 * kSortThreads ? 4 : 8);
 }
 
+// The most tiles that n rows or fewer are cut into.
+int most_tiles(int64_t n) {
+    int64_t most = 0;
+    for (int rounds = 2; rounds <= 8; rounds *= 2) {
+        const int64_t last = rounds < 8 ? std::min<int64_t>(n, 2 * kSMs * rounds * kSortThreads) : n;
+        most = std::max(most, ceil_div(last, rounds * kSortThreads));
+    }
+    return (int)most;
+}
+
 template <typename F>
 int dispatch_rounds(int rounds, F&& f) {
     switch (rounds) {
@@ -847,6 +857,13 @@ int dispatch_rounds(int rounds, F&& f) {
         case 4: return f(std::integral_constant<int, 4>{});
         default: return f(std::integral_constant<int, 8>{});
     }
+}
+
+// The most chunks that n rows or fewer are cut into.
+int most_chunks(int64_t n, int units) {
+    const int64_t s = slots_for(std::min(units, 256));
+    const int64_t few = std::max<int64_t>(kSMs * 4, ceil_div(n, s * kMaxRun));
+    return (int)std::max(std::min({ceil_div(n, s * kMinRun), few, (int64_t)kSMs * 16}), ceil_div(n, s * (kMaxChunk / s)));
 }
 
 int bits_of(int64_t v) {
@@ -861,16 +878,16 @@ GradLayout grad_layout(int64_t n, int64_t rows, int dim) {
     L.bits = bits_of(std::max<int64_t>(rows, 1) - 1);
     L.passes = std::max(1, (L.bits + kMaxDigitBits - 1) / kMaxDigitBits);
     const int digit = (L.bits + L.passes - 1) / L.passes;
-    // the launch picks its unit from the gradients' alignment: room for either
-    L.chunks_max = 0;
+    // the launch picks its unit from the gradients' alignment, and fewer rows other tiles and chunks: room for all
+    L.chunks_max = 1;
     for (int units = dim; units >= 1; units = units % 2 == 0 ? units / 2 : 0)
-        L.chunks_max = std::max(L.chunks_max, segment_plan(n, units).nchunks);
+        L.chunks_max = std::max(L.chunks_max, most_chunks(n, units));
     size_t off = 0;
     L.first_keys = off; off += align256((size_t)n * 4);
     for (int i = 0; i < 2; ++i) {
         L.items[i] = off; off += i < L.passes ? align256((size_t)n * 8) : 0;
     }
-    L.hist = off; off += align256((size_t)L.ntiles * ((size_t)1 << digit) * 4);
+    L.hist = off; off += align256((size_t)most_tiles(n) * ((size_t)1 << digit) * 4);
     L.totals = off; off += align256(((size_t)1 << kMaxDigitBits) * 4);
     L.valid = off; off += 256;
     L.first_key = off; off += align256((size_t)L.chunks_max * 4);

@@ -622,7 +622,8 @@ struct Positions {
 // used, of some 520 instructions a pair 180 decode), by the stores with several (500K at degree 2, 8 views:
 // 17 us, 11.5 for the bytes).
 // Blocks an SM: a single view in whole rows holds one channel at a time, 72 registers and 7 blocks (33.4 us;
-// 35.5 left to the compiler); several views hold all elements of both Gaussians, 3 blocks at degree 3.
+// 35.5 left to the compiler); several views hold all elements of both Gaussians (degree 3 with 2 / 3 / 4 / 5
+// blocks: 479K and 7 views 21.8 / 18.4 / 21.3 / 34.6 us, 916K and 4 views 26.5 / 26.4 / 24.8 / 35.2).
 template <int DEG, bool WHOLE, bool ONE>
 constexpr int colour_blocks() { return ONE && WHOLE ? 7 : (DEG == 3 ? 3 : 5); }
 

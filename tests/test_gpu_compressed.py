@@ -146,6 +146,27 @@ def test_gradient_units(cuda, n, dim, stride, offset, kind):
     assert ((got.cpu().double() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("n", [1025, 8191, 8192, 8193, 16_383, 16_384, 16_385])
+@pytest.mark.parametrize("rows", [1, 256, 257, 65_536, 65_537, (1 << 24) + 1])
+def test_gradient_sizes_of_the_cluster_sort(cuda, n, rows):
+    """One or two rows a thread of a cluster, one to four passes of 8 bits; filtered rows; equal bits again."""
+    gen = rng(n + rows)
+    grads = torch.randn(n, 2, generator=gen)
+    idx = make_indices(n, rows, gen, 0.5)
+    out = torch.full((rows, 2), 7.0, device=cuda)
+    gc.table_gradient(grads.to(cuda), idx.to(cuda), rows, out=out)
+    want, bound = gradient_exact(grads, idx, rows, 1.0)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    live = n - n // 5
+    f2g = (torch.randperm(n, generator=gen) + 1).to(torch.int32)
+    counts = torch.tensor([live, 0, 0, 0], dtype=torch.int32)
+    a = gc.table_gradient(grads.to(cuda), idx.to(cuda), rows, fgidx_to_gidx=f2g.to(cuda), device_counts=counts.to(cuda))
+    want, bound = gradient_exact(grads, idx, rows, 1.0, f2g, live)
+    assert ((a.cpu().double() - want).abs() <= bound).all()
+    b = gc.table_gradient(grads.to(cuda), idx.to(cuda), rows, fgidx_to_gidx=f2g.to(cuda), device_counts=counts.to(cuda))
+    assert torch.equal(a.view(torch.int32), b.view(torch.int32))
+
+
 @pytest.mark.parametrize("n", [1, 30, 1000])
 @pytest.mark.parametrize("rows,dim,out_stride", [(3, 1, 1), (60_000, 48, 48), (60_000, 48, 52), (5_000, 27, 29),
                                                  (17_000_000, 2, 2), (900, 130, 132), (40_000, 3, 4)])
@@ -201,8 +222,7 @@ def test_gradient_of_long_runs(cuda, n, dim):
 @pytest.mark.parametrize("n", [1023, 1024, 1025, 4095, 4096, 4097, 8193])
 @pytest.mark.parametrize("rows", [1, 2, 256, 257, 1024, 1025, 70_000, (1 << 20) + 1])
 def test_gradient_sizes_where_the_sort_changes(cuda, n, rows):
-    """One launch up to 1024 rows, one sorting block up to 4096, then tiles of 4096; digits of 8 and 10
-    bits, one to three passes."""
+    """One launch up to 1024 rows, then one cluster that sorts; one to three passes of 8 bits."""
     gen = rng(n + rows)
     grads = torch.randn(n, 4, generator=gen)
     idx = make_indices(n, rows, gen)

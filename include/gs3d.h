@@ -568,7 +568,7 @@ GS3D_API int gs3d_table_lookup(const gs3d_rows* table, const int32_t* indices, f
 #define GS3D_TABLE_ACCUMULATE 1u /* add to table_grads instead of overwriting them */
 
 /* Bytes of workspace gs3d_table_gradient needs for at most grad_rows rows of gradients of dim
- * elements and a table of table_rows rows. */
+ * elements and a table of table_rows rows; 0 up to 1024 rows (the workspace may then be NULL). */
 GS3D_API int gs3d_table_gradient_workspace_size(int64_t grad_rows, int64_t table_rows, int32_t dim,
                                                 size_t* bytes);
 

@@ -67,11 +67,12 @@ def test_gradient_refusals():
     refused(call(n_idx=3), "3 indices for 4 rows")
     refused(call(n_idx=-1, f2g=DATA), "indices")
     refused(call(idx=None), "NULL indices")
-    refused(call(ws=DATA + 128), "aligned")
+    many = dict(g=rows(n=1025), n_idx=1025)
+    refused(call(ws=DATA + 128, **many), "aligned")
     size = C.c_size_t(0)
-    _abi.check(LIB.gs3d_table_gradient_workspace_size(4, 7, 48, C.byref(size)))
-    assert call(nbytes=size.value - 1) == _abi.GS3D_ERR_WORKSPACE
-    assert call(ws=None) == _abi.GS3D_ERR_WORKSPACE
+    _abi.check(LIB.gs3d_table_gradient_workspace_size(1025, 7, 48, C.byref(size)))
+    assert call(nbytes=size.value - 1, **many) == _abi.GS3D_ERR_WORKSPACE
+    assert call(ws=None, **many) == _abi.GS3D_ERR_WORKSPACE
     assert call(t=rows(n=0, data=None)) == _abi.GS3D_OK
     refused(LIB.gs3d_table_gradient_workspace_size(4, 7, 48, None), "NULL")
     for bad in ((-1, 7, 48), (BIG, 7, 48), (4, -1, 48), (4, BIG, 48), (4, 7, 0)):
@@ -80,9 +81,9 @@ def test_gradient_refusals():
 
 def test_gradient_workspace_grows_with_the_rows():
     size, last = C.c_size_t(0), 0
-    for n in (0, 1, 1000, 100_000, 3_000_000, 1 << 30):
+    for n in (0, 1, 1024, 1025, 100_000, 3_000_000, 1 << 30):
         _abi.check(LIB.gs3d_table_gradient_workspace_size(n, 65_536, 48, C.byref(size)))
-        assert size.value >= max(last, 4 * n)
+        assert size.value >= max(last, 4 * n) if n > 1024 else size.value == 0
         last = size.value
 
 

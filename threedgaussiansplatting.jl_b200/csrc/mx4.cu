@@ -70,7 +70,8 @@ __device__ __forceinline__ float larger(__half2 m) { return fmaxf(__low2float(m)
 __device__ __forceinline__ float larger(__nv_bfloat162 m) { return fmaxf(__low2float(m), __high2float(m)); }
 template <typename T>
 using Word = typename std::conditional<
-    sizeof(T) == 4, float, typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type>::type;
+    sizeof(T) == 4, float,
+    typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type>::type;
 
 // Every block turns its largest magnitude into the scale it asks for (monotone, positive: fp32 bits
 // order like unsigned integers) and the largest one stays; a lone block stores it. A maximum does not
@@ -226,7 +227,8 @@ struct TensorScale {
 // A block's scale byte and the codes of its first EL elements v (zeros behind the row's end), two a byte,
 // in words of eight. EL < block size: rows of at most EL elements.
 template <int FMT, int EL>
-__device__ __forceinline__ uint32_t quantise_block(const float (&v)[EL], const TensorScale& t, uint32_t (&words)[EL / 8]) {
+__device__ __forceinline__ uint32_t quantise_block(const float (&v)[EL], const TensorScale& t,
+                                                   uint32_t (&words)[EL / 8]) {
     float a = fabsf(v[0]);
 #pragma unroll
     for (int k = 1; k < EL; ++k) a = max_abs(a, v[k]);
@@ -389,10 +391,10 @@ __global__ void __launch_bounds__(256) k_mx4_quantise(const T* __restrict__ x, i
 }
 
 // ---- dequantise ------------------------------------------------------------------------------
-// Rows of packs of N elements (16 bytes, or four), back to back: the codes and values of all rows are one run each. A thread fills
-// kDequantisePacks packs of output, next to its neighbours' each time. WHOLE: rows of whole blocks,
-// whose scales are one run too. Bound by memory: 3M x 48 fp32 97 us (657 MB, 6.7 TB/s); 139 with one pack a
-// thread, 152 with the packs of a thread side by side.
+// Rows of packs of N elements (16 bytes, or four), back to back: the codes and values of all rows are one
+// run each. A thread fills kDequantisePacks packs of output, next to its neighbours' each time. WHOLE: rows
+// of whole blocks, whose scales are one run too. Bound by memory: 3M x 48 fp32 97 us (657 MB, 6.7 TB/s); 139
+// with one pack a thread, 152 with the packs of a thread side by side.
 constexpr int kDequantisePacks = 4;
 
 template <typename T, int FMT, int N, bool WHOLE>
@@ -717,7 +719,8 @@ struct ColoursLaunch {
             k_mx4_colours<DEG, FMT, WHOLE, true><<<grid, 128, 0, stream>>>(a, order, mo4, n, cv, nv, 1, out, view_stride);
         } else {
             // all views a block, unless that leaves SMs without: then as many shares of them as fill two waves
-            const int shares = (int)std::min<int64_t>(nv, std::max<int64_t>(1, 2 * 6 * (int64_t)device_sm_count() / grid));
+            const int64_t waves = 2 * 6 * (int64_t)device_sm_count();
+            const int shares = (int)std::min<int64_t>(nv, std::max<int64_t>(1, waves / grid));
             const int views = (int)ceil_div(nv, shares);
             k_mx4_colours<DEG, FMT, WHOLE, false><<<dim3(grid, (unsigned)ceil_div(nv, views)), 128, 0, stream>>>(
                 a, order, mo4, n, cv, nv, views, out, view_stride);

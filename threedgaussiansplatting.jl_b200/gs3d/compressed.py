@@ -148,12 +148,13 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a float32 table gradient of {shape}")
         o = _rows_c(out, "out")
         nbytes = _gradient_workspace_bytes(g.rows, o.rows, g.dim)
-        ws = grads.new_empty(nbytes, dtype=torch.uint8)
+        ws = grads.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _abi.check(_abi.lib().gs3d_table_gradient(
             g, indices.data_ptr(), indices.shape[0],
             None if fgidx_to_gidx is None else fgidx_to_gidx.data_ptr(),
             None if device_counts is None else device_counts.data_ptr(), scale, o,
-            _abi.GS3D_TABLE_ACCUMULATE if accumulate else 0, ws.data_ptr(), nbytes, handle))
+            _abi.GS3D_TABLE_ACCUMULATE if accumulate else 0, ws.data_ptr() if nbytes else None, nbytes,
+            handle))
     finally:
         _leave(context)
     return out

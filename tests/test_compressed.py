@@ -213,6 +213,24 @@ def test_mx4_rows_checks():
         MX4Rows.empty(3, 48, "int4", "cpu")
 
 
+def test_a_tensor_scale_of_another_device_or_type_never_reaches_a_kernel():
+    """A kernel follows the pointer: a scale in host memory beside codes on the GPU would fault it."""
+    for fmt, device, ts in (("nvfp4", "meta", torch.ones(1)), ("nvfp4", "cpu", torch.ones(1).double()),
+                            ("nvfp4", "cpu", torch.ones(2)), ("mxfp4", "cpu", torch.ones(1))):
+        with pytest.raises(ValueError, match="scale"):
+            MX4Rows.empty(3, 48, fmt, device, ts)
+        q = MX4Rows.empty(3, 48, fmt, device)  # without one for now
+        if fmt == "nvfp4":
+            q.tensor_scale = ts
+            with pytest.raises(ValueError, match="scale"):
+                q.to_c()
+    assert MX4Rows.empty(3, 48, "nvfp4", "cpu", torch.ones(1)).to_c().tensor_scale
+    q = MX4Rows.empty(3, 48, "mxfp4", "cpu")
+    q.scales = q.scales.to("meta")
+    with pytest.raises(ValueError, match="one device"):
+        q.to_c()
+
+
 def test_compressed_gaussians_checks():
     q = MX4Rows.empty(6, 48, "mxfp4", "cpu")
     mo, cov, idx = torch.zeros(6, 4), torch.zeros(6, 6), torch.ones(6, dtype=torch.int32)

@@ -397,22 +397,34 @@ class MX4Rows:
             raise ValueError(f"codes {tuple(self.codes.shape)} and scales {tuple(self.scales.shape)} "
                              f"are not those of {self.format} rows of {dim} elements")
         for t in (self.codes, self.scales):
-            if t.dtype != torch.uint8 or not t.is_contiguous() or t.device != self.codes.device:
+            if t.dtype != torch.uint8 or not t.is_contiguous():
                 raise ValueError("codes and scales must be contiguous uint8 tensors on one device")
-        ts = self.tensor_scale
-        if self.format == "nvfp4":
-            if ts is None or ts.numel() != 1 or ts.dtype != torch.float32 or ts.device != self.codes.device:
-                raise ValueError("nvfp4 rows need a (1,) float32 tensor scale on their device")
-        elif ts is not None:
-            raise ValueError("mxfp4 rows have no tensor scale")
+        if self.format == "nvfp4" and self.tensor_scale is None:
+            raise ValueError("nvfp4 rows need a (1,) float32 tensor scale on their device")
+        self._check_memory()
+
+    def _check_memory(self) -> None:
+        """Kernels follow these pointers: all on the codes' device, the scale of the type they read."""
+        device, ts = self.codes.device, self.tensor_scale
+        if self.scales.device != device:
+            raise ValueError("codes and scales must be contiguous uint8 tensors on one device")
+        if ts is None:
+            return
+        if self.format != "nvfp4":
+            raise ValueError(f"{self.format} rows have no tensor scale")
+        if ts.device != device or ts.dtype != torch.float32 or ts.numel() != 1:
+            raise ValueError("nvfp4 rows need a (1,) float32 tensor scale on their device")
 
     @classmethod
     def empty(cls, rows: int, dim: int, format: str, device, tensor_scale=None) -> "MX4Rows":
-        return cls.empty_beside(torch.empty(0, device=device), rows, dim, format, tensor_scale)
+        """Rows to be written (nvfp4 ones need their `tensor_scale` before a call takes them)."""
+        q = cls.empty_beside(torch.empty(0, device=device), rows, dim, format, tensor_scale)
+        q._check_memory()
+        return q
 
     @classmethod
     def empty_beside(cls, t: torch.Tensor, rows: int, dim: int, format: str, tensor_scale=None) -> "MX4Rows":
-        """`empty` on `t`'s device."""
+        """`empty` on `t`'s device; the scale is not checked here."""
         if format not in MX4_FORMATS:
             raise ValueError(f"4-bit format {format!r} is not in {sorted(MX4_FORMATS)}")
         q = object.__new__(cls)  # right by construction: not checked again
@@ -439,6 +451,7 @@ class MX4Rows:
                        None if ts is None else ts.to(device), self.dim, self.format)
 
     def to_c(self) -> _abi.MX4RowsC:
+        self._check_memory()  # again: the fields can be assigned
         ts = self.tensor_scale
         return _abi.MX4RowsC(self.codes.shape[0], self.dim, MX4_FORMATS[self.format][0], self.codes.data_ptr(),
                              self.scales.data_ptr(), None if ts is None else ts.data_ptr())

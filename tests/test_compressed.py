@@ -256,6 +256,23 @@ def test_rows_of_a_tensor():
             gc._rows_c(bad, "t")
 
 
+def test_sizes_that_do_not_fit_the_calls_fields_are_refused():
+    """The library takes a row's length and the number of Gaussians as 32 bits: what does not fit must not
+    come out as the small number that its low bits are."""
+    big = 1 << 32
+    meta = lambda *s, **k: torch.empty(s, device="meta", **k)  # noqa: E731
+    for t in (meta(1, big + 48), meta(2, 3, big // 2 + 16), meta(1, (1 << 16) + 1)):
+        with pytest.raises(ValueError, match="elements a row"):
+            gc._rows_c(t, "t")
+    assert gc._rows_c(meta(1, 1 << 16), "t").dim == 1 << 16
+    u8 = dict(dtype=torch.uint8)
+    q = MX4Rows(meta(1, big // 2 + 24, **u8), meta(1, big // 32 + 2, **u8), None, big + 48, "mxfp4")
+    with pytest.raises(ValueError, match="elements a row"):
+        q.to_c()
+    with pytest.raises(ValueError, match="Gaussians"):
+        gc.mx4_colours(MX4Rows.empty(4, 48, "mxfp4", "meta"), meta(big + 4, 4), [[0.0, 0.0, 0.0]], 3)
+
+
 def test_calls_need_cuda_tensors_of_the_right_kind():
     t, i = torch.zeros(4, 48), torch.ones(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):

@@ -33,6 +33,7 @@ GS3D_F32 = 0
 GS3D_F16 = 1
 GS3D_BF16 = 2
 GS3D_TABLE_ACCUMULATE = 1
+GS3D_MAX_ROW_DIM = 1 << 16
 GS3D_NVFP4 = 0
 GS3D_MXFP4 = 1
 

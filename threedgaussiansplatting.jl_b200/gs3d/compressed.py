@@ -38,6 +38,8 @@ def _rows_c(t: torch.Tensor, what: str) -> _abi.RowsC:
     rows, dim = shape[0], shape[1]
     for size in shape[2:]:
         dim *= size
+    if dim > _abi.GS3D_MAX_ROW_DIM:  # the C field has 32 bits and would take the low ones
+        raise ValueError(f"{what}: {dim} elements a row (at most {_abi.GS3D_MAX_ROW_DIM})")
     if t.is_contiguous():
         return _abi.RowsC(rows, dim, dim, kind, t.data_ptr())
     expect = 1
@@ -224,8 +226,10 @@ def mx4_colours(rows: MX4Rows, means: torch.Tensor, positions, sh_degree: int,
     if pos.ndim != 2 or pos.shape[1] != 3:
         raise ValueError(f"positions must be (views, 3), got {pos.shape}")
     _check_indices(indices)
-    device = _check_device(rows.codes, means, indices, out)
     n = means.shape[0]
+    if n >= 1 << 31:  # the C argument has 32 bits and would take the low ones
+        raise ValueError(f"{n} Gaussians (below 2^31)")
+    device = _check_device(rows.codes, means, indices, out)
     if means.shape != (n, 4) or means.dtype != torch.float32 or not means.is_contiguous():
         raise ValueError("means must be a contiguous (n, 4) float32 tensor")
     if indices is not None and indices.shape[0] != n:

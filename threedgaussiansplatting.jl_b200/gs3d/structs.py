@@ -452,6 +452,8 @@ class MX4Rows:
 
     def to_c(self) -> _abi.MX4RowsC:
         self._check_memory()  # again: the fields can be assigned
+        if self.dim > _abi.GS3D_MAX_ROW_DIM:  # the C field has 32 bits and would take the low ones
+            raise ValueError(f"{self.dim} elements a row (at most {_abi.GS3D_MAX_ROW_DIM})")
         ts = self.tensor_scale
         return _abi.MX4RowsC(self.codes.shape[0], self.dim, MX4_FORMATS[self.format][0], self.codes.data_ptr(),
                              self.scales.data_ptr(), None if ts is None else ts.data_ptr())

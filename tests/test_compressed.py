@@ -273,6 +273,18 @@ def test_sizes_that_do_not_fit_the_calls_fields_are_refused():
         gc.mx4_colours(MX4Rows.empty(4, 48, "mxfp4", "meta"), meta(big + 4, 4), [[0.0, 0.0, 0.0]], 3)
 
 
+def test_table_gradient_of_larger_gradient_buffers(monkeypatch):
+    """backward() takes gradient buffers with room for more Gaussians than the render's; so does the table."""
+    from types import SimpleNamespace
+    seen = []
+    monkeypatch.setattr(gc, "table_gradient", lambda g, *a: seen.append((g.shape, a[5].shape)))
+    table = gc.SHTable(torch.zeros(2, 3, 4), torch.ones(6, dtype=torch.int32))
+    for room, n in ((9, 6), (6, 6), (6, 9)):
+        table.gradient(SimpleNamespace(sh_coeffs_grads=torch.zeros(room, 3, 4)),
+                       SimpleNamespace(fgidx_to_gidx=torch.zeros(n, dtype=torch.int32), device_counts=torch.zeros(4, dtype=torch.int32)))
+    assert seen == [((6, 3, 4), (6,)), ((6, 3, 4), (6,)), ((6, 3, 4), (9,))]
+
+
 def test_calls_need_cuda_tensors_of_the_right_kind():
     t, i = torch.zeros(4, 48), torch.ones(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):

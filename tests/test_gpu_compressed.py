@@ -907,6 +907,20 @@ def test_table_trainer_step_is_its_parts(cuda):
     assert torch.equal(g.sh_coeffs, expanded)  # what this step rendered
 
 
+def test_table_gradient_of_larger_gradient_buffers(cuda):
+    """backward() takes gradient buffers with room for more Gaussians than the render's."""
+    from types import SimpleNamespace
+    gen = rng(21)
+    n, rows = 2000, 30
+    table = gc.SHTable(torch.randn(rows, 3, 16, generator=gen).to(cuda), make_indices(n, rows, gen).to(cuda), 0.5)
+    grads = torch.randn(n + 700, 3, 16, generator=gen).to(cuda)
+    f2g = (torch.randperm(n, generator=gen) + 1).to(torch.int32)
+    buffers = SimpleNamespace(fgidx_to_gidx=f2g.to(cuda), device_counts=torch.tensor([1500, 0, 0, 0], dtype=torch.int32, device=cuda))
+    got = table.gradient(SimpleNamespace(sh_coeffs_grads=grads), buffers)
+    want, bound = gradient_exact(grads.cpu(), table.indices.cpu(), rows, 0.5, f2g, 1500)
+    assert ((got.cpu().double().view(rows, -1) - want).abs() <= bound).all()
+
+
 def test_table_trainer_runs(cuda):
     from gs3d.training import TableTrainer, TrainingOptions
     g, table, cams, targets, ro, til = table_scene(cuda)

@@ -276,9 +276,12 @@ class SHTable:
     def gradient(self, fgradients, buffers, out: torch.Tensor | None = None, accumulate: bool = False,
                  stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """Gradient of `coeffs` from the SH gradients of backward() (FilteredGaussiansGradients and
-        the RenderBuffers of its render)."""
-        return table_gradient(fgradients.sh_coeffs_grads, self.indices, self.rows, self.scale, out,
-                              accumulate, buffers.fgidx_to_gidx, buffers.device_counts, stream)
+        the RenderBuffers of its render). backward() leaves the coefficients above the render's SH degree as
+        they were (zeros in fresh buffers), and so their sums. Gradient buffers may hold more Gaussians than
+        the render's; their further rows belong to none."""
+        grads, f2g = fgradients.sh_coeffs_grads, buffers.fgidx_to_gidx
+        return table_gradient(grads[:f2g.shape[0]], self.indices, self.rows, self.scale, out, accumulate, f2g,
+                              buffers.device_counts, stream)
 
     def to(self, device) -> "SHTable":
         return SHTable(self.coeffs.to(device), self.indices.to(device), self.scale)

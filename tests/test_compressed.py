@@ -307,6 +307,18 @@ def test_calls_need_cuda_tensors_of_the_right_kind():
         gc.fit_table(torch.zeros(4, 3, 16), 0)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_fit_table_refuses_what_has_no_mean(bad):
+    """One coefficient that is not finite would make its row's mean NaN, the nearest row of every Gaussian
+    after that, and so the whole table."""
+    sh = torch.randn(50, 3, 4, generator=torch.Generator().manual_seed(1))
+    sh[7, 1, 2] = bad
+    with pytest.raises(ValueError, match="finite"):
+        gc.fit_table(sh, 5)
+    with pytest.raises(ValueError, match="float32"):
+        gc.fit_table(sh.half(), 5)
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("table", [False, True])
 def test_compressed_model_file_round_trip(tmp_path, fmt, table):

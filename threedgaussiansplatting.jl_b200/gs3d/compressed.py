@@ -288,13 +288,15 @@ class SHTable:
 
 
 def fit_table(sh_coeffs: torch.Tensor, nb_rows: int, iterations: int = 10, seed: int = 0) -> SHTable:
-    """A table of (at most) `nb_rows` rows for `sh_coeffs` ((n, 3, order) float32 on a CUDA device)
+    """A table of (at most) `nb_rows` rows for `sh_coeffs` ((n, 3, order) finite float32 on a CUDA device)
     by Lloyd's algorithm: rows start as a random choice of the Gaussians' coefficients, then every
     Gaussian takes its nearest row and every row the mean of its Gaussians (rows without any keep
     their value). A one-off preparation: the distances are torch products, in chunks."""
     n = sh_coeffs.shape[0]
     if n < 1 or nb_rows < 1:
         raise ValueError(f"a table of {nb_rows} rows for {n} Gaussians")
+    if sh_coeffs.dtype != torch.float32 or not bool(torch.isfinite(sh_coeffs).all()):
+        raise ValueError("the coefficients must be finite float32 values")
     x = sh_coeffs.reshape(n, -1)
     gen = torch.Generator().manual_seed(int(seed))
     pick = torch.randperm(n, generator=gen)[:nb_rows].to(x.device)

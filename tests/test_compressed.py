@@ -346,3 +346,25 @@ def test_compressed_model_file_refusals(tmp_path):
         io.load_compressed(tmp_path / "x.npz")
     with pytest.raises(ValueError, match="npz"):
         scripts.compress(tmp_path / "m.ply", tmp_path / "m.ply", device="cpu")
+
+
+def test_a_table_trainer_holds_no_moments_of_the_gaussians_own_coefficients(monkeypatch):
+    """Its optimizers are the geometry's and the table's: nothing of n x 48 moments, nor statistics for a
+    densification that never happens, is allocated on the way there."""
+    from gs3d import training
+    from gs3d.optimizer import AdamMoments
+    from gs3d.scene import SceneSpec, look_at_camera, synthetic_gaussians
+    g = synthetic_gaussians(SceneSpec(20, "uniform:1", -3.5, 0.4), 2)
+    cam = look_at_camera(96, 64, 60.0, (0, 0.4, 2.5))
+    args = (g, gc.SHTable(torch.zeros(4, 3, 16), torch.ones(20, dtype=torch.int32)), [cam], [torch.rand(96, 64, 3)],
+            training.RenderOptions.for_camera(cam, 3), training.Tiling.for_camera(cam),
+            training.TrainingOptions(scene_radius=2.5))
+    made, zeros = [], AdamMoments.zeros
+    monkeypatch.setattr(AdamMoments, "zeros", lambda n, degree, device: made.append((n, degree)) or zeros(n, degree, device))
+    monkeypatch.setattr(training.adc_mod.AdcBuffers, "create", lambda *a: pytest.fail("statistics"))
+    tr = training.TableTrainer(*args)
+    assert made == [(20, 0), (4, 3)]
+    assert tr.optimizer.moments.n == 20 and tr.table_optimizer.moments.n == 4 and not tr.rebuild_sh_grads
+    with pytest.raises(ValueError, match="rebuild_sh_grads"):
+        training.TableTrainer(*args, rebuild_sh_grads=True)
+    assert not training.TableTrainer(*args, rebuild_sh_grads=False).rebuild_sh_grads

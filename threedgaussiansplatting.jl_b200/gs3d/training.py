@@ -141,8 +141,7 @@ class Trainer:
         self._next_orders = []
         self.loss = LossComputer(self.width, self.height, dev, options.loss_dssim_vs_L1_weight)
         self.fgradients = FilteredGaussiansGradients.create(gaussians.n, gaussians.sh_degree, dev)
-        self.optimizer = AdamOptimizer(gaussians, options.learning_rates())
-        self.adc_buffers = adc_mod.AdcBuffers.create(gaussians.n, dev)
+        self._create_optimizer()
         self.iteration_nb = 0
         self.rng = np.random.default_rng(seed)
         self.cameras_order = self.rng.permutation(len(cameras))
@@ -152,6 +151,11 @@ class Trainer:
         # False: renders never block; a duplicate-key overflow is flagged in
         # render_buffers.device_counts[2] instead of growing the buffers
         self.render_host_sync = True
+
+    def _create_optimizer(self) -> None:
+        """The optimizer with its moments, and the statistics that densification needs."""
+        self.optimizer = AdamOptimizer(self.gaussians, self.options.learning_rates())
+        self.adc_buffers = adc_mod.AdcBuffers.create(self.gaussians.n, self.device)
 
     # -- schedule pieces (training.jl:253-302) ---------------------------------------------
     def current_camera_index(self) -> int:
@@ -340,23 +344,29 @@ class TableTrainer(Trainer):
         if coeffs.shape[1:] != gaussians.sh_coeffs.shape[1:] or sh_table.indices.shape[0] != gaussians.n:
             raise ValueError(f"a table of {tuple(coeffs.shape)} with {sh_table.indices.shape[0]} indices for "
                              f"SH coefficients of {tuple(gaussians.sh_coeffs.shape)}")
+        if kwargs.pop("rebuild_sh_grads", False):
+            raise ValueError("rebuild_sh_grads: a table's gradient needs the SH gradients that it leaves out")
+        self.sh_table = sh_table
         super().__init__(gaussians, cameras, targets, render_options, tiling, options,
                          rebuild_sh_grads=False, **kwargs)
-        self.sh_table = sh_table
-        dev, n, rows = self.device, gaussians.n, sh_table.rows
-        # the geometry's optimizer: the Gaussians without coefficients (SH degree 0, zero gradients)
+
+    def _create_optimizer(self) -> None:
+        """One optimizer for the geometry and one for the table; no statistics, since nothing is densified."""
+        g, table, dev = self.gaussians, self.sh_table, self.device
+        n, rows = g.n, table.rows
+        # the geometry's: the Gaussians without coefficients (SH degree 0, zero gradients)
         bare = torch.zeros((n, 3, 1), dtype=torch.float32, device=dev)
-        self.optimizer = AdamOptimizer(GaussiansVector(*gaussians.tensors()[:3], bare),
-                                       options.learning_rates())
+        self.optimizer = AdamOptimizer(GaussiansVector(*g.tensors()[:3], bare), self.options.learning_rates())
         self._geometry_gradients = FilteredGaussiansGradients(
             **{**self.fgradients.__dict__, "sh_coeffs_grads": torch.zeros_like(bare)})
         # the table's: as many Gaussians as it has rows, without geometry gradients, all of them updated
         zeros = lambda k: torch.zeros((rows, k), dtype=torch.float32, device=dev)  # noqa: E731
-        self.table_optimizer = AdamOptimizer(GaussiansVector(zeros(4), zeros(3), zeros(4), coeffs),
-                                             options.learning_rates())
-        self._table_gradients = FilteredGaussiansGradients.create(rows, gaussians.sh_degree, dev)
+        self.table_optimizer = AdamOptimizer(GaussiansVector(zeros(4), zeros(3), zeros(4), table.coeffs),
+                                             self.options.learning_rates())
+        self._table_gradients = FilteredGaussiansGradients.create(rows, g.sh_degree, dev)
         self._table_rows = torch.arange(1, rows + 1, dtype=torch.int32, device=dev)
         self._table_counts = torch.tensor([rows, 0, 0, 0], dtype=torch.int32, device=dev)
+        self.adc_buffers = None
 
     def maybe_increase_sh_degree(self) -> None:
         pass

@@ -313,6 +313,21 @@ def test_gradient_strides_and_accumulation(cuda, kind, dim, stride, out_stride, 
     assert (out[12] == 0).all()
 
 
+@pytest.mark.parametrize("n", [3000, 100_000])
+def test_gradient_into_a_large_table_with_rows_apart(cuda, n):
+    """The table's rows are zeroed element by element, over several turns of the blocks that do it."""
+    gen = rng(n)
+    rows, dim, stride, offset = 120_000, 27, 29, 1
+    grads = torch.randn(n, dim, generator=gen)
+    idx = make_indices(n, rows, gen, 2.0)
+    buf = torch.full((rows * stride + offset,), 5.0, device=cuda)
+    out = torch.as_strided(buf, (rows, dim), (stride, 1), offset)
+    gc.table_gradient(grads.to(cuda), idx.to(cuda), rows, out=out)
+    want, bound = gradient_exact(grads, idx, rows, 1.0)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    assert (torch.as_strided(buf, (rows - 1, stride - dim), (stride, 1), offset + dim) == 5.0).all() and float(buf[0]) == 5.0
+
+
 def test_gradient_edges(cuda):
     idx = torch.ones(4, dtype=torch.int32, device=cuda)
     g = torch.ones(4, 3, device=cuda)
@@ -508,6 +523,18 @@ def test_tensor_scale(cuda, kind, n):
         flat[(at + 77) % flat.shape[0]] = 0.0
 
 
+@pytest.mark.parametrize("kind", TYPES)
+def test_tensor_scale_is_the_quotient_up_to_its_two_roundings(cuda, kind):
+    """The definition is largest / 2688; the reciprocal of 2688 and the product with it round by at most
+    2^-24 each: within (1 + 2^-24)^2 - 1 of the quotient."""
+    gen = rng(9)
+    for k in range(-12, 13):
+        x = (torch.randn(9, 48, generator=gen) * 2.0 ** k).to(kind)
+        top = x.double().abs().max()
+        got = gc.mx4_tensor_scale(x.to(cuda)).cpu().double()
+        assert float((got * 2688 - top).abs()) <= ((1 + 2.0 ** -24) ** 2 - 1) * float(top)
+
+
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
 def test_quantise_ratios_of_small_numbers(cuda, kind):
     """16-bit elements and a power-of-two maximum: quotients that meet the borders exactly."""
@@ -556,6 +583,29 @@ def test_quantise_strides(cuda, kind, dim, stride, offset):
         want = torch.full_like(out, 9.0)
         torch.as_strided(want, (n, dim), (stride, 1), offset).copy_(gc.mx4_dequantise(b, kind))
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+def test_quantise_strides_of_many_rows(cuda, kind, fmt):
+    """Rows apart and misaligned, more of them than the element-by-element kernels' grids hold at once:
+    600K (or 400K) blocks and 9.6M elements for 303K threads, and a tensor scale of many blocks."""
+    n, dim, stride, offset = 200_000, 48, 49, 1
+    buf = (torch.randn(n * stride + offset, generator=rng(14)) * 0.1).to(kind).to(cuda)
+    x = torch.as_strided(buf, (n, dim), (stride, 1), offset)
+    x[n - 2, 5] = -7.0  # the largest magnitude, in the last turn
+    buf[stride * 5 : stride * 5 + 1] = 100.0  # between the rows: not part of them
+    plain = x.contiguous()
+    if fmt == "nvfp4":
+        assert torch.equal(gc.mx4_tensor_scale(x), gc.mx4_tensor_scale(plain))
+        assert float(gc.mx4_tensor_scale(x)) == float(np.float32(7.0) * (np.float32(1) / np.float32(2688)))
+    a, b = gc.mx4_quantise(x, fmt), gc.mx4_quantise(plain, fmt)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    out = torch.full((n * stride + offset,), 9.0, dtype=kind, device=cuda)
+    gc.mx4_dequantise(a, out=torch.as_strided(out, (n, dim), (stride, 1), offset))
+    want = torch.full_like(out, 9.0)
+    torch.as_strided(want, (n, dim), (stride, 1), offset).copy_(gc.mx4_dequantise(b, kind))
+    assert torch.equal(out, want)
 
 
 def test_quantise_empty(cuda):
@@ -855,6 +905,45 @@ def test_fit_table(cuda):
     rows = table.expand()
     assert table.coeffs.shape == (2, 3, 4) and float((rows - sh).abs().max()) < 0.2
     assert gc.fit_table(sh[:3], 10).rows == 3
+
+
+def test_fit_table_rows_are_their_members_means(cuda):
+    """Of separated clusters, where one more iteration changes nothing: a row is the mean of its m members
+    within (m + 2) u mean|x| (m - 1 roundings of the sum, one of the quotient)."""
+    gen = rng(7)
+    which = torch.randint(0, 5, (4001,), generator=gen)
+    centre = torch.eye(5).repeat_interleave(3, dim=1)[:, :12] * 4 - 2
+    sh = (centre[which] + 0.05 * torch.randn(4001, 12, generator=gen)).view(-1, 3, 4)
+    table = gc.fit_table(sh.to(cuda), 60, iterations=100, seed=2)
+    again = gc.fit_table(sh.to(cuda), 60, iterations=101, seed=2)
+    assert torch.equal(table.indices, again.indices) and torch.equal(table.coeffs, again.coeffs)
+    x, c, i = sh.double().view(-1, 12), table.coeffs.cpu().double().view(60, 12), table.indices.cpu().long() - 1
+    for k in i.unique().tolist():
+        mine = x[i == k]
+        bound = (len(mine) + 2) * U * mine.abs().mean(dim=0)
+        assert ((c[k] - mine.mean(dim=0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("iterations", [1, 3])
+def test_fit_table_takes_the_nearest_row(cuda, iterations):
+    """The comparison is of |c|^2 / 2 - <x, c> in fp32: d products and sums a side, so that a row may be taken
+    whose value is above the least by 2 (d + 2) u (|c|^2 / 2 + |x| |c|) at most."""
+    x = torch.randn(3000, 27, generator=rng(5))
+    table = gc.fit_table(x.view(-1, 3, 9).to(cuda), 50, iterations=iterations, seed=1)
+    c, x = table.coeffs.cpu().double().view(50, 27), x.double()
+    value = 0.5 * (c * c).sum(dim=1) - x @ c.t()
+    size = float(0.5 * (c * c).sum(dim=1).max() + x.norm(dim=1).max() * c.norm(dim=1).max())
+    mine = value.gather(1, table.indices.cpu().long()[:, None] - 1)[:, 0]
+    assert ((mine - value.min(dim=1).values) <= 2 * (27 + 2) * U * size).all()
+
+
+def test_fit_table_rows_without_members(cuda):
+    """Two values among 40 Gaussians and ten rows: eight rows end without members and keep what they had."""
+    sh = torch.tensor([[1.0] * 12, [-0.5] * 12])[torch.arange(40) % 2].view(40, 3, 4).to(cuda)
+    table = gc.fit_table(sh, 10, iterations=4, seed=3)
+    assert table.rows == 10 and len(table.indices.unique()) == 2
+    assert torch.equal(table.expand(), sh)
+    assert ((table.coeffs == 1.0) | (table.coeffs == -0.5)).all()
 
 
 # -- training and scripts ---------------------------------------------------------------------------

@@ -581,7 +581,8 @@ GS3D_API int gs3d_table_gradient_workspace_size(int64_t grad_rows, int64_t table
  *     outside 1 .. n_indices are skipped).
  * device_counts != NULL: only the first device_counts[0] rows take part (read on the device,
  * clamped to grads->rows); the others are not read. Indices outside 1 .. table_grads->rows are
- * skipped. table_grads is GS3D_F32. The workspace (256-byte aligned) is scratch for this call. */
+ * skipped. table_grads is GS3D_F32 and overlaps no input. The workspace (256-byte aligned) is scratch
+ * for this call. */
 GS3D_API int gs3d_table_gradient(const gs3d_rows* grads, const int32_t* indices, int64_t n_indices,
                                  const int32_t* fgidx_to_gidx, const int32_t* device_counts,
                                  float scale, const gs3d_rows* table_grads, uint32_t flags,
@@ -622,7 +623,7 @@ GS3D_API int gs3d_mx4_tensor_scale(const gs3d_rows* x, float* tensor_scale, gs3d
  * value again). */
 GS3D_API int gs3d_mx4_quantise(const gs3d_rows* x, const gs3d_mx4_rows* out, gs3d_stream_t stream);
 
-/* out = the values x stands for, rounded to out's type (same rows and dim). */
+/* out = the values x stands for, rounded to out's type (same rows and dim; apart from x's arrays). */
 GS3D_API int gs3d_mx4_dequantise(const gs3d_mx4_rows* x, const gs3d_rows* out, gs3d_stream_t stream);
 
 /* The colours of n Gaussians from 4-bit SH rows, seen from n_views cameras (view_positions: HOST

@@ -144,6 +144,30 @@ def test_colour_refusals():
     assert call(n=0, means=None, out=None, stride=0) == _abi.GS3D_OK
 
 
+def covers(n, dim, stride, elem, at):
+    return {at + elem * (r * stride) + b for r in range(n) for b in range(elem * dim)}
+
+
+def test_results_over_inputs_are_refused():
+    """A lookup into its own table and a gradient into its own gradients would read what other threads have
+    written. Rows that lie between one another's are fine; where both have gaps and their strides differ,
+    ranges that meet are left to the caller."""
+    bf, f32 = _abi.GS3D_BF16, _abi.GS3D_F32
+    elem = {bf: 2, f32: 4}
+    shapes = [(6, 5, 5, f32), (6, 5, 13, f32), (3, 4, 16, f32), (1, 7, 7, bf), (9, 3, 26, bf), (4, 10, 10, bf), (0, 5, 5, f32)]
+    kept = 0
+    for x in shapes:
+        for y in shapes:
+            for at in range(-330, 331, 6):
+                meet = bool(covers(*x[:3], elem[x[3]], 0) & covers(*y[:3], elem[y[3]], at))
+                gap_free = any(r[0] == 1 or r[1] == r[2] for r in (x, y))
+                known = gap_free or x[2] * elem[x[3]] == y[2] * elem[y[3]]
+                got = gc._rows_meet(gc._row_bytes(rows(*x, DATA)), gc._row_bytes(rows(*y, DATA + at)))
+                assert got == (meet and known), (x, y, at)
+                kept += meet and known
+    assert kept > 500
+
+
 def test_misaligned_words_are_refused():
     pos = (C.c_float * 3)()
     r, out, q = rows(), rows(), mx4()

@@ -352,6 +352,27 @@ def test_gradient_edges(cuda):
         gc.table_gradient(g, idx[:3], 3)
 
 
+def test_results_over_inputs(cuda):
+    """Refused; beside one another's rows in one buffer they are what they are elsewhere."""
+    gen = rng(31)
+    buf = torch.randn(400, 96, generator=gen).to(cuda)
+    table, idx = buf[:, :48], make_indices(400, 400, gen).to(cuda)
+    want = gc.table_lookup(table, idx, scale=2.0)
+    want_grad = gc.table_gradient(table, idx, 400)
+    for out in (table, buf[:, 20:68], buf[:200].view(400, 48)):
+        with pytest.raises(ValueError, match="overlap"):
+            gc.table_lookup(table, idx, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            gc.table_gradient(table, idx, 400, out=out)
+    assert torch.equal(gc.table_lookup(table, idx, scale=2.0, out=buf[:, 48:]), want) and torch.equal(buf[:, 48:], want)
+    gc.table_gradient(table, idx, 400, out=buf[:, 48:])
+    assert torch.equal(buf[:, 48:], want_grad)
+    q = gc.mx4_quantise(table, "mxfp4")
+    inside = q.codes.view(-1)[: 24 * 4 * 20].view(torch.float32).view(10, 48)
+    with pytest.raises(ValueError, match="overlap"):
+        gc.mx4_dequantise(MX4Rows(q.codes[:10], q.scales[:10], None, 48, "mxfp4"), out=inside)
+
+
 def test_gradient_is_the_lookups(cuda):
     """<d_out, lookup(table + h v)> differences: the lookup is linear in the table, so with values that
     fp32 holds exactly the difference quotient equals <gradient, v> exactly."""

@@ -53,6 +53,37 @@ def _rows_c(t: torch.Tensor, what: str) -> _abi.RowsC:
     return _abi.RowsC(rows, stride, dim, kind, t.data_ptr())
 
 
+def _row_bytes(r: _abi.RowsC) -> tuple[int, int, int, int]:
+    """First byte, byte behind the last, stride and length of the rows (of rows without gaps: one row)."""
+    e = 4 if r.type == _abi.GS3D_F32 else 2
+    begin, stride, size = r.data or 0, r.row_stride * e, r.dim * e
+    end = begin + (r.rows - 1) * stride + size if r.rows > 0 else begin
+    if r.rows > 1 and stride == size:
+        stride = size = end - begin
+    return begin, end, stride, size
+
+
+def _rows_meet(a: tuple[int, int, int, int], b: tuple[int, int, int, int]) -> bool:
+    """Whether rows (of _row_bytes) are known to share bytes: exactly, but for rows with gaps of
+    different strides, which may lie between one another's."""
+    (a0, a1, sa, la), (b0, b1, sb, lb) = a, b
+    if a0 == a1 or b0 == b1 or a0 >= b1 or b0 >= a1:
+        return False
+    if a1 - a0 == la:  # a is one range: the first row of b that ends behind its start
+        return b0 + max(0, -((b0 + lb - 1 - a0) // sb)) * sb < a1
+    if b1 - b0 == lb:
+        return a0 + max(0, -((a0 + la - 1 - b0) // sa)) * sa < b1
+    if sa != sb:
+        return False
+    d = (b0 - a0) % sa
+    return d < la or sa - d < lb
+
+
+def _check_apart(out: _abi.RowsC, x: tuple[int, int, int, int], what: str) -> None:
+    if _rows_meet(_row_bytes(out), x):
+        raise ValueError(f"out overlaps {what}")
+
+
 def _check_device(first: torch.Tensor, *others) -> torch.device:
     device = first.device
     if device.type != "cuda":
@@ -103,18 +134,22 @@ def table_lookup(table: torch.Tensor, indices: torch.Tensor, scale: float = 1.0,
                  stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """out[i] = scale * table[indices[i] - 1]: the rows of `table` ((rows, ...), float32, float16 or
     bfloat16) for 1-based int32 `indices`; an index outside 1 .. rows gives zeros. Products are
-    fp32, rounded once to `dtype` (default: the table's). `out` ((n, ...)) is filled in place."""
+    fp32, rounded once to `dtype` (default: the table's). `out` ((n, ...), apart from the table) is
+    filled in place."""
     _check_indices(indices)
     device = _check_device(table, indices, out)
     t = _rows_c(table, "table")
     shape = (indices.shape[0], *table.shape[1:])
     handle, context = _enter(device, stream)
     try:
-        if out is None:
+        given = out is not None
+        if not given:
             out = table.new_empty(shape, dtype=dtype)
         elif out.shape != shape or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a lookup of {shape} {dtype or out.dtype}")
         o = _rows_c(out, "out")
+        if given:
+            _check_apart(o, _row_bytes(t), "the table")
         _abi.check(_abi.lib().gs3d_table_lookup(t, indices.data_ptr(), scale, o, handle))
     finally:
         _leave(context)
@@ -130,7 +165,8 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
     of grads[f] over the rows f with index k + 1, summed in an order fixed by the indices.
     `fgidx_to_gidx`: row f of `grads` belongs to filtered Gaussian f (as in
     FilteredGaussiansGradients.sh_coeffs_grads) and has index indices[fgidx_to_gidx[f] - 1];
-    `device_counts`: only the first device_counts[0] rows take part. `accumulate`: add to `out`."""
+    `device_counts`: only the first device_counts[0] rows take part. `accumulate`: add to `out`
+    (apart from `grads`)."""
     _check_indices(indices)
     _check_indices(fgidx_to_gidx, "fgidx_to_gidx")
     device = _check_device(grads, indices, fgidx_to_gidx, device_counts, out)
@@ -144,11 +180,14 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
     shape = (int(nb_rows), *grads.shape[1:])
     handle, context = _enter(device, stream)
     try:
-        if out is None:
+        given = out is not None
+        if not given:
             out = grads.new_empty(shape, dtype=torch.float32)
         elif out.shape != shape or out.dtype != torch.float32:
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} for a float32 table gradient of {shape}")
         o = _rows_c(out, "out")
+        if given:
+            _check_apart(o, _row_bytes(g), "grads")
         nbytes = _gradient_workspace_bytes(g.rows, o.rows, g.dim)
         ws = grads.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _abi.check(_abi.lib().gs3d_table_gradient(
@@ -207,9 +246,15 @@ def mx4_dequantise(rows: MX4Rows, dtype: torch.dtype = torch.float32, out: torch
     device = _check_device(rows.codes, out)
     handle, context = _enter(device, stream)
     try:
-        if out is None:
+        given = out is not None
+        if not given:
             out = rows.codes.new_empty((rows.rows, rows.dim), dtype=dtype)
-        _abi.check(_abi.lib().gs3d_mx4_dequantise(rows.to_c(), _rows_c(out, "out"), handle))
+        o = _rows_c(out, "out")
+        if given:
+            for t, what in ((rows.codes, "the codes"), (rows.scales, "the scales")):
+                begin, size = t.data_ptr(), t.numel()
+                _check_apart(o, (begin, begin + size, size, size), what)
+        _abi.check(_abi.lib().gs3d_mx4_dequantise(rows.to_c(), o, handle))
     finally:
         _leave(context)
     return out

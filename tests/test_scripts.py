@@ -112,3 +112,22 @@ def test_annealed_means_lr_degenerate_step_counts():
     assert annealed_means_lr(5, one) == pytest.approx(one.final_means_lr, rel=1e-6)
     zero = TrainingOptions(scene_radius=1.0, nb_lr_annealing_steps=0)   # x clamps to 0
     assert annealed_means_lr(9, zero) == pytest.approx(zero.initial_means_lr, rel=1e-6)
+
+
+def test_evaluate_takes_a_trainer_without_prepare_model(monkeypatch):
+    """What evaluate() reads of a trainer is its model, camera size, options and buffers; bringing the
+    model up to date first is for trainers that have something to do there."""
+    from types import SimpleNamespace
+
+    from gs3d import loss
+    rgb = torch.full((3, 2, 3), 0.25)
+    state = dict(width=3, height=2, options=SimpleNamespace(loss_dssim_vs_L1_weight=0.2), gaussians=None, tiling=None,
+                 render_options=None, render_buffers=None, render_outputs=SimpleNamespace(rgb=rgb))
+    monkeypatch.setattr(scripts, "gs_render", lambda *a, **k: None)
+    monkeypatch.setattr(loss, "LossComputer", lambda *a: lambda x, y, s: torch.tensor([0.0, 0.5, 0.125, 0.0]))
+    want = {"mse": 0.25, "mae": 0.5, "dssim": 0.125}
+    args = ([None], [torch.full((3, 2, 3), 0.75)], "cpu")
+    assert scripts.evaluate(SimpleNamespace(**state), *args) == want
+    prepared = []
+    assert scripts.evaluate(SimpleNamespace(**state, prepare_model=lambda: prepared.append(1)), *args) == want
+    assert prepared == [1]

@@ -113,7 +113,8 @@ def evaluate(trainer, cameras, images, device) -> dict[str, float] | None:
     from .loss import LossComputer
     w, h = trainer.width, trainer.height
     lc = LossComputer(w, h, device, trainer.options.loss_dssim_vs_L1_weight)
-    trainer.prepare_model()
+    if hasattr(trainer, "prepare_model"):
+        trainer.prepare_model()
     scratch = torch.empty((w, h, 3), dtype=torch.float32, device=device)
     mse = mae = dssim = 0.0
     for cam, img in zip(cameras, images):

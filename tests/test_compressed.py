@@ -267,6 +267,20 @@ def test_compressed_gaussians_checks():
             CompressedGaussiansVector(*bad)
 
 
+def test_compressed_gaussians_are_checked_again_before_a_render():
+    """The fields can be assigned: what a kernel would follow or misread does not get there."""
+    make = lambda: CompressedGaussiansVector(torch.zeros(6, 4), torch.zeros(6, 6),  # noqa: E731
+                                             MX4Rows.empty(6, 48, "mxfp4", "cpu"), torch.ones(6, dtype=torch.int32))
+    assert make().to_c().n == 6
+    for name, value in (("indices", torch.ones(6, dtype=torch.int64)), ("indices", torch.ones(5, dtype=torch.int32)),
+                        ("indices", torch.ones(6, dtype=torch.int32, device="meta")), ("means_opacities", torch.zeros(7, 4)),
+                        ("covariances", torch.zeros(6, 6, device="meta")), ("sh", MX4Rows.empty(6, 47, "mxfp4", "cpu"))):
+        g = make()
+        setattr(g, name, value)
+        with pytest.raises(ValueError):
+            g.to_c()
+
+
 def test_rows_of_a_tensor():
     t = torch.zeros(5, 3, 16)
     assert (lambda c: (c.rows, c.row_stride, c.dim, c.type))(gc._rows_c(t, "t")) == (5, 48, 48, _abi.GS3D_F32)

@@ -507,6 +507,7 @@ class CompressedGaussiansVector:
             None if self.indices is None else self.indices.to(device))
 
     def to_c(self) -> _abi.RenderOnlyGaussiansC:
+        self.__post_init__()  # again: the fields can be assigned
         return _abi.RenderOnlyGaussiansC(self.n, self.sh_degree, _ptr(self.means_opacities),
                                          _ptr(self.covariances), None)
 

@@ -33,8 +33,9 @@ __device__ __forceinline__ float mx4_scale(uint32_t byte) {
 
 // Elements as fp16, times 2^-14: exponent and mantissa bits at bits 11..9 (the element's subnormal is
 // then fp16's), the sign at bit 15. By integer operations: the hardware's conversion from e2m1x2 is
-// shorter, but nvcc 12.9 returned wrong elements for it wherever the byte came from a 16- or 8-bit load
-// or from a shift that depends on the thread.
+// shorter, but as nvcc 12.9 compiles it the elements are wrong (for 252 of the 256 bytes) where its byte
+// comes straight from an 8-bit load through __ldg or from shared memory, as some of the uses here do; from
+// 16- and 32-bit words, shifted or joined, they are right.
 // The two elements of a byte:
 __device__ __forceinline__ __half2 e2m1_pair_half(uint32_t byte) {
     const uint32_t h = ((byte << 9) & 0x0e00u) | ((byte << 12) & 0x8000u) | ((byte << 21) & 0x0e000000u) |

@@ -637,7 +637,8 @@ __device__ __forceinline__ void sum_chunk(const T* __restrict__ grads, int strid
                                           bool open_left, bool open_right, float* __restrict__ partial) {
     using Unit = RowUnit<T, VB>;
     // rows in flight a slot (1.2M x 119 bf16, an element a thread: 8 / 12 / 16 rows 53 / 46 / 41 us; 1M x 27
-    // fp32: 54 / 55 / 58)
+    // fp32: 54 / 55 / 58). In k_table_segments the half types then spill 12 to 44 bytes of their 48 or 64
+    // registers a thread, fp32 none.
     constexpr int N = Unit::N, AHEAD = VB == 16 ? 6 : (VB < 8 && sizeof(T) == 2 ? 16 : 8);
     const int slot = threadIdx.x / pl.tile_units, lane = threadIdx.x - slot * pl.tile_units;
     const int unit = blockIdx.y * pl.tile_units + lane;
@@ -869,10 +870,11 @@ struct GradLayout {
     int ntiles, passes, bits, chunks_max;
 };
 
-// Rows a slot adds: enough blocks for few rows, few borders for many (3M x 48 fp32: 32 / 48 / 96 rows 197 /
-// 194 / 196 us; 500K x 27 bf16: 39.6 / 37.4 / 41.5), and more for long rows, of which a block has few
-// slots, so that some 16 chunks an SM are left to join (1.2M x 119 bf16, 52 rows of which few are much
-// used: 198 us in all with 48 rows a slot and a join of 256 columns a block, 67 so).
+// Rows a slot adds: enough blocks for few rows, few borders for many (500K x 27 bf16 of which 300K take part,
+// 32 / 48 / 94 rows: 34.8 / 32.2 / 37.1 us a call), and more for many or long rows, of which a block has few
+// slots, so that at most some 16 chunks an SM are left to join (1.2M x 119 bf16, 52 rows of which few are much
+// used: 198 us in all with 48 rows a slot and a join of 256 columns a block, 67 so). 3M x 48 fp32 hardly
+// depends on it: 61 rows by that rule 194.8 us a call, with 32 / 48 / 96 rows 194.0 / 192.1 / 193.4.
 constexpr int kMinRun = 4, kMaxRun = 48, kMaxChunk = 2048;
 
 // Bytes of a row that a thread reads at once: 16 where the rows allow it, else 8, 4 or an element.

@@ -204,7 +204,8 @@ def table_gradient(grads: torch.Tensor, indices: torch.Tensor, nb_rows: int, sca
 # -- 4-bit rows -------------------------------------------------------------------------------
 def mx4_tensor_scale(x: torch.Tensor, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """(1,) float32: max(largest finite |x| * (1 / 2688), 2^-100), reciprocal and product in float32: the
-    nvfp4 tensor scale with which the block scales of `x` ((rows, ...)) use their range."""
+    nvfp4 tensor scale with which the block scales of `x` ((rows, ...)) use their range. At most one unit in
+    the last place from the quotient by 2688 rounded once."""
     device = _check_device(x)
     c = _rows_c(x, "x")
     handle, context = _enter(device, stream)

@@ -613,7 +613,7 @@ typedef struct gs3d_mx4_rows {
 /* tensor_scale[0] = max(largest finite |x| * (1 / 2688), 2^-100), 2688 = 6 * 448, the reciprocal and the
  * product in fp32: the GS3D_NVFP4 tensor scale with which the block scales of x use their range. That is
  * the fp32 number nearest to the quotient by 2688 for some 77 % of all x and its neighbour for the others;
- * gs3d_mx4_quantise takes any scale, for callers that want the quotient itself. */
+ * gs3d_mx4_quantise takes any scale of the range above, the quotient rounded once among them. */
 GS3D_API int gs3d_mx4_tensor_scale(const gs3d_rows* x, float* tensor_scale, gs3d_stream_t stream);
 
 /* Quantise x into `out` (same rows and dim). Per block with largest magnitude a: GS3D_NVFP4 block

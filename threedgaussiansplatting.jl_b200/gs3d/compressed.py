@@ -221,7 +221,7 @@ def mx4_quantise(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Ten
                  stream: torch.cuda.Stream | None = None) -> MX4Rows:
     """The rows of `x` ((rows, ...), float32, float16 or bfloat16) as 4-bit elements with block
     scales (gs3d_mx4_quantise). `tensor_scale` (nvfp4): (1,) float32 on the device, from 2^-100 to
-    the largest float32 / 2688; None: mx4_tensor_scale(x)."""
+    the largest float32 / 2688, which the rows keep (not a copy); None: mx4_tensor_scale(x)."""
     device = _check_device(x, tensor_scale)
     c = _rows_c(x, "x")
     handle, context = _enter(device, stream)
@@ -322,9 +322,9 @@ class SHTable:
     def gradient(self, fgradients, buffers, out: torch.Tensor | None = None, accumulate: bool = False,
                  stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """Gradient of `coeffs` from the SH gradients of backward() (FilteredGaussiansGradients and
-        the RenderBuffers of its render). backward() leaves the coefficients above the render's SH degree as
-        they were (zeros in fresh buffers), and so their sums. Gradient buffers may hold more Gaussians than
-        the render's; their further rows belong to none."""
+        the RenderBuffers of its render). Above the render's SH degree backward() leaves the gradients as they
+        were (zeros in fresh buffers), and those are what is summed there. Gradient buffers may hold more
+        Gaussians than the render's; their further rows belong to none."""
         grads, f2g = fgradients.sh_coeffs_grads, buffers.fgidx_to_gidx
         return table_gradient(grads[:f2g.shape[0]], self.indices, self.rows, self.scale, out, accumulate, f2g,
                               buffers.device_counts, stream)
